@@ -89,6 +89,16 @@ class DeviceArray:
     def contiguous(self) -> "DeviceArray":
         return self
 
+    def is_contiguous(self) -> bool:
+        return True
+
+    def stride(self) -> tuple:
+        st, n = [], 1
+        for s in reversed(self.shape):
+            st.append(n)
+            n *= max(s, 1)
+        return tuple(reversed(st))
+
     def _view(self, shape, offset_bytes: int = 0) -> "DeviceArray":
         return DeviceArray(shape, self.dtype, self._ptr + offset_bytes, self._base or self)
 
@@ -248,6 +258,12 @@ def stream():
     if torch is not None:
         return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
     return None
+
+
+def raw_stream(device: int):
+    """:func:`stream` as a plain number (the current stream of ``device``), for the calls whose
+    host time counts."""
+    return torch._C._cuda_getCurrentRawStream(device) if torch is not None else None
 
 
 def upload(a):

@@ -8,6 +8,10 @@ reference's exception types: ``ValueError`` for GQA/shape mismatches and a
 quantised conv without a kernel size, ``IndexError`` for embedding ids outside
 the table.  There is no CPU path; without the library or a GPU they raise.
 
+The paged-cache and beam-search operators (``paged_extend``, ``paged_append``,
+``paged_attention``, ``beam_select``, ``paged_reorder``; :mod:`.paged`) have no
+counterpart there and take device arrays only.
+
 Constant tables (Hann window, linear-interpolation positions) are built on the
 host in float64 exactly as the reference builds them, then used on the device.
 """
@@ -21,6 +25,8 @@ import numpy as np
 
 from . import _dev as D
 from ._lib import call
+from .paged import (BeamStep, PagedStep, beam_select, paged_append, paged_attention, paged_extend,  # noqa: F401
+                    paged_reorder)
 from .quant import QTensor
 
 torch = D.torch

@@ -1,0 +1,349 @@
+"""Operators of the paged key/value cache and of beam search (re-exported by :mod:`.ops`).
+
+A cache layer is a pool of pages ``(pages, kv_heads, page_size, head_dim)`` for keys and one for
+values; a transposed view of ``(pages, page_size, kv_heads, head_dim)`` serves as well (rows of
+``head_dim`` elements stay contiguous).  A request's pages are named by its row of ``block_tables``
+(int32), and a *slot* is ``page * page_size + row``.  The operators chain into a decode step::
+
+    step = ops.paged_extend(lens, new_lens, block_tables, free_pages, free_count, page_size, max_tokens)
+    q = ops.paged_append(qkv, step.slots, step.pos, k_pages, v_pages, heads, cos, sin)
+    out = ops.paged_attention(q, k_pages, v_pages, block_tables, step.lens)
+    ...                                                # the other layers, the head
+    best = ops.beam_select(logits, scores, counts, done, stop=(6561, 6761))
+    ops.paged_reorder(k_all, v_all, block_tables, best.parents, step.lens)
+
+Pools, tables and state are updated in place, so every argument is a device array; a host array
+raises ValueError.  Shape, type and alignment errors raise ValueError, configurations that are not
+built RuntimeError.  The calls are ordered on the current stream of the current device (on which
+all arrays have to be), take no persistent workspace and can be captured into a CUDA graph: what
+they read on the device (lengths, tables, flags) may change between replays.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Optional, Tuple
+
+import numpy as np
+
+from . import _dev as D
+from ._lib import check, load
+
+torch = D.torch
+
+MAX_BEAMS = 32   # CV3_MAX_BEAMS
+
+if torch is not None:
+    _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+else:
+    _TYPES = {np.dtype(np.float32): 0, np.dtype(np.float16): 1}
+
+
+class PagedStep(NamedTuple):
+    """What :func:`paged_extend` gives: one row per new token, and the new state."""
+    slots: object        # int64 (max_tokens,), -1 behind the last token
+    seq: object          # int32 (max_tokens,) request of the token, -1 behind the last
+    pos: object          # int32 (max_tokens,) its position in the request
+    offsets: object      # int32 (batch + 1,) rows of request b: offsets[b] .. offsets[b + 1]
+    lens: object         # int32 (batch,) tokens held, the new ones included
+    free_count: object   # int32 (1,) pages left on the stack
+
+
+class BeamStep(NamedTuple):
+    """What :func:`beam_select` gives, ``(groups, beams)`` each, best first."""
+    tokens: object       # int64
+    parents: object      # int32
+    scores: object       # float32
+    counts: object       # int32
+    done: object         # int32
+
+
+def _device(name: str, *arrays) -> int:
+    """The device of the arrays: all on the current one, or ValueError."""
+    if torch is None:
+        for x in arrays:
+            if not isinstance(x, D.DeviceArray):
+                raise ValueError(f"{name}: device arrays are expected, got {type(x).__name__}")
+        D.require_cuda()
+        return 0
+    here = -2
+    for x in arrays:
+        try:
+            at = x.get_device()
+        except AttributeError:
+            at = -1
+        if at < 0:
+            raise ValueError(f"{name}: CUDA tensors are expected, got a host {type(x).__name__}")
+        if here == -2:
+            here = at
+        elif at != here:
+            raise ValueError(f"{name}: tensors on cuda:{here} and cuda:{at}")
+    if here != torch.cuda.current_device():
+        raise ValueError(f"{name}: tensors on cuda:{here}, the current device is cuda:{torch.cuda.current_device()}")
+    return here
+
+
+def _ints(name: str, what: str, x, n: int, dtype=None) -> int:
+    """Pointer of ``n`` contiguous int32 (or ``dtype``) values."""
+    if x.dtype != (D.I32 if dtype is None else dtype) or x.numel() != n or not x.is_contiguous():
+        raise ValueError(f"{name}: {what} must be {n} contiguous {'int32' if dtype is None else dtype} values, got "
+                         f"{tuple(x.shape)} {x.dtype}")
+    return x.data_ptr()
+
+
+def _table(name: str, tables, rows: Optional[int]) -> Tuple[int, int, int]:
+    """(pointer, row stride, columns) of an int32 block table."""
+    shape, st = tables.shape, tables.stride()
+    if len(shape) != 2 or tables.dtype != D.I32 or (rows is not None and shape[0] != rows) \
+            or (shape[0] > 0 and shape[1] > 1 and st[1] != 1):
+        raise ValueError(f"{name}: block_tables must be int32 (requests, blocks) with contiguous rows, got "
+                         f"{tuple(shape)} {tables.dtype}")
+    return tables.data_ptr(), st[0] if shape[0] > 1 else max(st[0], shape[1]), shape[1]
+
+
+def _type(name: str, x) -> int:
+    t = _TYPES.get(x.dtype)
+    if t is None:
+        raise ValueError(f"{name}: float32, float16 or bfloat16 expected, got {x.dtype}")
+    return t
+
+
+def _pools(name: str, k, v, dims: int):
+    """(type, shape, k strides, v strides) of a pair of page pools with contiguous rows."""
+    shape, ks, vs = k.shape, k.stride(), v.stride()
+    if len(shape) != dims or tuple(v.shape) != tuple(shape) or v.dtype != k.dtype:
+        raise ValueError(f"{name}: k_pages and v_pages must be alike, {dims}-dimensional "
+                         f"(..., kv_heads, page_size, head_dim), got {tuple(shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    if ks[-1] != 1 or vs[-1] != 1:
+        raise ValueError(f"{name}: the rows of head_dim elements must be contiguous")
+    if min(ks) < 0 or min(vs) < 0 or shape[-2] == 0 or shape[-3] == 0:
+        raise ValueError(f"{name}: empty or reversed page dimensions")
+    return _type(name, k), shape, ks, vs
+
+
+def _like(name: str, out, shape, dtype):
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or not out.is_contiguous():
+        raise ValueError(f"{name}: out must be contiguous {tuple(shape)} {dtype}, got {tuple(out.shape)} {out.dtype}")
+    return out
+
+
+def paged_extend(lens, new_lens, block_tables, free_pages, free_count, page_size: int, max_tokens: int, release=None,
+                 out: Optional[PagedStep] = None) -> PagedStep:
+    """Cache pages and slots for the new tokens of every request.
+
+    Request ``b`` holds ``lens[b]`` tokens (int32) and gets ``new_lens[b]`` more; where ``release[b]``
+    is not 0 it first gives its pages back and starts from none, so a finished request's place serves
+    the next one in the same call.  ``free_pages[:free_count]`` is the stack of free page numbers
+    (updated in place, as is ``block_tables``).  Requests are served in order; from the first whose
+    pages, rows (``max_tokens`` over all) or table columns do not suffice on, none gets new tokens.
+    Returns a :class:`PagedStep`; ``out`` gives it its tensors (``out.lens`` may be ``lens`` and
+    ``out.free_count`` may be ``free_count``: the state then advances in place).
+    """
+    name = "paged_extend"
+    arrays = (lens, new_lens, block_tables, free_pages, free_count)
+    d = _device(name, *(arrays if release is None else arrays + (release,)))
+    n, T = lens.shape[0], int(max_tokens)
+    if page_size <= 0 or T < 0:
+        raise ValueError(f"{name}: page_size {page_size}, max_tokens {max_tokens}")
+    pl, pn = _ints(name, "lens", lens, n), _ints(name, "new_lens", new_lens, n)
+    pr = None if release is None else _ints(name, "release", release, n)
+    tp, ld, cols = _table(name, block_tables, n)
+    cap = free_pages.numel()
+    pf, pc = _ints(name, "free_pages", free_pages, cap), _ints(name, "free_count", free_count, 1)
+    if out is None:
+        slots = D.empty((T,), D.I64)
+        if torch is not None:
+            seq, pos, offsets, lens_out, count, scratch = torch.empty(
+                2 * T + 3 * n + 3, dtype=torch.int32, device=lens.device).split((T, T, n + 1, n, 1, n + 1))
+        else:
+            seq, pos, offsets, lens_out, count, scratch = (D.empty((m,), D.I32) for m in (T, T, n + 1, n, 1, n + 1))
+        out = PagedStep(slots, seq, pos, offsets, lens_out, count)
+    else:
+        _device(name, *out)
+        _ints(name, "out.slots", out.slots, T, D.I64)
+        for what, x, m in (("seq", out.seq, T), ("pos", out.pos, T), ("offsets", out.offsets, n + 1),
+                           ("lens", out.lens, n), ("free_count", out.free_count, 1)):
+            _ints(name, "out." + what, x, m)
+        scratch = D.empty((n + 1,), D.I32)
+    rc = load().cv3_paged_extend(pl, pn, pr, n, tp, ld, cols, page_size, pf, cap, pc, T, out.slots.data_ptr(),
+                                 out.seq.data_ptr(), out.pos.data_ptr(), out.offsets.data_ptr(), out.lens.data_ptr(),
+                                 out.free_count.data_ptr(), scratch.data_ptr(), D.raw_stream(d))
+    if rc:
+        check(rc, name)
+    return out
+
+
+def paged_append(qkv, slots, pos, k_pages, v_pages, heads: int, cos=None, sin=None, out=None, bad=None):
+    """RoPE of fused qkv rows and the store of their keys and values by slot.
+
+    ``qkv`` ``(rows, (heads + 2 * kv_heads) * head_dim)`` holds query, key and value heads; returns the
+    rotated queries ``(rows, heads, head_dim)`` in its type and writes keys (rotated) and values in the
+    pools' type at ``slots`` (int64; -1: not stored).  ``cos`` / ``sin`` are fp32 ``(positions,
+    head_dim)`` half-split tables read at ``pos`` (int32); without them nothing is rotated and ``pos``
+    may be None.  A slot outside the pool, or a position outside the tables, stores nothing and counts
+    into ``bad`` (int32, one value).  The slots of one call must differ.
+    """
+    name = "paged_append"
+    d = _device(name, qkv, slots, k_pages, v_pages, *(x for x in (pos, cos, sin, out, bad) if x is not None))
+    kt, shape, ks, vs = _pools(name, k_pages, v_pages, 4)
+    pages, kv, ps, dim = shape
+    t = _type(name, qkv)
+    if qkv.dim() != 2 or heads <= 0 or qkv.shape[1] != (heads + 2 * kv) * dim:
+        raise ValueError(f"{name}: qkv rows of ({heads} + 2 * {kv}) * {dim} elements expected, got {tuple(qkv.shape)}")
+    rows, (ldq, one) = qkv.shape[0], qkv.stride()
+    if one != 1:
+        raise ValueError(f"{name}: qkv rows must be contiguous")
+    pslots = _ints(name, "slots", slots, rows, D.I64)
+    pc = psn = None
+    positions = 0
+    if (cos is None) != (sin is None) or (cos is not None and pos is None):
+        raise ValueError(f"{name}: cos, sin and pos go together")
+    ppos = None if pos is None else _ints(name, "pos", pos, rows)
+    if cos is not None:
+        positions = cos.shape[0]
+        for x in (cos, sin):
+            if x.dtype != D.F32 or tuple(x.shape) != (positions, dim) or not x.is_contiguous():
+                raise ValueError(f"{name}: cos and sin must be contiguous float32 (positions, {dim})")
+        pc, psn = cos.data_ptr(), sin.data_ptr()
+    if out is None:
+        out = D.empty((rows, heads, dim), qkv.dtype)
+    else:
+        _like(name, out, (rows, heads, dim), qkv.dtype)
+    pbad = None if bad is None else _ints(name, "bad", bad, 1)
+    rc = load().cv3_paged_append(qkv.data_ptr(), t, rows, ldq if rows > 1 else qkv.shape[1], pc, psn, positions, pslots,
+                                 ppos, heads, kv, dim, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), kt, ks[0],
+                                 ks[1], ks[2], vs[0], vs[1], vs[2], pages, ps,
+                                 pbad, D.raw_stream(d))
+    if rc:
+        check(rc, name)
+    return out
+
+
+def paged_attention(q, k_pages, v_pages, block_tables, lens, scale: Optional[float] = None, window: int = 0, out=None,
+                    return_lse: bool = False, bad=None):
+    """Softmax attention of one new token per request over its cached tokens.
+
+    ``q`` ``(batch, heads, head_dim)`` -> the same shape and type; GQA when the pools have fewer heads;
+    the pools may have another element type (an fp16 or bf16 cache under fp32 activations keeps fp32
+    arithmetic).  ``lens`` (int32) counts the cached tokens, the new one included; ``window`` > 0 keeps
+    the last ``window`` of them.  A request without tokens gives zeros.  ``return_lse`` adds the fp32
+    ``(batch, heads)`` logarithms of the softmax sums (-inf without tokens), by which results over
+    separate caches are joined.  Tokens of a page number outside the pool are left out and counted
+    (per table entry) into ``bad``.
+    """
+    name = "paged_attention"
+    d = _device(name, q, k_pages, v_pages, block_tables, lens, *(x for x in (out, bad) if x is not None))
+    kt, shape, ks, vs = _pools(name, k_pages, v_pages, 4)
+    pages, kv, ps, dim = shape
+    qt = _type(name, q)
+    if q.dim() != 3 or q.shape[2] != dim:
+        raise ValueError(f"{name}: q must be (batch, heads, {dim}), got {tuple(q.shape)}")
+    B, H = q.shape[0], q.shape[1]
+    if H == 0 or H % kv:
+        raise ValueError(f"{H} query heads is not a multiple of {kv} kv heads")
+    qsb, qsh, one = q.stride()
+    if one != 1:
+        raise ValueError(f"{name}: the heads of q must be contiguous")
+    window = int(window)
+    if window < 0:
+        raise ValueError(f"{name}: window {window}")
+    tp, ld, cols = _table(name, block_tables, B)
+    plens = _ints(name, "lens", lens, B)
+    if out is None:
+        out = D.empty((B, H, dim), q.dtype)
+    else:
+        _like(name, out, (B, H, dim), q.dtype)
+    pbad = None if bad is None else _ints(name, "bad", bad, 1)
+    lse = D.empty((B, H)) if return_lse else None
+    lib = load()
+    words = lib.cv3_paged_attention_workspace(B, H, kv, dim, cols * ps)
+    ws = D.empty((words,)) if words else None
+    rc = lib.cv3_paged_attention(q.data_ptr(), qt, qsb, qsh, k_pages.data_ptr(), v_pages.data_ptr(), kt, ks[0], ks[1],
+                                 ks[2], vs[0], vs[1], vs[2], pages, ps, tp, ld, cols, plens, B, H, kv, dim, window,
+                                 1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), H * dim, dim,
+                                 None if lse is None else lse.data_ptr(), pbad, None if ws is None else ws.data_ptr(), words, D.raw_stream(d))
+    if rc:
+        check(rc, name)
+    return (out, lse) if return_lse else out
+
+
+def beam_select(logits, scores, counts, done, stop: Optional[Tuple[int, int]] = None, min_len=None,
+                length_penalty: float = 0.0, out: Optional[BeamStep] = None) -> BeamStep:
+    """The best continuations of every group's hypotheses.
+
+    ``logits`` ``(groups, beams, vocab)``; ``scores`` (float32 sums of log-probabilities), ``counts``
+    and ``done`` (int32) are ``(groups, beams)``.  A candidate's key is its new score divided by its
+    length to the power ``length_penalty``; the ``beams`` best of all ``beams * vocab`` are kept, equal
+    keys in the order of the lower hypothesis and token.  A token in ``stop`` (first, end) finishes a
+    hypothesis, and is no candidate while it has fewer than ``min_len[group]`` tokens; a finished one
+    stays as it is (token 0).  A score of -inf marks a hypothesis that does not exist, as all but the
+    first at the start.  NaN logits are no candidates.  Keys are computed in 64 bits.  ``out`` gives the
+    :class:`BeamStep` its tensors, which may be the input state.
+    """
+    name = "beam_select"
+    d = _device(name, logits, scores, counts, done, *((min_len,) if min_len is not None else ()))
+    t = _type(name, logits)
+    if logits.dim() != 3:
+        raise ValueError(f"{name}: logits must be (groups, beams, vocab), got {tuple(logits.shape)}")
+    G, K, V = logits.shape
+    sg, sk, sv = logits.stride()
+    if (V > 1 and sv != 1) or (G > 1 and sg != K * sk):
+        raise ValueError(f"{name}: rows of logits must be contiguous and evenly spaced")
+    n = G * K
+    if scores.dtype != D.F32 or scores.numel() != n or not scores.is_contiguous():
+        raise ValueError(f"{name}: scores must be {n} contiguous float32 values")
+    pc, pd = _ints(name, "counts", counts, n), _ints(name, "done", done, n)
+    pm = None if min_len is None else _ints(name, "min_len", min_len, G)
+    lo, hi = (0, 0) if stop is None else stop
+    if not 0 <= lo <= hi <= V:
+        raise ValueError(f"{name}: stop tokens {lo}..{hi} outside the vocabulary of {V}")
+    if out is None:
+        if torch is not None:
+            parents, cnt, fin = torch.empty((3, G, K), dtype=torch.int32, device=logits.device).unbind(0)
+        else:
+            parents, cnt, fin = (D.empty((G, K), D.I32) for _ in range(3))
+        out = BeamStep(D.empty((G, K), D.I64), parents, D.empty((G, K)), cnt, fin)
+    else:
+        _device(name, logits, *out)
+        for x, dt in zip(out, (D.I64, D.I32, D.F32, D.I32, D.I32)):
+            _like(name, x, (G, K), dt)
+    lib = load()
+    size = lib.cv3_beam_workspace(G, K, V)
+    ws = D.empty((max(size, 8) // 8,), D.I64)
+    rc = lib.cv3_beam_select(logits.data_ptr(), t, sk if n > 1 else V, G, K, V, scores.data_ptr(), pc, pd, lo, hi, pm,
+                             length_penalty, out.tokens.data_ptr(), out.parents.data_ptr(), out.scores.data_ptr(),
+                             out.counts.data_ptr(), out.done.data_ptr(), ws.data_ptr(), size, D.raw_stream(d))
+    if rc:
+        check(rc, name)
+    return out
+
+
+def paged_reorder(k_pages, v_pages, block_tables, parents, lens) -> None:
+    """The cache follows the beams, in place.
+
+    Pools ``(layers, pages, kv_heads, page_size, head_dim)`` (or one layer without the first
+    dimension); ``block_tables`` ``(groups * beams, blocks)``; ``parents`` int32 ``(groups, beams)``;
+    ``lens`` int32 ``(groups * beams,)``, alike within a group.  Beam k becomes what beam
+    ``parents[g][k]`` was: full pages are shared through the table, the tokens of the last, partly
+    filled page are copied into the page that beam k's own row names there (and no other beam's).
+    """
+    name = "paged_reorder"
+    d = _device(name, k_pages, v_pages, block_tables, parents, lens)
+    dims = len(k_pages.shape)
+    if dims not in (4, 5):
+        raise ValueError(f"{name}: pools of 4 or 5 dimensions expected, got {tuple(k_pages.shape)}")
+    kt, shape, ks, vs = _pools(name, k_pages, v_pages, dims)
+    if dims == 4:
+        shape, ks, vs = (1,) + tuple(shape), (0,) + tuple(ks), (0,) + tuple(vs)
+    layers, pages, kv, ps, dim = shape
+    if len(parents.shape) != 2:
+        raise ValueError(f"{name}: parents must be (groups, beams), got {tuple(parents.shape)}")
+    G, K = parents.shape
+    pp = _ints(name, "parents", parents, G * K)
+    tp, ld, cols = _table(name, block_tables, G * K)
+    plens = _ints(name, "lens", lens, G * K)
+    rc = load().cv3_paged_reorder(k_pages.data_ptr(), v_pages.data_ptr(), kt, layers, pages, kv, ps, dim, ks[0], ks[1],
+                                  ks[2], ks[3], vs[0], vs[1], vs[2], vs[3], tp, ld, cols, pp,
+                                  plens, G, K, D.raw_stream(d))
+    if rc:
+        check(rc, name)

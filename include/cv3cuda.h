@@ -376,6 +376,105 @@ int cv3_head_select(const float* logits, int64_t batch, int64_t vocab, int64_t s
                     int* step, void* stream);
 
 /* ------------------------------------------------------------------ */
+/* paged key/value cache and beam search                                */
+/* ------------------------------------------------------------------ */
+
+/* No counterparts in the reference, whose cache is one array per sequence
+ * (cv3cpu/models/qwen2.py:74-121) and whose decoding keeps one hypothesis
+ * (cv3cpu/models/llm.py:80-149).
+ *
+ * A cache layer is a pool of pages: token row r of page p for kv head h starts at
+ * element p*s_p + h*s_h + r*s_t of k_pages / v_pages (strides in elements, rows of
+ * head_dim contiguous elements on 16-byte boundaries), so both [page][kv_head][row]
+ * and [page][row][kv_head] pools are read in place.  Request b's token t lives in
+ * row t % page_size of page block_tables[b*table_ld + t / page_size] (int32); a slot
+ * is page * page_size + row (int64). */
+#define CV3_TYPE_F32 0
+#define CV3_TYPE_F16 1
+#define CV3_TYPE_BF16 2
+
+/* Pages and slots for the new tokens of `batch` requests.  Request b holds lens[b]
+ * tokens (with release non-NULL and release[b] != 0 it first gives its pages back and
+ * holds none) and gets new_lens[b] more.  Free pages are a stack: free_pages[0 ..
+ * *free_count) of free_cap entries, given back and taken at its end, requests in
+ * order.  Requests are served in order while their pages, their rows (max_tokens in
+ * all) and the max_blocks columns of their table rows suffice; from the first that
+ * does not fit on none gets anything.  Negative numbers count as 0.
+ * Written: the new entries of block_tables; slots / seq / pos [max_tokens], one row
+ * per new token, requests one after another (rows behind the last: slot -1, seq -1,
+ * pos 0); offsets [batch + 1], request b's rows being offsets[b] .. offsets[b+1];
+ * lens_out [batch]; *free_count_out.  lens_out may be lens, free_count_out may be
+ * free_count.  scratch: batch + 1 ints. */
+int cv3_paged_extend(const int* lens, const int* new_lens, const int* release, int64_t batch, int* block_tables,
+                     int64_t table_ld, int64_t max_blocks, int64_t page_size, int* free_pages, int64_t free_cap,
+                     const int* free_count, int64_t max_tokens, int64_t* slots, int* seq, int* pos, int* offsets,
+                     int* lens_out, int* free_count_out, int* scratch, void* stream);
+
+/* cv3_rope_qkv_append into pages: rows of fused qkv [rows][ldq] (q heads, k heads, v
+ * heads; element type `type`) -> q_out [rows][heads][head_dim] of that type, rotated;
+ * k rotated and v as it is, in the cache's type kv_type, at slots[r].  Slot -1 stores
+ * nothing; another slot outside the pool, or a position outside the tables
+ * [positions][head_dim], stores nothing and adds 1 to *bad (may be NULL).  NULL
+ * tables: no rotation (pos may be NULL).  Slots of one call must differ.  head_dim a
+ * multiple of 16 up to 256; rows on 16-byte boundaries. */
+int cv3_paged_append(const void* qkv, int type, int64_t rows, int64_t ldq, const float* cos_table,
+                     const float* sin_table, int64_t positions, const int64_t* slots, const int* pos, int64_t heads,
+                     int64_t kv_heads, int64_t head_dim, void* q_out, void* k_pages, void* v_pages, int kv_type,
+                     int64_t ksp, int64_t ksh, int64_t kst, int64_t vsp, int64_t vsh, int64_t vst, int64_t num_pages,
+                     int64_t page_size, int* bad, void* stream);
+
+/* One new token's attention per request over its pages: out[b][h] = softmax(scale *
+ * q[b][h] . K) V over request b's cached tokens [max(0, lens[b] - window), lens[b])
+ * (window 0: all; lens beyond the table's columns count as these).  q and out: element
+ * (b, h, d) at b*s_b + h*s_h + d, type q_type; the cache's type kv_type may be another.
+ * GQA: query head h uses kv head h / (heads / kv_heads).  A request without tokens
+ * gives zeros.  Tokens of a page number outside the pool are left out, and each such
+ * table entry adds 1 to *bad (may be NULL).  lse (may be NULL) [batch][heads]: the
+ * logarithm of the softmax's sum (-inf without tokens).  head_dim 32, 64, 96 or 128.
+ * workspace: cv3_paged_attention_workspace() floats (its max_len: max_blocks *
+ * page_size), nothing kept in it between calls. */
+int cv3_paged_attention(const void* q, int q_type, int64_t qsb, int64_t qsh, const void* k_pages, const void* v_pages,
+                        int kv_type, int64_t ksp, int64_t ksh, int64_t kst, int64_t vsp, int64_t vsh, int64_t vst,
+                        int64_t num_pages, int64_t page_size, const int* block_tables, int64_t table_ld,
+                        int64_t max_blocks, const int* lens, int64_t batch, int64_t heads, int64_t kv_heads,
+                        int64_t head_dim, int64_t window, float scale, void* out, int64_t osb, int64_t osh, float* lse,
+                        int* bad, float* workspace, int64_t workspace_floats, void* stream);
+int64_t cv3_paged_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                      int64_t max_len);
+
+/* Beam search's choice.  Group g's `beams` hypotheses have scores (sums of
+ * log-probabilities), counts (tokens so far) and done flags [groups][beams], and
+ * logits rows (g*beams + k) of `vocab` entries, ld apart.  Candidate (k, v) has the key
+ * (scores[k] + log_softmax(logits[k])[v]) / (counts[k] + 1)^length_penalty; a done
+ * hypothesis has one candidate, itself (token 0, key scores[k] / counts[k]^
+ * length_penalty).  Tokens of [stop_lo, stop_hi) end a hypothesis; they are no
+ * candidates while counts[k] < min_len[g] (min_len may be NULL).  NaN logits, and
+ * hypotheses with a score of -inf or NaN, give no candidates.  The `beams` best keys
+ * in descending order (equal keys: the lowest k*vocab + v; -inf keys where too few
+ * remain) give tokens, parents (k), the new scores (fp32), counts and done flags, which
+ * may be the input buffers.  Keys are computed in 64 bits.
+ * workspace: cv3_beam_workspace() bytes, 8-byte aligned, nothing kept in it. */
+#define CV3_MAX_BEAMS 32
+int cv3_beam_select(const void* logits, int type, int64_t ld, int64_t groups, int64_t beams, int64_t vocab,
+                    const float* scores, const int* counts, const int* done, int64_t stop_lo, int64_t stop_hi,
+                    const int* min_len, double length_penalty, int64_t* tokens, int* parents, float* scores_out,
+                    int* counts_out, int* done_out, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t cv3_beam_workspace(int64_t groups, int64_t beams, int64_t vocab);
+
+/* The cache follows the beams: rows g*beams .. of block_tables are a group's beams, all
+ * of the length lens[g*beams].  Beam k becomes what beam parents[g][k] was: the table
+ * entries of full pages are taken over (the pages are shared from then on), and the
+ * tokens of the last, partly filled page are copied in every layer into the page that
+ * beam k's own row names there, which no other beam may name.  A parent outside
+ * [0, beams) counts as k; a beam whose own or whose parent's last page lies outside the
+ * pool keeps that page as it is.  Pools: layers s_l apart. */
+int cv3_paged_reorder(void* k_pages, void* v_pages, int kv_type, int64_t layers, int64_t num_pages, int64_t kv_heads,
+                      int64_t page_size, int64_t head_dim, int64_t ksl, int64_t ksp, int64_t ksh, int64_t kst,
+                      int64_t vsl, int64_t vsp, int64_t vsh, int64_t vst, int* block_tables, int64_t table_ld,
+                      int64_t max_blocks, const int* parents, const int* lens, int64_t groups, int64_t beams,
+                      void* stream);
+
+/* ------------------------------------------------------------------ */
 /* DiT flow estimator and Euler/CFG solve (cv3cpu/models/dit.py, flow.py) */
 /* ------------------------------------------------------------------ */
 

@@ -1,0 +1,234 @@
+"""Refusals of the paged-cache and beam-search operators, without a GPU: host arrays, shapes, types,
+strides and alignment are rejected before anything reaches the device (the host checks run here on
+CPU tensors with the device check replaced, the C ABI on made-up addresses that it must not touch)."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+from conftest import pkg
+
+import oracle.paged as ref
+
+
+@pytest.fixture
+def ops(monkeypatch):
+    import torch
+    p = pkg("paged")
+    monkeypatch.setattr(p, "_device", lambda name, *arrays: 0)
+
+    def no_launch():
+        raise AssertionError("the arguments were accepted")
+    monkeypatch.setattr(p, "load", no_launch)
+    monkeypatch.setattr(p.D, "require_cuda", lambda: None)
+    monkeypatch.setattr(p.D, "empty", lambda shape, dtype=None: torch.empty(shape, dtype=dtype or torch.float32))
+    return p
+
+
+def _i32(*shape):
+    import torch
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def test_host_arrays_are_refused():
+    import torch
+    p = pkg("paged")
+    x = torch.zeros(2, 4, 64)
+    pool = torch.zeros(3, 2, 16, 64)
+    for bad in (x, x.numpy()):
+        with pytest.raises(ValueError, match="CUDA tensors are expected"):
+            p.paged_attention(bad, pool, pool, _i32(2, 3), _i32(2))
+    with pytest.raises(ValueError, match="CUDA tensors are expected"):
+        p.beam_select(torch.zeros(1, 2, 9), torch.zeros(1, 2), _i32(1, 2), _i32(1, 2))
+    with pytest.raises(ValueError, match="CUDA tensors are expected"):
+        p.paged_extend(_i32(2), _i32(2), _i32(2, 3), _i32(9), _i32(1), 16, 4)
+    with pytest.raises(ValueError, match="CUDA tensors are expected"):
+        p.paged_append(torch.zeros(2, 8 * 64), torch.zeros(2, dtype=torch.int64), _i32(2), pool, pool, 4)
+    with pytest.raises(ValueError, match="CUDA tensors are expected"):
+        p.paged_reorder(pool, pool, _i32(4, 3), _i32(2, 2), _i32(4))
+
+
+def test_other_devices_are_refused(monkeypatch):
+    import torch
+    p = pkg("paged")
+
+    class On:
+        def __init__(self, d):
+            self.d = d
+
+        def get_device(self):
+            return self.d
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    assert p._device("op", On(0), On(0)) == 0
+    with pytest.raises(ValueError, match="cuda:0 and cuda:1"):
+        p._device("op", On(0), On(1))
+    with pytest.raises(ValueError, match="current device is cuda:0"):
+        p._device("op", On(1), On(1))
+
+
+def test_extend_refusals(ops):
+    import torch
+    good = dict(lens=_i32(3), new_lens=_i32(3), block_tables=_i32(3, 5), free_pages=_i32(9), free_count=_i32(1),
+                page_size=16, max_tokens=4)
+    with pytest.raises(AssertionError, match="accepted"):
+        ops.paged_extend(**good)
+    for change in (dict(new_lens=_i32(2)), dict(lens=torch.zeros(3, dtype=torch.int64)), dict(block_tables=_i32(2, 5)),
+                   dict(block_tables=_i32(5, 3).T), dict(free_count=_i32(2)), dict(page_size=0), dict(max_tokens=-1),
+                   dict(release=_i32(4)), dict(lens=_i32(6)[::2]), dict(free_pages=torch.zeros(9)),
+                   dict(out=ops.PagedStep(*[_i32(4)] * 6)),
+                   dict(block_tables=torch.zeros(3, 5))):
+        with pytest.raises(ValueError):
+            ops.paged_extend(**{**good, **change})
+
+
+def test_append_refusals(ops):
+    import torch
+    pool = torch.zeros(3, 2, 16, 64)
+    tab = torch.zeros(50, 64)
+    good = dict(qkv=torch.zeros(4, 8 * 64), slots=torch.zeros(4, dtype=torch.int64), pos=_i32(4), k_pages=pool,
+                v_pages=pool.clone(), heads=4, cos=tab, sin=tab)
+    with pytest.raises(AssertionError, match="accepted"):
+        ops.paged_append(**good)
+    for change in (dict(heads=5), dict(heads=0), dict(slots=_i32(4)), dict(slots=torch.zeros(3, dtype=torch.int64)),
+                   dict(cos=None), dict(pos=None), dict(pos=_i32(5)), dict(cos=torch.zeros(50, 32)),
+                   dict(cos=tab.double()), dict(k_pages=pool.double(), v_pages=pool.double()),
+                   dict(v_pages=pool.half()), dict(v_pages=pool[:2]), dict(k_pages=pool[0], v_pages=pool[0]),
+                   dict(k_pages=pool.transpose(2, 3), v_pages=pool.transpose(2, 3)),
+                   dict(qkv=torch.zeros(4, 8 * 64, dtype=torch.int32)), dict(qkv=torch.zeros(8 * 64, 4).T),
+                   dict(out=torch.zeros(4, 4, 32)), dict(bad=_i32(2)), dict(qkv=torch.zeros(4, 8, 64))):
+        with pytest.raises(ValueError):
+            ops.paged_append(**{**good, **change})
+
+
+def test_attention_refusals(ops):
+    import torch
+    pool = torch.zeros(3, 2, 16, 64)
+    good = dict(q=torch.zeros(2, 4, 64), k_pages=pool, v_pages=pool, block_tables=_i32(2, 3), lens=_i32(2))
+    with pytest.raises(AssertionError, match="accepted"):
+        ops.paged_attention(**good)
+    for change in (dict(q=torch.zeros(2, 3, 64)), dict(q=torch.zeros(2, 4, 32)), dict(q=torch.zeros(4, 64)),
+                   dict(q=torch.zeros(2, 64, 4).transpose(1, 2)), dict(q=torch.zeros(2, 4, 64, dtype=torch.float64)),
+                   dict(lens=_i32(3)), dict(lens=torch.zeros(2)), dict(block_tables=_i32(3, 3)), dict(window=-1),
+                   dict(out=torch.zeros(2, 4, 64, dtype=torch.float16)), dict(out=torch.zeros(4, 2, 64).transpose(0, 1)),
+                   dict(v_pages=torch.zeros(3, 2, 8, 64)), dict(q=torch.zeros(2, 0, 64)), dict(bad=_i32(0)),
+                   dict(k_pages=torch.zeros(3, 2, 0, 64), v_pages=torch.zeros(3, 2, 0, 64))):
+        with pytest.raises(ValueError):
+            ops.paged_attention(**{**good, **change})
+
+
+def test_beam_and_reorder_refusals(ops):
+    import torch
+    good = dict(logits=torch.zeros(2, 3, 50), scores=torch.zeros(2, 3), counts=_i32(2, 3), done=_i32(2, 3))
+    with pytest.raises(AssertionError, match="accepted"):
+        ops.beam_select(**good)
+    for change in (dict(logits=torch.zeros(6, 50)), dict(scores=torch.zeros(2, 2)), dict(scores=_i32(2, 3)),
+                   dict(counts=torch.zeros(2, 3)), dict(done=torch.zeros(2, 3, dtype=torch.bool)), dict(stop=(3, 51)),
+                   dict(stop=(5, 4)), dict(stop=(-1, 4)), dict(min_len=_i32(3)),
+                   dict(logits=torch.zeros(2, 50, 3).transpose(1, 2)), dict(logits=torch.zeros(3, 2, 50).transpose(0, 1)),
+                   dict(logits=torch.zeros(2, 3, 50, dtype=torch.int32)), dict(out=ops.BeamStep(*[_i32(2, 3)] * 5))):
+        with pytest.raises(ValueError):
+            ops.beam_select(**{**good, **change})
+    pool = torch.zeros(2, 9, 2, 16, 64)
+    fine = dict(k_pages=pool, v_pages=pool, block_tables=_i32(6, 3), parents=_i32(2, 3), lens=_i32(6))
+    with pytest.raises(AssertionError, match="accepted"):
+        ops.paged_reorder(**fine)
+    for change in (dict(k_pages=pool[0, 0]), dict(v_pages=pool[0]), dict(block_tables=_i32(5, 3)), dict(parents=_i32(6)),
+                   dict(lens=_i32(2)), dict(parents=torch.zeros(2, 3)), dict(k_pages=pool.int(), v_pages=pool.int())):
+        with pytest.raises(ValueError):
+            ops.paged_reorder(**{**fine, **change})
+
+
+def test_c_entries_refuse_before_any_device_work():
+    L = pkg("_lib")
+    lib = L.load()
+    P = ctypes.c_void_p
+    V, U = L.CV3_ERR_VALUE, L.CV3_ERR_UNSUPPORTED
+
+    def attention(dim=64, kv=2, heads=4, ps=16, strides=(2048, 1024, 64), k=1 << 20, kt=0, cols=3, ld=3, window=0):
+        return lib.cv3_paged_attention(P(1 << 20), 0, heads * dim, dim, P(k), P(1 << 20), kt, *strides, *strides, 9, ps,
+                                       P(1 << 20), ld, cols, P(1 << 20), 0, heads, kv, dim, window, 0.1, P(1 << 20),
+                                       heads * dim, dim, None, None, None, 0, None)
+    assert attention() == 0                                  # no requests: nothing to do
+    assert attention(dim=80) == U and b"head_dim" in lib.cv3_last_error()
+    assert attention(kv=3) == V and b"not a multiple" in lib.cv3_last_error()
+    assert attention(strides=(2048, 1024, 62)) == V and b"16-byte" in lib.cv3_last_error()
+    assert attention(k=(1 << 20) + 4) == V
+    assert attention(kt=5) == V and attention(ps=0) == V and attention(ld=2) == V and attention(window=-1) == V
+    assert attention(cols=1 << 28, ld=1 << 28) == V and b"32-bit" in lib.cv3_last_error()
+
+    def append(dim=64, ldq=8 * 64, rows=0, qkv=1 << 20, cos=None, sin=None, t=0):
+        return lib.cv3_paged_append(P(qkv), t, rows, ldq, cos, sin, 0, None, None, 4, 2, dim, P(1 << 20), P(1 << 20),
+                                    P(1 << 20), 0, 2048, 1024, 64, 2048, 1024, 64, 9, 16, None, None)
+    assert append() == 0
+    assert append(dim=72) == U and append(ldq=500) == V and append(ldq=8 * 64 + 2) == V and append(t=3) == V
+    assert append(qkv=(1 << 20) + 8) == V and append(cos=P(1 << 20)) == V
+
+    def extend(tokens=4, ps=16, cols=3, ld=3, cap=9):
+        return lib.cv3_paged_extend(None, None, None, 2, None, ld, cols, ps, None, cap, None, tokens, *[None] * 8)
+    assert extend(ps=0) == V and extend(tokens=-1) == V and extend(ld=2) == V and extend(tokens=1 << 31) == V
+    assert extend(cols=1 << 28, ld=1 << 28) == V and extend(cap=-1) == V
+
+    def beam(beams=4, vocab=100, ld=100, stop=(0, 0), t=0, ws=None, size=0, groups=2):
+        return lib.cv3_beam_select(None, t, ld, groups, beams, vocab, None, None, None, *stop, None, 0.0, None, None, None,
+                                   None, None, ws, size, None)
+    assert beam(groups=0) == 0
+    assert beam(beams=33) == U and beam(beams=0) == U and beam(ld=99) == V and beam(stop=(5, 4)) == V and beam(t=9) == V
+    assert beam() == V and b"workspace" in lib.cv3_last_error()
+    assert beam(ws=P(1 << 20), size=lib.cv3_beam_workspace(2, 4, 100) - 1) == V
+    assert beam(ws=P((1 << 20) + 4), size=1 << 20) == V
+
+    def reorder(beams=4, dim=64, st=64, t=0, groups=0):
+        s = (1 << 16, 2048, 1024, st)
+        return lib.cv3_paged_reorder(P(1 << 20), P(1 << 20), t, 2, 9, 2, 16, dim, *s, *s, None, 3, 3, None, None, groups,
+                                     beams, None)
+    assert reorder() == 0 and reorder(beams=1, groups=3) == 0
+    assert reorder(beams=33) == U and reorder(st=63) == V and reorder(dim=62, st=64) == V and reorder(t=4) == V
+    with pytest.raises(RuntimeError):
+        L.check(reorder(beams=33), "cv3_paged_reorder")
+
+
+def test_oracle_extend_and_reorder_by_hand():
+    """The restatement itself on cases small enough to write down."""
+    t = np.array([[4, -1], [5, 6]], np.int32)
+    s = np.array([0, 1, 2, 3, 9, 9], np.int32)
+    tables, stack, slots, seq, pos, off, lens, count = ref.extend([2, 3], [3, 1], t, s, 4, 2, 5, [0, 1])
+    assert tables.tolist() == [[4, 6], [5, 6]] or tables.tolist() == [[4, -1], [5, 6]]
+    # request 0 needs two more pages than its two columns hold: nobody is served
+    assert lens.tolist() == [2, 0] and off.tolist() == [0, 0, 0] and count == 6 and stack.tolist() == [0, 1, 2, 3, 5, 6]
+    tables, stack, slots, seq, pos, off, lens, count = ref.extend([2, 3], [2, 1], t, s, 4, 2, 5, [0, 1])
+    assert tables.tolist() == [[4, 6], [5, 6]] and lens.tolist() == [4, 1] and count == 4
+    assert slots.tolist() == [12, 13, 10, -1, -1] and seq.tolist() == [0, 0, 1, -1, -1] and pos.tolist() == [2, 3, 0, 0, 0]
+    k = np.arange(2 * 3 * 2, dtype=np.float32).reshape(1, 6, 1, 2, 1)
+    kk, vv, tt = ref.reorder(k, k, np.array([[0, 1, 2], [3, 4, 5]], np.int32), np.array([[1, 1]], np.int32), [3, 3])
+    assert tt.tolist() == [[3, 1, 2], [3, 4, 5]]
+    assert kk[0, 1, 0, :, 0].tolist() == [8, 3] and kk[0, 4, 0, :, 0].tolist() == [8, 9]
+
+
+def test_oracle_beam_against_torch():
+    import torch
+    rng = np.random.default_rng(0)
+    x = rng.normal(size=(2, 3, 40))
+    s = rng.normal(size=(2, 3)).astype(np.float32)
+    z = np.zeros((2, 3), np.int32)
+    tok, par, sc, cnt, done = ref.beam(x, s, z, z, (35, 40))
+    cum = torch.log_softmax(torch.from_numpy(x), -1) + torch.from_numpy(s)[..., None].double()
+    v, i = cum.view(2, -1).topk(3)
+    assert np.array_equal(par * 40 + tok, i.numpy()) and np.allclose(sc, v.numpy(), rtol=1e-12)
+    assert np.all(cnt == 1) and np.array_equal(done, tok >= 35)
+
+
+def test_oracle_attention_against_torch():
+    import torch
+    rng = np.random.default_rng(0)
+    k, v = rng.normal(size=(2, 5, 2, 4, 8))
+    t = np.array([[3, 1, 0], [4, 2, 9]], np.int32)
+    q = rng.normal(size=(2, 4, 8))
+    out, lse = ref.attention(q, k, v, t, [11, 8], 0.3, 6)
+    for b, (lo, n) in enumerate(((5, 11), (2, 8))):
+        for h in range(4):
+            kk = torch.from_numpy(np.concatenate([k[p, h // 2] for p in t[b, :-(-n // 4)]])[lo:n])
+            vv = torch.from_numpy(np.concatenate([v[p, h // 2] for p in t[b, :-(-n // 4)]])[lo:n])
+            a = 0.3 * (kk @ torch.from_numpy(q[b, h]))
+            assert np.allclose(out[b, h], (torch.softmax(a, 0) @ vv).numpy())
+            assert np.isclose(lse[b, h], float(torch.logsumexp(a, 0)))
