@@ -2,7 +2,28 @@
 //
 // out[b][h] = sum_j p_j V[j], p = softmax(scale * q[b][h] . K[j]) over the request's cached keys j
 // in [max(0, len - window), len); a request without keys gives zeros and a log-sum of -inf.
+//
+// Bound by the cache's bytes: every key and value is read once for the up to 8 query heads that share
+// it.  Three choices follow.
+//
+// 1. Work is cut evenly, whatever the lengths.  A pair (request, group of up to 8 heads of a kv head)
+//    has ceil(keys / TK) tiles; all pairs' tiles in order form one line, of which each of the grid's
+//    CTAs takes an equal piece (found from the lengths on the device, so a captured launch follows
+//    them).  A CTA meets at most two pairs that it does not hold whole -- the one that began before
+//    its piece and the one that goes on behind it -- and leaves their partial results (running
+//    maximum, sum, unnormalised output) in two slots; a second launch joins the slots of every pair
+//    that was cut, in CTA order, so the result does not depend on timing.
+// 2. One pass, nothing staged.  A warp takes KI keys of each tile with matrix instructions whose
+//    operands come straight from global memory into registers: the keys' and values' 16-byte pieces
+//    land in the lanes that need them because the order in which head dimensions (for q.k) and the
+//    order in which output columns (for p.v) enter a product is free.
+// 3. fp32 arithmetic on the tf32 matrix pipe.  fp16 and bf16 keys and values are tf32 numbers
+//    exactly; fp32 ones are split into two (the low 13 bits apart).  The products have 16 rows and at
+//    most 8 heads, so rows 0..7 hold the upper tf32 part of q (then of p) and rows 8..15 the lower
+//    part: 22 bits of both at no cost.  The matrix pipe truncates when it adds, so only one tile's
+//    p.v is summed there; tiles are added in fp32 registers, the softmax's rescaling on the way.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -13,89 +34,493 @@ struct AttnArgs {
   int q_type;
   int64_t qsb, qsh;
   const void *k, *v;
-  int64_t ksp, ksh, kst, vsp, vsh, vst, pages, ps;
+  int64_t ksp, ksh, kst, vsp, vsh, vst, pages;
+  int ps;
+  uint32_t ps_mul, ps_shift;  // n / ps = (n * ps_mul) >> ps_shift for 0 <= n < 2^31 (64-bit product)
   const int* tables;
-  int64_t ld, max_blocks;
+  int64_t ld;
+  int max_keys;  // columns * page size
   const int* lens;
-  int heads, kv_heads;
-  int64_t window;
+  int batch, heads, kv_heads, group, groups;  // group: heads per kv head; groups: of up to 8 of them
+  int window;
   float scale;
   void* out;
   int64_t osb, osh;
   float* lse;
   int* bad;
+  float* part;  // [CTA][2][8][D] unnormalised outputs
+  float* stat;  // [CTA][2][8][2] maximum (base 2) and sum
+  int2* cut;    // [pair] first CTA and number of CTAs (0: nothing to join)
 };
 
-constexpr int AW = 8;  // warps: each takes every AW-th key
+constexpr int NW = 8;                  // warps of a CTA, each with KI keys of every tile
+constexpr int HT = 8;                  // query heads of a CTA (rows of a product that are not lower parts)
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float TINY = 1e-37f;         // stands for a lower part of 0, so that 0 * inf does not arise
 
-// One CTA per (request, query head); a warp's lanes hold D / 32 dimensions of the head.
+// Keys of a warp's step: about 8 KB of keys and values for the warp, which with two CTAs per SM
+// keeps enough loads in flight.
 template <typename KT, int D>
-__global__ void __launch_bounds__(AW * 32) paged_attention_kernel(const AttnArgs a) {
-  constexpr int E = D / 32;
-  __shared__ float part[AW][D], pm[AW], pl[AW];
+constexpr int keys_per_step() {
+  return D * (int)sizeof(KT) <= 128 ? 32 : D * (int)sizeof(KT) <= 256 ? 16 : 8;
+}
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t tf32_hi(uint32_t x) { return x & 0xFFFFE000u; }
+
+__device__ __forceinline__ float exp2_fast(float x) {  // relative error 2^-22
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int BYTES>
+struct Raw;
+template <>
+struct Raw<16> { uint32_t r[4]; };
+template <>
+struct Raw<8> { uint32_t r[2]; };
+
+__device__ __forceinline__ void fetch(Raw<16>& x, const void* p, bool ok) {
+  x.r[0] = x.r[1] = x.r[2] = x.r[3] = 0u;
+  if (ok)
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(x.r[0]), "=r"(x.r[1]), "=r"(x.r[2]), "=r"(x.r[3]) : "l"(p));
+}
+__device__ __forceinline__ void fetch(Raw<8>& x, const void* p, bool ok) {
+  x.r[0] = x.r[1] = 0u;
+  if (ok) asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(x.r[0]), "=r"(x.r[1]) : "l"(p));
+}
+
+// element e of a piece as fp32 bits
+template <typename KT, int B>
+__device__ __forceinline__ uint32_t element(const Raw<B>& x, int e) {
+  if constexpr (sizeof(KT) == 4) {
+    return x.r[e];
+  } else if constexpr (std::is_same<KT, __nv_bfloat16>::value) {
+    return e & 1 ? x.r[e >> 1] & 0xFFFF0000u : x.r[e >> 1] << 16;
+  } else {
+    const __half h = __ushort_as_half((unsigned short)(e & 1 ? x.r[e >> 1] >> 16 : x.r[e >> 1] & 0xFFFFu));
+    return __float_as_uint(__half2float(h));
+  }
+}
+
+// what the upper tf32 part leaves of x (0 of an infinity)
+__device__ __forceinline__ uint32_t tf32_rest(uint32_t x) {
+  const float f = __uint_as_float(x), r = f - __uint_as_float(tf32_hi(x));
+  return fabsf(f) == INFINITY ? 0u : __float_as_uint(r);
+}
+
+__device__ __forceinline__ int page_index(const AttnArgs& a, int key) {
+  return (int)(((uint64_t)(uint32_t)key * a.ps_mul) >> a.ps_shift);
+}
+
+// first visible key and end of request b
+__device__ __forceinline__ void visible(const AttnArgs& a, int b, int& lo, int& hi) {
+  hi = min(max(a.lens[b], 0), a.max_keys);
+  lo = a.window > 0 ? max(hi - a.window, 0) : 0;
+}
+
+// UNI: page_size is a multiple of 16, so 16 (or 8) keys from a multiple of 16 share a page
+template <typename KT, int D, bool UNI>
+__global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnArgs a) {
+  constexpr int KI = keys_per_step<KT, D>(), NT = KI / 8, TK = NW * KI;
+  constexpr bool WIDE = sizeof(KT) == 4;          // keys and values need a lower part
+  constexpr int KE = 16 / sizeof(KT);             // elements of a key piece; 4 lanes cover 4 * KE dimensions
+  constexpr int KC = D / (4 * KE);
+  constexpr int VE = sizeof(KT) == 2 && D % 64 == 0 ? 8 : 4;  // of a value piece; 8 lanes cover 8 * VE
+  constexpr int VC = D / (8 * VE);
+  constexpr int VB = VE * (int)sizeof(KT);
+  constexpr int GK = UNI ? (KI >= 16 ? KI / 16 : 1) : NT;  // page lookups of a step: per 16 keys, or per 8 and row
+  __shared__ __align__(16) uint32_t sq[D / 8][32][4];      // q as product operands, lower parts in rows 8..15
+  __shared__ float so[NW][HT][D];
+  __shared__ float sm[NW][HT], sl[NW][HT];
   dep_wait();
   dep_release();
-  const int h = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t b = blockIdx.y;
-  const int g = h / (a.heads / a.kv_heads);
-  const int64_t len = min((int64_t)max(a.lens[b], 0), a.max_blocks * a.ps);
-  const int64_t lo = a.window > 0 ? max(len - a.window, (int64_t)0) : 0;
-  float q[E], acc[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = cv3p::load_any(a.q, a.q_type, b * a.qsb + h * a.qsh + lane * E + e) * a.scale;
-    acc[e] = 0.f;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = lane >> 2, t = lane & 3;
+  const int per = a.kv_heads * a.groups;  // pairs of a request
+  const int c = blockIdx.x;
+
+  // requests without keys: zeros, nothing to join
+  for (int b = c; b < a.batch; b += gridDim.x) {
+    int lo, hi;
+    visible(a, b, lo, hi);
+    if (hi > lo) continue;
+    for (int i = tid; i < a.heads * D; i += NW * 32)
+      cv3p::store_any(a.out, a.q_type, b * a.osb + (i / D) * a.osh + i % D, 0.f);
+    if (a.lse)
+      for (int i = tid; i < a.heads; i += NW * 32) a.lse[(int64_t)b * a.heads + i] = -INFINITY;
+    for (int i = tid; i < per; i += NW * 32) a.cut[(int64_t)b * per + i] = make_int2(0, 0);
   }
-  for (int64_t j = lo + warp; j < len; j += AW) {
-    const int64_t blk = j / a.ps, r = j - blk * a.ps;
-    const int page = a.tables[b * a.ld + blk];
-    if (page < 0 || page >= a.pages) {
-      if (a.bad && h == 0 && lane == 0 && (r == 0 || j == lo)) atomicAdd(a.bad, 1);
-      continue;
+
+  // the whole line and this CTA's piece of it; every warp finds it by itself
+  auto tiles_of = [&](int b) -> int {
+    int lo, hi;
+    visible(a, b, lo, hi);
+    return hi > lo ? (hi - (lo & -KI) + TK - 1) / TK : 0;
+  };
+  int64_t W = 0;
+  for (int b = lane; b < a.batch; b += 32) W += tiles_of(b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) W += __shfl_xor_sync(0xffffffffu, W, o);
+  W *= per;
+  const int64_t C = min((int64_t)gridDim.x, W);  // every CTA that works has a tile
+  if (c >= C) return;
+  int64_t u = W * c / C;
+  const int64_t u_end = W * (c + 1) / C;
+  int b = 0;
+  int64_t before = 0;  // tiles of the requests before b (one pair each)
+  for (int b0 = 0;; b0 += 32) {
+    const int64_t mine = b0 + lane < a.batch ? tiles_of(b0 + lane) : 0;
+    int64_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
     }
-    const KT* kr = static_cast<const KT*>(a.k) + page * a.ksp + g * a.ksh + r * a.kst + lane * E;
-    const KT* vr = static_cast<const KT*>(a.v) + page * a.vsp + g * a.vsh + r * a.vst + lane * E;
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], cv3p::to_f32<KT>(kr[e]), s);
-    s = warp_sum(s);
-    const float mn = fmaxf(m, s);
-    const float c = m == -INFINITY ? 0.f : expf(m - mn), p = s == -INFINITY ? 0.f : expf(s - mn);
-    m = mn;
-    l = l * c + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * c + p * cv3p::to_f32<KT>(vr[e]);
+    const unsigned past = __ballot_sync(0xffffffffu, (before + sum) * per > u);
+    if (past) {
+      const int at = __ffs(past) - 1;
+      b = b0 + at;
+      before += __shfl_sync(0xffffffffu, sum - mine, at);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
   }
+
+  while (u < u_end) {
+    // the pair that u lies in
+    int lo, hi;
+    visible(a, b, lo, hi);
+    const int tiles = hi > lo ? (hi - (lo & -KI) + TK - 1) / TK : 0;
+    if (tiles == 0) { ++b; continue; }
+    const int64_t u_b = before * per;
+    const int pair = (int)((u - u_b) / tiles);
+    if (pair >= per) { before += tiles; ++b; continue; }
+    const int64_t u0 = u_b + (int64_t)pair * tiles;
+    const int t0 = (int)(u - u0), t1 = (int)min((int64_t)tiles, u_end - u0);
+    const int g = pair / a.groups, h0 = g * a.group + (pair - g * a.groups) * HT;
+    const int nh = min(HT, (g + 1) * a.group - h0);
+    const bool whole = t0 == 0 && t1 == tiles;
+    u = u0 + t1;
+
+    __syncthreads();  // the last pair's shared memory is done with
+    for (int i = tid; i < D / 8 * 32; i += NW * 32) {
+      const int s = i >> 5, ln = i & 31, row = ln >> 2;
+      const int d = s / (KE / 2) * 4 * KE + (ln & 3) * KE + s % (KE / 2) * 2;
+      uint32_t v[4] = {0u, 0u, 0u, 0u};
+      if (row < nh) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) part[warp][lane * E + e] = acc[e];
-  if (lane == 0) { pm[warp] = m; pl[warp] = l; }
-  __syncthreads();
-  float M = -INFINITY, L = 0.f;
-  for (int w = 0; w < AW; ++w) M = fmaxf(M, pm[w]);
-  for (int w = 0; w < AW; ++w) L += pl[w] == 0.f ? 0.f : pl[w] * expf(pm[w] - M);  // (a NaN score: l is NaN)
-  for (int e = threadIdx.x; e < D; e += AW * 32) {
-    float o = 0.f;
-    for (int w = 0; w < AW; ++w) o += pl[w] == 0.f ? 0.f : part[w][e] * expf(pm[w] - M);
-    cv3p::store_any(a.out, a.q_type, b * a.osb + h * a.osh + e, L == 0.f ? 0.f : o / L);
+        for (int e = 0; e < 2; ++e) {
+          const float x = cv3p::load_any(a.q, a.q_type, b * a.qsb + (h0 + row) * a.qsh + d + e) * (a.scale * LOG2E);
+          const uint32_t r = tf32_rest(__float_as_uint(x));
+          v[2 * e] = tf32_hi(__float_as_uint(x));
+          v[2 * e + 1] = (r & 0x7FFFFFFFu) ? r : __float_as_uint(copysignf(TINY, x));
+        }
+      }
+      *reinterpret_cast<uint4*>(&sq[s][ln][0]) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+    __syncthreads();
+
+    const KT* kb = static_cast<const KT*>(a.k) + g * a.ksh;
+    const KT* vb = static_cast<const KT*>(a.v) + g * a.vsh;
+    const int* table = a.tables + b * a.ld;
+    const bool counts = a.bad && pair == 0;
+    float o[D / 8][2], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = 0.f;
+
+    // the page of a key, -1 for none; `mine`: this lane counts a bad one
+    auto page_of = [&](int key, bool mine) -> int {
+      if (key < lo || key >= hi) return -1;
+      const int blk = page_index(a, key);
+      const int p = table[blk];
+      const bool ok = (unsigned)p < (unsigned)a.pages;
+      if (!ok && counts && mine && (key == lo || key == blk * a.ps)) atomicAdd(a.bad, 1);
+      return ok ? p : -1;
+    };
+
+    Raw<16> kr[NT][KC];
+    Raw<VB> vr[NT][2][VC];
+    const int first = (lo & -KI) + t0 * TK + warp * KI, end = min(hi, (lo & -KI) + t1 * TK);
+    // pages of a step: UNI: of its 16-key groups (any visible key of one names it); else of the rows
+    // that this lane reads: key n, values 2t and 2t + 1 of each 8 keys
+    int pg[GK][UNI ? 1 : 3];
+    auto look = [&](int key0) {
+#pragma unroll
+      for (int i = 0; i < GK; ++i) {
+        if constexpr (UNI) {
+          const int k0 = key0 + i * 16;
+          pg[i][0] = k0 < hi && k0 + min(KI, 16) > lo ? page_of(max(k0, lo), lane == 0) : -1;
+        } else {
+          pg[i][0] = page_of(key0 + i * 8 + n, false);
+          pg[i][1] = page_of(key0 + i * 8 + 2 * t, n == 0);
+          pg[i][2] = page_of(key0 + i * 8 + 2 * t + 1, n == 0);
+        }
+      }
+    };
+    auto row_of = [&](int key) -> int { return key - page_index(a, key) * a.ps; };
+    auto load_k = [&](int key0) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int key = key0 + i * 8 + n;
+        const int p = UNI ? pg[i / 2][0] : pg[i][0];
+        const bool ok = p >= 0 && key >= lo && key < hi;
+        const KT* src = kb + (int64_t)p * a.ksp + (int64_t)row_of(key) * a.kst + t * KE;
+#pragma unroll
+        for (int x = 0; x < KC; ++x) fetch(kr[i][x], src + x * 4 * KE, ok);
+      }
+    };
+    auto load_v = [&](int key0) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int key = key0 + i * 8 + 2 * t + r;
+          const int p = UNI ? pg[i / 2][0] : pg[i][1 + r];
+          const bool ok = p >= 0 && key >= lo && key < hi;
+          const KT* src = vb + (int64_t)p * a.vsp + (int64_t)row_of(key) * a.vst + n * VE;
+#pragma unroll
+          for (int x = 0; x < VC; ++x) fetch(vr[i][r][x], src + x * 8 * VE, ok);
+        }
+      }
+    };
+
+    if (first < end) {
+      look(first);
+      load_k(first);
+    }
+    for (int key0 = first; key0 < end; key0 += TK) {
+      load_v(key0);
+      // which of this lane's scores (keys 2t, 2t + 1 of each 8) count
+      bool seen[NT][2];
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int key = key0 + i * 8 + 2 * t + r;
+          seen[i][r] = (UNI ? pg[i / 2][0] : pg[i][1 + r]) >= 0 && key >= lo && key < hi;
+        }
+      const int next = key0 + TK;
+      if (next < end) look(next);
+      float s0[NT][4], s1[NT][4];  // two chains: even and odd steps, or upper and lower parts of the keys
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s0[i][e] = s1[i][e] = 0.f;
+#pragma unroll
+      for (int s = 0; s < D / 8; ++s) {
+        const uint4 q4 = *reinterpret_cast<const uint4*>(&sq[s][lane][0]);
+        const uint32_t qa[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const uint32_t b0 = element<KT>(kr[i][s / (KE / 2)], s % (KE / 2) * 2);
+          const uint32_t b1 = element<KT>(kr[i][s / (KE / 2)], s % (KE / 2) * 2 + 1);
+          if constexpr (WIDE) {
+            mma_tf32(s0[i], qa, tf32_hi(b0), tf32_hi(b1));
+            mma_tf32(s1[i], qa, tf32_rest(b0), tf32_rest(b1));
+          } else {
+            mma_tf32(s & 1 ? s1[i] : s0[i], qa, b0, b1);
+          }
+        }
+      }
+      if (next < end) load_k(next);
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float x = (s0[i][r] + s1[i][r]) + (s0[i][2 + r] + s1[i][2 + r]);
+          s0[i][r] = seen[i][r] ? x : -INFINITY;
+          top = fmaxf(top, s0[i][r]);
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float fade = exp2_fast(m - ref);
+      m = top;
+      l *= fade;
+      uint32_t p[NT][4];
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float x = exp2_fast(s0[i][r] - ref);
+          l += x;
+          p[i][2 * r] = tf32_hi(__float_as_uint(x));
+          p[i][2 * r + 1] = __float_as_uint(fmaxf(x - __uint_as_float(p[i][2 * r]), TINY));
+        }
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const uint32_t b0 = element<KT>(vr[i][0][j / VE], j % VE), b1 = element<KT>(vr[i][1][j / VE], j % VE);
+          if constexpr (WIDE) {
+            mma_tf32(acc, p[i], tf32_hi(b0), tf32_hi(b1));
+            mma_tf32(acc, p[i], tf32_rest(b0), tf32_rest(b1));
+          } else {
+            mma_tf32(acc, p[i], b0, b1);
+          }
+        }
+        o[j][0] = fmaf(o[j][0], fade, acc[0] + acc[2]);
+        o[j][1] = fmaf(o[j][1], fade, acc[1] + acc[3]);
+      }
+    }
+
+    // the warps' shares of the pair
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (t == 0) { sm[warp][n] = m; sl[warp][n] = l; }
+#pragma unroll
+    for (int x = 0; x < VC; ++x)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        so[warp][n][x * 8 * VE + 2 * t * VE + e] = o[x * VE + e][0];
+        so[warp][n][x * 8 * VE + (2 * t + 1) * VE + e] = o[x * VE + e][1];
+      }
+    __syncthreads();
+    const int slot = t0 > 0 ? 0 : 1;
+    for (int i = tid; i < nh * D; i += NW * 32) {
+      const int h = i / D, e = i - h * D;
+      float M = -INFINITY, L = 0.f, x = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w][h]);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        if (sl[w][h] == 0.f) continue;  // saw nothing (a NaN score leaves a NaN sum)
+        const float f = exp2_fast(sm[w][h] - M);
+        L = fmaf(sl[w][h], f, L);
+        x = fmaf(so[w][h][e], f, x);
+      }
+      if (whole) {
+        cv3p::store_any(a.out, a.q_type, b * a.osb + (h0 + h) * a.osh + e, L == 0.f ? 0.f : x / L);
+        if (a.lse && e == 0) a.lse[(int64_t)b * a.heads + h0 + h] = L == 0.f ? -INFINITY : (M + log2f(L)) / LOG2E;
+      } else {
+        const int64_t at = ((int64_t)c * 2 + slot) * HT + h;
+        a.part[at * D + e] = x;
+        if (e == 0) { a.stat[at * 2] = M; a.stat[at * 2 + 1] = L; }
+      }
+    }
+    if (t0 == 0 && tid == 0) {  // who holds the pair: CTA x has the tiles from W * x / C on
+      const int last = (int)(((u0 + tiles) * C - 1) / W);
+      a.cut[(int64_t)b * per + pair] = whole ? make_int2(0, 0) : make_int2(c, last - c + 1);
+    }
   }
-  if (a.lse && threadIdx.x == 0) a.lse[b * a.heads + h] = L == 0.f ? -INFINITY : M + logf(L);
 }
 
+// Joins the parts of every pair that was cut.  WPH warps share a head: one where there are pairs
+// enough to fill the GPU, all of them where few long pairs have many parts each.
+template <int D, int WPH>
+__global__ void __launch_bounds__(NW * 32) paged_join_kernel(const AttnArgs a) {
+  constexpr int E = D / 32;
+  __shared__ float so[NW][D], sm[NW], sl[NW];
+  dep_wait();
+  dep_release();
+  const int pair = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.y * (NW / WPH) + warp / WPH;
+  const int2 cut = a.cut[pair];
+  if (cut.y == 0) return;
+  const int per = a.kv_heads * a.groups, b = pair / per, r = pair - b * per;
+  const int g = r / a.groups, h0 = g * a.group + (r - g * a.groups) * HT;
+  const int nh = min(HT, (g + 1) * a.group - h0);
+  float M = -INFINITY, L = 0.f, x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = 0.f;
+  if (h < nh) {
+    // part i: the pair's first CTA left it in slot 1, the others in slot 0
+    for (int i0 = warp % WPH; i0 < cut.y; i0 += 4 * WPH) {
+      float pm[4], pl[4], px[4][E];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * WPH;
+        pm[u] = -INFINITY;
+        pl[u] = 0.f;
+        if (i < cut.y) {
+          const int64_t at = ((int64_t)(cut.x + i) * 2 + (i == 0)) * HT + h;
+          pm[u] = a.stat[at * 2];
+          pl[u] = a.stat[at * 2 + 1];
+#pragma unroll
+          for (int e = 0; e < E; ++e) px[u][e] = a.part[at * D + e * 32 + lane];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (pl[u] == 0.f) continue;
+        const float top = fmaxf(M, pm[u]), f = L == 0.f ? 0.f : exp2_fast(M - top), w = exp2_fast(pm[u] - top);
+        M = top;
+        L = L * f + pl[u] * w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = x[e] * f + px[u][e] * w;
+      }
+    }
+  }
+  if constexpr (WPH > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) so[warp][e * 32 + lane] = x[e];
+    if (lane == 0) { sm[warp] = M; sl[warp] = L; }
+    __syncthreads();
+    if (warp % WPH) return;
+    for (int w = 1; w < WPH; ++w) {
+      if (sl[warp + w] == 0.f) continue;
+      const float top = fmaxf(M, sm[warp + w]), f = L == 0.f ? 0.f : exp2_fast(M - top), y = exp2_fast(sm[warp + w] - top);
+      M = top;
+      L = L * f + sl[warp + w] * y;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = x[e] * f + so[warp + w][e * 32 + lane] * y;
+    }
+  }
+  if (h >= nh) return;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    cv3p::store_any(a.out, a.q_type, b * a.osb + (h0 + h) * a.osh + e * 32 + lane, L == 0.f ? 0.f : x[e] / L);
+  if (a.lse && lane == 0) a.lse[(int64_t)b * a.heads + h0 + h] = L == 0.f ? -INFINITY : (M + log2f(L)) / LOG2E;
+}
+
+using Fn = void (*)(const AttnArgs);
+
 template <typename KT>
-void (*pick(int64_t d))(const AttnArgs) {
+Fn pick(int64_t d, bool uni) {
   switch (d) {
-    case 32: return paged_attention_kernel<KT, 32>;
-    case 64: return paged_attention_kernel<KT, 64>;
-    case 96: return paged_attention_kernel<KT, 96>;
-    default: return paged_attention_kernel<KT, 128>;
+    case 32: return uni ? paged_attention_kernel<KT, 32, true> : paged_attention_kernel<KT, 32, false>;
+    case 64: return uni ? paged_attention_kernel<KT, 64, true> : paged_attention_kernel<KT, 64, false>;
+    case 96: return uni ? paged_attention_kernel<KT, 96, true> : paged_attention_kernel<KT, 96, false>;
+    default: return uni ? paged_attention_kernel<KT, 128, true> : paged_attention_kernel<KT, 128, false>;
   }
 }
+
+Fn pick_join(int64_t d, bool wide) {
+  switch (d) {
+    case 32: return wide ? paged_join_kernel<32, NW> : paged_join_kernel<32, 1>;
+    case 64: return wide ? paged_join_kernel<64, NW> : paged_join_kernel<64, 1>;
+    case 96: return wide ? paged_join_kernel<96, NW> : paged_join_kernel<96, 1>;
+    default: return wide ? paged_join_kernel<128, NW> : paged_join_kernel<128, 1>;
+  }
+}
+
+int64_t pairs_of(int64_t batch, int64_t heads, int64_t kv_heads) {
+  return batch * kv_heads * ((heads / kv_heads + HT - 1) / HT);
+}
+
+// two CTAs on every SM; fewer where the table holds fewer tiles (of the smallest kind: 8 keys a warp)
+int64_t grid_of(int64_t pairs, int64_t max_len) {
+  return std::max<int64_t>(1, std::min<int64_t>(2 * cv3::sm_count(), pairs * ((max_len + NW * 8 - 1) / (NW * 8) + 1)));
+}
+
+int64_t floats_of(int64_t pairs, int64_t grid, int64_t d) { return 2 * pairs + grid * 2 * HT * (d + 2); }
 
 }  // namespace
 
 extern "C" int64_t cv3_paged_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                                  int64_t max_len) {
-  return 0;
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
+  const int64_t pairs = pairs_of(batch, heads, kv_heads);
+  return floats_of(pairs, grid_of(pairs, max_len), head_dim);
 }
 
 extern "C" int cv3_paged_attention(const void* q, int q_type, int64_t qsb, int64_t qsh, const void* k_pages,
@@ -116,13 +541,33 @@ extern "C" int cv3_paged_attention(const void* q, int q_type, int64_t qsb, int64
   const int ce = 16 / cv3p::type_size(kv_type);
   CV3_REQUIRE(cv3p::aligned16(k_pages) && cv3p::aligned16(v_pages) && (ksp | ksh | kst | vsp | vsh | vst) % ce == 0,
               CV3_ERR_VALUE, "paged_attention: cache rows must start on 16-byte boundaries");
-  CV3_REQUIRE(max_blocks * page_size <= INT32_MAX, CV3_ERR_VALUE, "paged_attention: positions are 32-bit numbers");
+  // (a tile behind the last key must not pass 2^31 either)
+  CV3_REQUIRE(page_size <= INT32_MAX && max_blocks * page_size <= INT32_MAX - 4096 && num_pages <= INT32_MAX && batch <= INT32_MAX, CV3_ERR_VALUE,
+              "paged_attention: positions and pages are 32-bit numbers");
   if (batch == 0) return CV3_OK;
-  const AttnArgs a = {q, q_type, qsb, qsh, k_pages, v_pages, ksp, ksh, kst, vsp, vsh, vst, num_pages, page_size,
-                      block_tables, table_ld, max_blocks, lens, (int)heads, (int)kv_heads, window, scale, out, osb, osh,
-                      lse, bad};
-  const auto fn = kv_type == CV3_TYPE_F32 ? pick<float>(head_dim)
-                  : kv_type == CV3_TYPE_F16 ? pick<__half>(head_dim) : pick<__nv_bfloat16>(head_dim);
-  return cv3::check_launch("paged_attention", cv3::launch_dep(fn, dim3((unsigned)heads, (unsigned)batch), dim3(AW * 32), 0,
-                                                              cv3::as_stream(stream), a));
+  const int64_t pairs = pairs_of(batch, heads, kv_heads), max_len = max_blocks * page_size;
+  const int64_t grid = grid_of(pairs, max_len);
+  CV3_REQUIRE(pairs <= INT32_MAX, CV3_ERR_VALUE, "paged_attention: too many requests and heads");
+  CV3_REQUIRE(workspace && workspace_floats >= floats_of(pairs, grid, head_dim) && ((uintptr_t)workspace & 7) == 0,
+              CV3_ERR_VALUE, "paged_attention: the workspace must hold cv3_paged_attention_workspace() floats");
+  // n / ps by a product: with shift s = 32 + ceil(log2 ps) the error of mul = ceil(2^s / ps) < 2^33 is too small to
+  // reach a quotient for n < 2^31; mul itself must stay below 2^32, so one step less for n < 2^31
+  int sh = 0;
+  while ((int64_t)1 << sh < page_size) ++sh;
+  const uint32_t mul = (uint32_t)((((uint64_t)1 << (31 + sh)) + page_size - 1) / page_size);
+  float* stat = workspace + 2 * pairs;
+  const AttnArgs a = {q, q_type, qsb, qsh, k_pages, v_pages, ksp, ksh, kst, vsp, vsh, vst, num_pages, (int)page_size, mul,
+                      (uint32_t)(31 + sh), block_tables, table_ld, (int)max_len, lens, (int)batch, (int)heads,
+                      (int)kv_heads, (int)(heads / kv_heads), (int)((heads / kv_heads + HT - 1) / HT),
+                      (int)std::min<int64_t>(window, INT32_MAX), scale, out, osb, osh, lse, bad,
+                      stat + grid * 2 * HT * 2, stat, reinterpret_cast<int2*>(workspace)};
+  const bool uni = page_size % 16 == 0;
+  const Fn fn = kv_type == CV3_TYPE_F32   ? pick<float>(head_dim, uni)
+                : kv_type == CV3_TYPE_F16 ? pick<__half>(head_dim, uni) : pick<__nv_bfloat16>(head_dim, uni);
+  cudaStream_t st = cv3::as_stream(stream);
+  int rc = cv3::check_launch("paged_attention", cv3::launch_dep(fn, dim3((unsigned)grid), dim3(NW * 32), 0, st, a));
+  if (rc || grid == 1) return rc;
+  const bool wide = pairs <= 64;
+  return cv3::check_launch("paged_join", cv3::launch_dep(pick_join(head_dim, wide), dim3((unsigned)pairs, wide ? HT : 1),
+                                                         dim3(NW * 32), 0, st, a));
 }

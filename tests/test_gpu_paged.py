@@ -340,7 +340,9 @@ def test_attention_extreme_values():
     vv = v[:1].copy()
     vv[0, 0, 4, 3] = np.inf
     got = ops.paged_attention(_cuda(q1), _cuda(kk), _cuda(vv), _cuda(one), _cuda(np.array([5], np.int32)))
-    assert float(got[0, 0, 3]) == np.inf and torch.equal(got[0, 0, 4:].cpu(), torch.from_numpy(vv[0, 0, 4, 4:]))
+    # one key counts, so the result is its value; values enter the products as two tf32 parts: what the upper part
+    # (11 bits) leaves is below 2^-10 of the value and keeps 11 bits itself, so less than 2^-20 of the value is lost
+    assert float(got[0, 0, 3]) == np.inf and np.all(np.abs(_np(got)[0, 0, 4:] - vv[0, 0, 4, 4:]) <= 2.0 ** -20 * np.abs(vv[0, 0, 4, 4:]))
     kk[0, 0, 2, 5] = np.nan
     got = ops.paged_attention(_cuda(q1), _cuda(kk), _cuda(vv), _cuda(one), _cuda(np.array([5], np.int32)))
     assert bool(got.isnan().all())
