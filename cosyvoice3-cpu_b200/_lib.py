@@ -100,16 +100,13 @@ SIGNATURES = {
     "cv3_q8_decode_gemv_mma": [P, I64, I64, I64, P, P, I64, I64, P, P, P, F, I32, P, I64, I64, P, I64, P, P],
     "cv3_decode_gemv_status": [P],
     "cv3_decode_attention_status": [P],
-    "cv3_paged_extend": [P, P, P, I64, P, I64, I64, I64, P, I64, P, I64, P, P, P, P, P, P, P, P],
-    "cv3_paged_append": [P, I32, I64, I64, P, P, I64, P, P, I64, I64, I64, P, P, P, I32, I64, I64, I64, I64, I64, I64,
-                         I64, I64, P, P],
-    "cv3_paged_attention": [P, I32, I64, I64, P, P, I32, I64, I64, I64, I64, I64, I64, I64, I64, P, I64, I64, P, I64,
-                            I64, I64, I64, I64, F, P, I64, I64, P, P, P, I64, P],
-    "cv3_paged_attention_workspace": [I64, I64, I64, I64, I64],
-    "cv3_beam_select": [P, I32, I64, I64, I64, I64, P, P, P, I64, I64, P, D, P, P, P, P, P, P, I64, P],
+    "cv3_paged_extend": [P, P],
+    "cv3_paged_append": [P, P],
+    "cv3_paged_attention": [P, P],
+    "cv3_paged_attention_workspace": [I64, I64, I64, I64, I32, I64],
+    "cv3_beam_select": [P, P],
     "cv3_beam_workspace": [I64, I64, I64],
-    "cv3_paged_reorder": [P, P, I32, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, P, I64, I64, P, P,
-                          I64, I64, P],
+    "cv3_paged_reorder": [P, P],
 }
 _RESTYPE = {"cv3_last_error": ctypes.c_char_p, "cv3_launch_count": ctypes.c_ulonglong,
             "cv3_decode_sync_words": ctypes.c_int64, "cv3_paged_attention_workspace": ctypes.c_int64,

@@ -236,29 +236,28 @@ extern "C" int64_t cv3_beam_workspace(int64_t groups, int64_t beams, int64_t voc
   return groups * beams * chunks_of(vocab) * (16 + 8 * beams);
 }
 
-extern "C" int cv3_beam_select(const void* logits, int type, int64_t ld, int64_t groups, int64_t beams, int64_t vocab,
-                               const float* scores, const int* counts, const int* done, int64_t stop_lo, int64_t stop_hi,
-                               const int* min_len, double length_penalty, int64_t* tokens, int* parents,
-                               float* scores_out, int* counts_out, int* done_out, void* workspace,
-                               int64_t workspace_bytes, void* stream) {
-  CV3_REQUIRE(groups >= 0 && vocab > 0 && vocab <= INT32_MAX && ld >= vocab && stop_lo <= stop_hi, CV3_ERR_VALUE,
-              "beam_select: bad shape");
-  CV3_REQUIRE(beams > 0 && beams <= CV3_MAX_BEAMS, CV3_ERR_UNSUPPORTED, "beam_select: %lld beams (1 to %d)",
-              (long long)beams, CV3_MAX_BEAMS);
-  CV3_REQUIRE(cv3p::type_ok(type), CV3_ERR_VALUE, "beam_select: unknown element type");
-  CV3_REQUIRE(groups * beams <= 65535, CV3_ERR_UNSUPPORTED, "beam_select: more than 65535 hypotheses");
-  if (groups == 0) return CV3_OK;
-  const int64_t chunks = chunks_of(vocab), n = groups * beams * chunks;
-  CV3_REQUIRE(workspace && workspace_bytes >= cv3_beam_workspace(groups, beams, vocab) && ((uintptr_t)workspace & 7) == 0,
+extern "C" int cv3_beam_select(const cv3_beam_params* p, void* stream) {
+  CV3_REQUIRE(p && p->size == (int64_t)sizeof(*p), CV3_ERR_VALUE, "beam_select: bad parameter block");
+  CV3_REQUIRE(p->groups >= 0 && p->vocab > 0 && p->vocab <= INT32_MAX && p->ld >= p->vocab && p->stop_lo <= p->stop_hi,
+              CV3_ERR_VALUE, "beam_select: bad shape");
+  CV3_REQUIRE(p->beams > 0 && p->beams <= CV3_MAX_BEAMS, CV3_ERR_UNSUPPORTED, "beam_select: %lld beams (1 to %d)",
+              (long long)p->beams, CV3_MAX_BEAMS);
+  CV3_REQUIRE(cv3p::type_ok(p->type), CV3_ERR_VALUE, "beam_select: unknown element type");
+  CV3_REQUIRE(p->groups <= 65535 && p->groups * p->beams <= 65535, CV3_ERR_UNSUPPORTED,
+              "beam_select: more than 65535 hypotheses");
+  if (p->groups == 0) return CV3_OK;
+  const int64_t chunks = chunks_of(p->vocab), n = p->groups * p->beams * chunks;
+  CV3_REQUIRE(p->workspace && p->workspace_bytes >= cv3_beam_workspace(p->groups, p->beams, p->vocab) &&
+                  ((uintptr_t)p->workspace & 7) == 0,
               CV3_ERR_VALUE, "beam_select: the workspace must hold cv3_beam_workspace() bytes");
-  char* w = static_cast<char*>(workspace);
-  const BeamArgs a = {logits, type, ld, groups, (int)beams, vocab, scores, counts, done, stop_lo, stop_hi, min_len,
-                      length_penalty, tokens, parents, scores_out, counts_out, done_out, chunks,
-                      reinterpret_cast<double*>(w), reinterpret_cast<float*>(w + 8 * n),
+  char* w = static_cast<char*>(p->workspace);
+  const BeamArgs a = {p->logits, (int)p->type, p->ld, p->groups, (int)p->beams, p->vocab, p->scores, p->counts, p->done,
+                      p->stop_lo, p->stop_hi, p->min_len, p->length_penalty, p->tokens, p->parents, p->scores_out,
+                      p->counts_out, p->done_out, chunks, reinterpret_cast<double*>(w), reinterpret_cast<float*>(w + 8 * n),
                       reinterpret_cast<unsigned long long*>(w + 16 * n)};
   cudaStream_t st = cv3::as_stream(stream);
-  int rc = cv3::check_launch("beam_scan", cv3::launch_dep(beam_scan_kernel, dim3((unsigned)chunks, (unsigned)(groups * beams)),
+  int rc = cv3::check_launch("beam_scan", cv3::launch_dep(beam_scan_kernel, dim3((unsigned)chunks, (unsigned)(p->groups * p->beams)),
                                                           dim3(BT), 0, st, a));
   if (rc) return rc;
-  return cv3::check_launch("beam_pick", cv3::launch_dep(beam_pick_kernel, dim3((unsigned)groups), dim3(BT), 0, st, a));
+  return cv3::check_launch("beam_pick", cv3::launch_dep(beam_pick_kernel, dim3((unsigned)p->groups), dim3(BT), 0, st, a));
 }

@@ -321,52 +321,49 @@ __global__ void __launch_bounds__(256) reorder_kernel(const ReorderArgs a) {
 
 }  // namespace
 
-extern "C" int cv3_paged_extend(const int* lens, const int* new_lens, const int* release, int64_t batch,
-                                int* block_tables, int64_t table_ld, int64_t max_blocks, int64_t page_size,
-                                int* free_pages, int64_t free_cap, const int* free_count, int64_t max_tokens,
-                                int64_t* slots, int* seq, int* pos, int* offsets, int* lens_out, int* free_count_out,
-                                int* scratch, void* stream) {
-  CV3_REQUIRE(batch >= 0 && max_blocks >= 0 && table_ld >= max_blocks && page_size > 0 && free_cap >= 0 && max_tokens >= 0,
+extern "C" int cv3_paged_extend(const cv3_paged_extend_params* p, void* stream) {
+  CV3_REQUIRE(p && p->size == (int64_t)sizeof(*p), CV3_ERR_VALUE, "paged_extend: bad parameter block");
+  CV3_REQUIRE(p->batch >= 0 && p->max_blocks >= 0 && p->table_ld >= p->max_blocks && p->page_size > 0 &&
+                  p->free_cap >= 0 && p->max_tokens >= 0,
               CV3_ERR_VALUE, "paged_extend: bad shape");
-  CV3_REQUIRE(max_tokens <= INT32_MAX && free_cap <= INT32_MAX && max_blocks * page_size <= INT32_MAX, CV3_ERR_VALUE,
-              "paged_extend: rows, pages and a request's positions are 32-bit numbers");
-  const ExtendArgs a = {lens, new_lens, release, batch, block_tables, table_ld, max_blocks, page_size, free_pages,
-                        free_cap, free_count, max_tokens, slots, seq, pos, offsets, lens_out, free_count_out, scratch};
+  CV3_REQUIRE(p->max_tokens <= INT32_MAX && p->free_cap <= INT32_MAX && p->page_size <= INT32_MAX &&
+                  p->max_blocks <= INT32_MAX && p->max_blocks * p->page_size <= INT32_MAX,
+              CV3_ERR_VALUE, "paged_extend: rows, pages and a request's positions are 32-bit numbers");
+  const ExtendArgs a = {p->lens, p->new_lens, p->release, p->batch, p->block_tables, p->table_ld, p->max_blocks,
+                        p->page_size, p->free_pages, p->free_cap, p->free_count, p->max_tokens, p->slots, p->seq, p->pos,
+                        p->offsets, p->lens_out, p->free_count_out, p->scratch};
   cudaStream_t st = cv3::as_stream(stream);
-  const int fused = max_tokens <= 4 * ET;
+  const int fused = p->max_tokens <= 4 * ET;
   int rc = cv3::check_launch("paged_extend", cv3::launch_dep(extend_scan_kernel, dim3(1), dim3(ET), 0, st, a, fused));
   if (rc || fused) return rc;
-  int64_t grid = (max_tokens + 255) / 256;
-  if (grid > cv3::sm_count() * 8) grid = cv3::sm_count() * 8;
+  const int64_t grid = std::min<int64_t>((p->max_tokens + 255) / 256, cv3::sm_count() * 8);
   return cv3::check_launch("paged_extend_rows",
                            cv3::launch_dep(extend_rows_kernel, dim3((unsigned)grid), dim3(256), 0, st, a));
 }
 
-extern "C" int cv3_paged_append(const void* qkv, int type, int64_t rows, int64_t ldq, const float* cos_table,
-                                const float* sin_table, int64_t positions, const int64_t* slots, const int* pos,
-                                int64_t heads, int64_t kv_heads, int64_t head_dim, void* q_out, void* k_pages,
-                                void* v_pages, int kv_type, int64_t ksp, int64_t ksh, int64_t kst, int64_t vsp,
-                                int64_t vsh, int64_t vst, int64_t num_pages, int64_t page_size, int* bad,
-                                void* stream) {
-  CV3_REQUIRE(rows >= 0 && heads > 0 && kv_heads > 0 && num_pages >= 0 && page_size > 0, CV3_ERR_VALUE,
-              "paged_append: bad shape");
-  CV3_REQUIRE(head_dim > 0 && head_dim % 16 == 0 && head_dim <= 256, CV3_ERR_UNSUPPORTED,
-              "paged_append: head_dim %lld (a multiple of 16 up to 256)", (long long)head_dim);
-  CV3_REQUIRE(cv3p::type_ok(type) && cv3p::type_ok(kv_type), CV3_ERR_VALUE, "paged_append: unknown element type");
-  CV3_REQUIRE((cos_table == nullptr) == (sin_table == nullptr) && (!cos_table || (pos && positions > 0)), CV3_ERR_VALUE,
-              "paged_append: cos and sin tables and positions go together");
-  CV3_REQUIRE(ldq >= (heads + 2 * kv_heads) * head_dim, CV3_ERR_VALUE, "paged_append: ldq too small");
-  const int ae = 16 / cv3p::type_size(type), ce = 16 / cv3p::type_size(kv_type);
-  CV3_REQUIRE(cv3p::aligned16(qkv) && cv3p::aligned16(q_out) && cv3p::aligned16(k_pages) && cv3p::aligned16(v_pages) &&
-                  ldq % ae == 0 && (ksp | ksh | kst | vsp | vsh | vst) % ce == 0,
+extern "C" int cv3_paged_append(const cv3_paged_append_params* p, void* stream) {
+  CV3_REQUIRE(p && p->size == (int64_t)sizeof(*p), CV3_ERR_VALUE, "paged_append: bad parameter block");
+  CV3_REQUIRE(p->rows >= 0 && p->heads > 0 && p->kv_heads > 0 && p->num_pages >= 0 && p->page_size > 0 &&
+                  p->heads + 2 * p->kv_heads <= INT32_MAX / 512,
+              CV3_ERR_VALUE, "paged_append: bad shape");
+  CV3_REQUIRE(p->head_dim > 0 && p->head_dim % 16 == 0 && p->head_dim <= 256, CV3_ERR_UNSUPPORTED,
+              "paged_append: head_dim %lld (a multiple of 16 up to 256)", (long long)p->head_dim);
+  CV3_REQUIRE(cv3p::type_ok(p->type) && cv3p::type_ok(p->kv_type), CV3_ERR_VALUE, "paged_append: unknown element type");
+  CV3_REQUIRE((p->cos_table == nullptr) == (p->sin_table == nullptr) && (!p->cos_table || (p->pos && p->positions > 0)),
+              CV3_ERR_VALUE, "paged_append: cos and sin tables and positions go together");
+  CV3_REQUIRE(p->ldq >= (p->heads + 2 * p->kv_heads) * p->head_dim, CV3_ERR_VALUE, "paged_append: ldq too small");
+  const int ae = 16 / cv3p::type_size((int)p->type), ce = 16 / cv3p::type_size((int)p->kv_type);
+  CV3_REQUIRE(cv3p::aligned16(p->qkv) && cv3p::aligned16(p->q_out) && cv3p::aligned16(p->k_pages) &&
+                  cv3p::aligned16(p->v_pages) && p->ldq % ae == 0 &&
+                  (p->ksp | p->ksh | p->kst | p->vsp | p->vsh | p->vst) % ce == 0,
               CV3_ERR_VALUE, "paged_append: rows must start on 16-byte boundaries");
-  if (rows == 0) return CV3_OK;
-  const AppendArgs a = {qkv, rows, ldq, cos_table, sin_table, positions, slots, pos, (int)heads, (int)kv_heads,
-                        (int)head_dim, q_out, k_pages, v_pages, ksp, ksh, kst, vsp, vsh, vst, num_pages, page_size, bad};
+  if (p->rows == 0) return CV3_OK;
+  const AppendArgs a = {p->qkv, p->rows, p->ldq, p->cos_table, p->sin_table, p->positions, p->slots, p->pos, (int)p->heads,
+                        (int)p->kv_heads, (int)p->head_dim, p->q_out, p->k_pages, p->v_pages, p->ksp, p->ksh, p->kst,
+                        p->vsp, p->vsh, p->vst, p->num_pages, p->page_size, p->bad};
   using Fn = void (*)(const AppendArgs);
   Fn fn = nullptr;
-  const int which = type * 3 + kv_type;
-  switch (which) {
+  switch ((int)p->type * 3 + (int)p->kv_type) {
     case 0: fn = append_kernel<float, float, 4>; break;
     case 1: fn = append_kernel<float, __half, 4>; break;
     case 2: fn = append_kernel<float, __nv_bfloat16, 4>; break;
@@ -377,36 +374,33 @@ extern "C" int cv3_paged_append(const void* qkv, int type, int64_t rows, int64_t
     case 7: fn = append_kernel<__nv_bfloat16, __half, 8>; break;
     default: fn = append_kernel<__nv_bfloat16, __nv_bfloat16, 8>; break;
   }
-  int64_t grid = rows;
-  if (grid > cv3::sm_count() * 8) grid = cv3::sm_count() * 8;
+  const int64_t grid = std::min<int64_t>(p->rows, cv3::sm_count() * 8);
   return cv3::check_launch("paged_append", cv3::launch_dep(fn, dim3((unsigned)grid), dim3(256), 0, cv3::as_stream(stream), a));
 }
 
-extern "C" int cv3_paged_reorder(void* k_pages, void* v_pages, int kv_type, int64_t layers, int64_t num_pages,
-                                 int64_t kv_heads, int64_t page_size, int64_t head_dim, int64_t ksl, int64_t ksp,
-                                 int64_t ksh, int64_t kst, int64_t vsl, int64_t vsp, int64_t vsh, int64_t vst,
-                                 int* block_tables, int64_t table_ld, int64_t max_blocks, const int* parents,
-                                 const int* lens, int64_t groups, int64_t beams, void* stream) {
-  CV3_REQUIRE(layers >= 0 && num_pages >= 0 && kv_heads > 0 && page_size > 0 && head_dim > 0 && groups >= 0 &&
-                  max_blocks >= 0 && table_ld >= max_blocks,
+extern "C" int cv3_paged_reorder(const cv3_paged_reorder_params* p, void* stream) {
+  CV3_REQUIRE(p && p->size == (int64_t)sizeof(*p), CV3_ERR_VALUE, "paged_reorder: bad parameter block");
+  CV3_REQUIRE(p->layers >= 0 && p->num_pages >= 0 && p->kv_heads > 0 && p->page_size > 0 && p->head_dim > 0 &&
+                  p->groups >= 0 && p->max_blocks >= 0 && p->table_ld >= p->max_blocks,
               CV3_ERR_VALUE, "paged_reorder: bad shape");
-  CV3_REQUIRE(beams > 0 && beams <= CV3_MAX_BEAMS, CV3_ERR_UNSUPPORTED, "paged_reorder: %lld beams (1 to %d)",
-              (long long)beams, CV3_MAX_BEAMS);
-  CV3_REQUIRE(cv3p::type_ok(kv_type), CV3_ERR_VALUE, "paged_reorder: unknown element type");
-  CV3_REQUIRE(groups <= 65535, CV3_ERR_UNSUPPORTED, "paged_reorder: more than 65535 groups");
-  const int64_t es = cv3p::type_size(kv_type);
-  CV3_REQUIRE(cv3p::aligned16(k_pages) && cv3p::aligned16(v_pages) && head_dim * es % 16 == 0 &&
-                  (ksl | ksp | ksh | kst | vsl | vsp | vsh | vst) * es % 16 == 0,
+  CV3_REQUIRE(p->beams > 0 && p->beams <= CV3_MAX_BEAMS, CV3_ERR_UNSUPPORTED, "paged_reorder: %lld beams (1 to %d)",
+              (long long)p->beams, CV3_MAX_BEAMS);
+  CV3_REQUIRE(cv3p::type_ok(p->kv_type), CV3_ERR_VALUE, "paged_reorder: unknown element type");
+  CV3_REQUIRE(p->groups <= 65535, CV3_ERR_UNSUPPORTED, "paged_reorder: more than 65535 groups");
+  const int64_t es = cv3p::type_size((int)p->kv_type);
+  CV3_REQUIRE(cv3p::aligned16(p->k_pages) && cv3p::aligned16(p->v_pages) && p->head_dim * es % 16 == 0 &&
+                  (p->ksl | p->ksp | p->ksh | p->kst | p->vsl | p->vsp | p->vsh | p->vst) * es % 16 == 0,
               CV3_ERR_VALUE, "paged_reorder: cache rows must be 16-byte pieces on 16-byte boundaries");
-  if (groups == 0 || beams == 1) return CV3_OK;
-  const ReorderArgs a = {static_cast<char*>(k_pages), static_cast<char*>(v_pages), ksl * es, ksp * es, ksh * es, kst * es,
-                         vsl * es, vsp * es, vsh * es, vst * es, layers, num_pages, kv_heads, page_size,
-                         head_dim * es / 16, block_tables, table_ld, max_blocks, parents, lens, groups, (int)beams};
-  const int64_t most = std::max<int64_t>(layers * 2 * kv_heads * (page_size - 1) * a.row16, max_blocks);
-  int64_t gx = std::max<int64_t>(1, std::min<int64_t>((most + 255) / 256, (cv3::sm_count() * 8 + groups - 1) / groups));
+  if (p->groups == 0 || p->beams == 1) return CV3_OK;
+  const ReorderArgs a = {static_cast<char*>(p->k_pages), static_cast<char*>(p->v_pages), p->ksl * es, p->ksp * es,
+                         p->ksh * es, p->kst * es, p->vsl * es, p->vsp * es, p->vsh * es, p->vst * es, p->layers,
+                         p->num_pages, p->kv_heads, p->page_size, p->head_dim * es / 16, p->block_tables, p->table_ld,
+                         p->max_blocks, p->parents, p->lens, p->groups, (int)p->beams};
+  const int64_t most = std::max<int64_t>(p->layers * 2 * p->kv_heads * (p->page_size - 1) * a.row16, p->max_blocks);
+  const int64_t gx = std::max<int64_t>(1, std::min<int64_t>((most + 255) / 256, (cv3::sm_count() * 8 + p->groups - 1) / p->groups));
   using Fn = void (*)(const ReorderArgs);
-  const Fn fn = beams <= 4 ? (Fn)reorder_kernel<4> : beams <= 8 ? (Fn)reorder_kernel<8>
-                : beams <= 16 ? (Fn)reorder_kernel<16> : (Fn)reorder_kernel<32>;
-  return cv3::check_launch("paged_reorder", cv3::launch_dep(fn, dim3((unsigned)gx, (unsigned)groups), dim3(256), 0,
+  const Fn fn = p->beams <= 4 ? (Fn)reorder_kernel<4> : p->beams <= 8 ? (Fn)reorder_kernel<8>
+                : p->beams <= 16 ? (Fn)reorder_kernel<16> : (Fn)reorder_kernel<32>;
+  return cv3::check_launch("paged_reorder", cv3::launch_dep(fn, dim3((unsigned)gx, (unsigned)p->groups), dim3(256), 0,
                                                             cv3::as_stream(stream), a));
 }

@@ -7,8 +7,8 @@
 
 namespace cv3p {
 
-inline int type_size(int type) { return type == CV3_TYPE_F32 ? 4 : 2; }
-inline bool type_ok(int type) { return type == CV3_TYPE_F32 || type == CV3_TYPE_F16 || type == CV3_TYPE_BF16; }
+inline int type_size(int64_t type) { return type == CV3_TYPE_F32 ? 4 : 2; }
+inline bool type_ok(int64_t type) { return type == CV3_TYPE_F32 || type == CV3_TYPE_F16 || type == CV3_TYPE_BF16; }
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <typename T>
@@ -61,6 +61,40 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) r.v[i] = from_f32<T>(x[i]);
   *reinterpret_cast<Vec<T, N>*>(p) = r;
+}
+
+// cv3::launch_dep with a cluster of `cluster` CTAs along x
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, unsigned cluster, cudaStream_t st,
+                           Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = cv3::dependent_launch_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// a float of another CTA of the cluster: `p` is the place of the same variable in this CTA
+__device__ __forceinline__ float cluster_load(const float* p, unsigned rank) {
+  uint32_t at;
+  float x;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
 }
 
 }  // namespace cv3p

@@ -12,7 +12,8 @@
 //    them).  A CTA meets at most two pairs that it does not hold whole -- the one that began before
 //    its piece and the one that goes on behind it -- and leaves their partial results (running
 //    maximum, sum, unnormalised output) in two slots; a second launch joins the slots of every pair
-//    that was cut, in CTA order, so the result does not depend on timing.
+//    that was cut, in CTA order, so the result does not depend on timing.  Short caches, whose cost
+//    is latency, take one launch instead: a cluster of CTAs per pair, joined through shared memory.
 // 2. One pass, nothing staged.  A warp takes KI keys of each tile with matrix instructions whose
 //    operands come straight from global memory into registers: the keys' and values' 16-byte pieces
 //    land in the lanes that need them because the order in which head dimensions (for q.k) and the
@@ -126,8 +127,9 @@ __device__ __forceinline__ void visible(const AttnArgs& a, int b, int& lo, int& 
   lo = a.window > 0 ? max(hi - a.window, 0) : 0;
 }
 
-// UNI: page_size is a multiple of 16, so 16 (or 8) keys from a multiple of 16 share a page
-template <typename KT, int D, bool UNI>
+// UNI: page_size is a multiple of 16, so 16 (or 8) keys from a multiple of 16 share a page.
+// CL: clusters of gridDim / pairs CTAs, one per pair, instead of even pieces of the line.
+template <typename KT, int D, bool UNI, bool CL>
 __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnArgs a) {
   constexpr int KI = keys_per_step<KT, D>(), NT = KI / 8, TK = NW * KI;
   constexpr bool WIDE = sizeof(KT) == 4;          // keys and values need a lower part
@@ -146,69 +148,8 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
   const int per = a.kv_heads * a.groups;  // pairs of a request
   const int c = blockIdx.x;
 
-  // requests without keys: zeros, nothing to join
-  for (int b = c; b < a.batch; b += gridDim.x) {
-    int lo, hi;
-    visible(a, b, lo, hi);
-    if (hi > lo) continue;
-    for (int i = tid; i < a.heads * D; i += NW * 32)
-      cv3p::store_any(a.out, a.q_type, b * a.osb + (i / D) * a.osh + i % D, 0.f);
-    if (a.lse)
-      for (int i = tid; i < a.heads; i += NW * 32) a.lse[(int64_t)b * a.heads + i] = -INFINITY;
-    for (int i = tid; i < per; i += NW * 32) a.cut[(int64_t)b * per + i] = make_int2(0, 0);
-  }
-
-  // the whole line and this CTA's piece of it; every warp finds it by itself
-  auto tiles_of = [&](int b) -> int {
-    int lo, hi;
-    visible(a, b, lo, hi);
-    return hi > lo ? (hi - (lo & -KI) + TK - 1) / TK : 0;
-  };
-  int64_t W = 0;
-  for (int b = lane; b < a.batch; b += 32) W += tiles_of(b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) W += __shfl_xor_sync(0xffffffffu, W, o);
-  W *= per;
-  const int64_t C = min((int64_t)gridDim.x, W);  // every CTA that works has a tile
-  if (c >= C) return;
-  int64_t u = W * c / C;
-  const int64_t u_end = W * (c + 1) / C;
-  int b = 0;
-  int64_t before = 0;  // tiles of the requests before b (one pair each)
-  for (int b0 = 0;; b0 += 32) {
-    const int64_t mine = b0 + lane < a.batch ? tiles_of(b0 + lane) : 0;
-    int64_t sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, (before + sum) * per > u);
-    if (past) {
-      const int at = __ffs(past) - 1;
-      b = b0 + at;
-      before += __shfl_sync(0xffffffffu, sum - mine, at);
-      break;
-    }
-    before += __shfl_sync(0xffffffffu, sum, 31);
-  }
-
-  while (u < u_end) {
-    // the pair that u lies in
-    int lo, hi;
-    visible(a, b, lo, hi);
-    const int tiles = hi > lo ? (hi - (lo & -KI) + TK - 1) / TK : 0;
-    if (tiles == 0) { ++b; continue; }
-    const int64_t u_b = before * per;
-    const int pair = (int)((u - u_b) / tiles);
-    if (pair >= per) { before += tiles; ++b; continue; }
-    const int64_t u0 = u_b + (int64_t)pair * tiles;
-    const int t0 = (int)(u - u0), t1 = (int)min((int64_t)tiles, u_end - u0);
-    const int g = pair / a.groups, h0 = g * a.group + (pair - g * a.groups) * HT;
-    const int nh = min(HT, (g + 1) * a.group - h0);
-    const bool whole = t0 == 0 && t1 == tiles;
-    u = u0 + t1;
-
+  // tiles [t0, t1) of a pair: the warps' maxima, sums and unnormalised outputs to shared memory
+  auto attend = [&](int b, int pair, int lo, int hi, int g, int h0, int nh, int t0, int t1) {
     __syncthreads();  // the last pair's shared memory is done with
     for (int i = tid; i < D / 8 * 32; i += NW * 32) {
       const int s = i >> 5, ln = i & 31, row = ln >> 2;
@@ -385,22 +326,145 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
         so[warp][n][x * 8 * VE + (2 * t + 1) * VE + e] = o[x * VE + e][1];
       }
     __syncthreads();
+  };
+  // the warps' shares of output element (h, e) together
+  auto gather = [&](int h, int e, float& M, float& L, float& x) {
+    M = -INFINITY;
+    L = x = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w][h]);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (sl[w][h] == 0.f) continue;  // saw nothing (a NaN score leaves a NaN sum)
+      const float f = exp2_fast(sm[w][h] - M);
+      L = fmaf(sl[w][h], f, L);
+      x = fmaf(so[w][h][e], f, x);
+    }
+  };
+  auto finish = [&](int b, int h, int e, float M, float L, float x) {
+    cv3p::store_any(a.out, a.q_type, b * a.osb + h * a.osh + e, L == 0.f ? 0.f : x / L);
+    if (a.lse && e == 0) a.lse[(int64_t)b * a.heads + h] = L == 0.f ? -INFINITY : (M + log2f(L)) / LOG2E;
+  };
+  auto heads_of = [&](int pair, int& g, int& h0, int& nh) {
+    g = pair / a.groups;
+    h0 = g * a.group + (pair - g * a.groups) * HT;
+    nh = min(HT, (g + 1) * a.group - h0);
+  };
+  auto tiles_of = [&](int b) -> int {
+    int lo, hi;
+    visible(a, b, lo, hi);
+    return hi > lo ? (hi - (lo & -KI) + TK - 1) / TK : 0;
+  };
+
+  if constexpr (CL) {
+    const int S = gridDim.x / (a.batch * per), rank = c % S;
+    const int b = c / S / per, pair = c / S - b * per;
+    int lo, hi, g, h0, nh;
+    visible(a, b, lo, hi);
+    heads_of(pair, g, h0, nh);
+    const int tiles = tiles_of(b);
+    const int t0 = (int)((int64_t)tiles * rank / S), t1 = (int)((int64_t)tiles * (rank + 1) / S);
+    attend(b, pair, lo, hi, g, h0, nh, t0, t1);
+    if (S == 1) {
+      for (int i = tid; i < nh * D; i += NW * 32) {
+        float M, L, x;
+        gather(i / D, i % D, M, L, x);
+        finish(b, h0 + i / D, i % D, M, L, x);
+      }
+      return;
+    }
+    __shared__ float stat[HT][2];
+    for (int i = tid; i < nh * D; i += NW * 32) {
+      float M, L, x;
+      gather(i / D, i % D, M, L, x);
+      so[0][i / D][i % D] = x;  // (read and written by this thread alone)
+      if (i % D == 0) { stat[i / D][0] = M; stat[i / D][1] = L; }
+    }
+    cv3p::cluster_sync();
+    for (int i = tid + rank * NW * 32; i < nh * D; i += S * NW * 32) {
+      const int h = i / D, e = i - h * D;
+      float M = -INFINITY, L = 0.f, x = 0.f, m[8], l[8], o[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        if (r >= S) break;
+        m[r] = cv3p::cluster_load(&stat[h][0], r);
+        l[r] = cv3p::cluster_load(&stat[h][1], r);
+        o[r] = cv3p::cluster_load(&so[0][h][e], r);
+        M = fmaxf(M, m[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        if (r >= S) break;
+        if (l[r] == 0.f) continue;
+        const float f = exp2_fast(m[r] - M);
+        L = fmaf(l[r], f, L);
+        x = fmaf(o[r], f, x);
+      }
+      finish(b, h0 + h, e, M, L, x);
+    }
+    cv3p::cluster_sync();  // no CTA leaves while another reads its shared memory
+    return;
+  }
+
+  // requests without keys: zeros, nothing to join
+  for (int b = c; b < a.batch; b += gridDim.x) {
+    if (tiles_of(b)) continue;
+    for (int i = tid; i < a.heads * D; i += NW * 32) finish(b, i / D, i % D, -INFINITY, 0.f, 0.f);
+    for (int i = tid; i < per; i += NW * 32) a.cut[(int64_t)b * per + i] = make_int2(0, 0);
+  }
+
+  // the whole line and this CTA's piece of it; every warp finds it by itself
+  int64_t W = 0;
+  for (int b = lane; b < a.batch; b += 32) W += tiles_of(b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) W += __shfl_xor_sync(0xffffffffu, W, o);
+  W *= per;
+  const int64_t C = min((int64_t)gridDim.x, W);  // every CTA that works has a tile
+  if (c >= C) return;
+  int64_t u = W * c / C;
+  const int64_t u_end = W * (c + 1) / C;
+  int b = 0;
+  int64_t before = 0;  // tiles of the requests before b (one pair each)
+  for (int b0 = 0;; b0 += 32) {
+    const int64_t mine = b0 + lane < a.batch ? tiles_of(b0 + lane) : 0;
+    int64_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, (before + sum) * per > u);
+    if (past) {
+      const int at = __ffs(past) - 1;
+      b = b0 + at;
+      before += __shfl_sync(0xffffffffu, sum - mine, at);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+
+  while (u < u_end) {
+    // the pair that u lies in
+    int lo, hi, g, h0, nh;
+    visible(a, b, lo, hi);
+    const int tiles = tiles_of(b);
+    if (tiles == 0) { ++b; continue; }
+    const int64_t u_b = before * per;
+    const int pair = (int)((u - u_b) / tiles);
+    if (pair >= per) { before += tiles; ++b; continue; }
+    heads_of(pair, g, h0, nh);
+    const int64_t u0 = u_b + (int64_t)pair * tiles;
+    const int t0 = (int)(u - u0), t1 = (int)min((int64_t)tiles, u_end - u0);
+    const bool whole = t0 == 0 && t1 == tiles;
+    u = u0 + t1;
+    attend(b, pair, lo, hi, g, h0, nh, t0, t1);
     const int slot = t0 > 0 ? 0 : 1;
     for (int i = tid; i < nh * D; i += NW * 32) {
       const int h = i / D, e = i - h * D;
-      float M = -INFINITY, L = 0.f, x = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w][h]);
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        if (sl[w][h] == 0.f) continue;  // saw nothing (a NaN score leaves a NaN sum)
-        const float f = exp2_fast(sm[w][h] - M);
-        L = fmaf(sl[w][h], f, L);
-        x = fmaf(so[w][h][e], f, x);
-      }
+      float M, L, x;
+      gather(h, e, M, L, x);
       if (whole) {
-        cv3p::store_any(a.out, a.q_type, b * a.osb + (h0 + h) * a.osh + e, L == 0.f ? 0.f : x / L);
-        if (a.lse && e == 0) a.lse[(int64_t)b * a.heads + h0 + h] = L == 0.f ? -INFINITY : (M + log2f(L)) / LOG2E;
+        finish(b, h0 + h, e, M, L, x);
       } else {
         const int64_t at = ((int64_t)c * 2 + slot) * HT + h;
         a.part[at * D + e] = x;
@@ -484,13 +548,19 @@ __global__ void __launch_bounds__(NW * 32) paged_join_kernel(const AttnArgs a) {
 
 using Fn = void (*)(const AttnArgs);
 
+template <typename KT, int D>
+Fn pick(bool uni, bool cl) {
+  if (cl) return uni ? paged_attention_kernel<KT, D, true, true> : paged_attention_kernel<KT, D, false, true>;
+  return uni ? paged_attention_kernel<KT, D, true, false> : paged_attention_kernel<KT, D, false, false>;
+}
+
 template <typename KT>
-Fn pick(int64_t d, bool uni) {
+Fn pick(int64_t d, bool uni, bool cl) {
   switch (d) {
-    case 32: return uni ? paged_attention_kernel<KT, 32, true> : paged_attention_kernel<KT, 32, false>;
-    case 64: return uni ? paged_attention_kernel<KT, 64, true> : paged_attention_kernel<KT, 64, false>;
-    case 96: return uni ? paged_attention_kernel<KT, 96, true> : paged_attention_kernel<KT, 96, false>;
-    default: return uni ? paged_attention_kernel<KT, 128, true> : paged_attention_kernel<KT, 128, false>;
+    case 32: return pick<KT, 32>(uni, cl);
+    case 64: return pick<KT, 64>(uni, cl);
+    case 96: return pick<KT, 96>(uni, cl);
+    default: return pick<KT, 128>(uni, cl);
   }
 }
 
@@ -503,71 +573,95 @@ Fn pick_join(int64_t d, bool wide) {
   }
 }
 
-int64_t pairs_of(int64_t batch, int64_t heads, int64_t kv_heads) {
-  return batch * kv_heads * ((heads / kv_heads + HT - 1) / HT);
-}
+// Keys of a CTA's tile (keys_per_step of the type and head dimension).
+int64_t tile_of(int64_t d, int64_t size) { return NW * (d * size <= 128 ? 32 : d * size <= 256 ? 16 : 8); }
 
-// two CTAs on every SM; fewer where the table holds fewer tiles (of the smallest kind: 8 keys a warp)
-int64_t grid_of(int64_t pairs, int64_t max_len) {
-  return std::max<int64_t>(1, std::min<int64_t>(2 * cv3::sm_count(), pairs * ((max_len + NW * 8 - 1) / (NW * 8) + 1)));
-}
+struct Plan {
+  int64_t pairs, grid, cluster, floats;  // cluster 0: even pieces and a join
+};
 
-int64_t floats_of(int64_t pairs, int64_t grid, int64_t d) { return 2 * pairs + grid * 2 * HT * (d + 2); }
+// Clusters where every CTA then has at most CLUSTER_STEPS tiles however long the requests (the host
+// knows the table's width only): as many CTAs per pair as tiles, up to 8 and one wave of two CTAs per
+// SM.  Else one wave that cuts the line into even pieces.
+constexpr int64_t CLUSTER_STEPS = 8;
+
+Plan plan_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t d, int64_t size, int64_t max_len) {
+  Plan p = {};
+  p.pairs = batch * kv_heads * ((heads / kv_heads + HT - 1) / HT);
+  const int64_t wave = 2 * cv3::sm_count(), tk = tile_of(d, size);
+  const int64_t tiles = max_len / tk + 2;  // (a window's first tile may begin before its first key)
+  int64_t s = 1;
+  while (s < 8 && s < tiles - 1 && p.pairs * s * 2 <= wave) s *= 2;
+  if ((tiles + s - 1) / s * ((p.pairs * s + wave - 1) / wave) <= CLUSTER_STEPS) {
+    p.cluster = s;
+    p.grid = p.pairs * s;
+  } else {
+    p.grid = std::min(wave, p.pairs * tiles);
+    p.floats = 2 * p.pairs + p.grid * 2 * HT * (d + 2);
+  }
+  return p;
+}
 
 }  // namespace
 
 extern "C" int64_t cv3_paged_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                                                 int64_t max_len) {
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
-  const int64_t pairs = pairs_of(batch, heads, kv_heads);
-  return floats_of(pairs, grid_of(pairs, max_len), head_dim);
+                                                 int kv_type, int64_t max_len) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_len < 0) return 0;
+  return plan_of(batch, heads, kv_heads, head_dim, cv3p::type_size(kv_type), max_len).floats;
 }
 
-extern "C" int cv3_paged_attention(const void* q, int q_type, int64_t qsb, int64_t qsh, const void* k_pages,
-                                   const void* v_pages, int kv_type, int64_t ksp, int64_t ksh, int64_t kst, int64_t vsp,
-                                   int64_t vsh, int64_t vst, int64_t num_pages, int64_t page_size,
-                                   const int* block_tables, int64_t table_ld, int64_t max_blocks, const int* lens,
-                                   int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window,
-                                   float scale, void* out, int64_t osb, int64_t osh, float* lse, int* bad,
-                                   float* workspace, int64_t workspace_floats, void* stream) {
-  CV3_REQUIRE(batch >= 0 && heads > 0 && kv_heads > 0 && num_pages >= 0 && page_size > 0 && max_blocks >= 0 &&
-                  table_ld >= max_blocks && window >= 0,
+extern "C" int cv3_paged_attention(const cv3_paged_attention_params* p, void* stream) {
+  CV3_REQUIRE(p && p->size == (int64_t)sizeof(*p), CV3_ERR_VALUE, "paged_attention: bad parameter block");
+  CV3_REQUIRE(p->batch >= 0 && p->heads > 0 && p->kv_heads > 0 && p->num_pages >= 0 && p->page_size > 0 &&
+                  p->max_blocks >= 0 && p->table_ld >= p->max_blocks && p->window >= 0,
               CV3_ERR_VALUE, "paged_attention: bad shape");
-  CV3_REQUIRE(heads % kv_heads == 0, CV3_ERR_VALUE, "%lld query heads is not a multiple of %lld kv heads",
-              (long long)heads, (long long)kv_heads);
-  CV3_REQUIRE(head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128, CV3_ERR_UNSUPPORTED,
-              "paged_attention: head_dim %lld (built for 32, 64, 96 and 128)", (long long)head_dim);
-  CV3_REQUIRE(cv3p::type_ok(q_type) && cv3p::type_ok(kv_type), CV3_ERR_VALUE, "paged_attention: unknown element type");
-  const int ce = 16 / cv3p::type_size(kv_type);
-  CV3_REQUIRE(cv3p::aligned16(k_pages) && cv3p::aligned16(v_pages) && (ksp | ksh | kst | vsp | vsh | vst) % ce == 0,
+  CV3_REQUIRE(p->heads % p->kv_heads == 0, CV3_ERR_VALUE, "%lld query heads is not a multiple of %lld kv heads",
+              (long long)p->heads, (long long)p->kv_heads);
+  const int64_t d = p->head_dim;
+  CV3_REQUIRE(d == 32 || d == 64 || d == 96 || d == 128, CV3_ERR_UNSUPPORTED,
+              "paged_attention: head_dim %lld (built for 32, 64, 96 and 128)", (long long)d);
+  CV3_REQUIRE(cv3p::type_ok(p->q_type) && cv3p::type_ok(p->kv_type), CV3_ERR_VALUE,
+              "paged_attention: unknown element type");
+  const int es = cv3p::type_size(p->kv_type), ce = 16 / es;
+  CV3_REQUIRE(cv3p::aligned16(p->k_pages) && cv3p::aligned16(p->v_pages) &&
+                  (p->ksp | p->ksh | p->kst | p->vsp | p->vsh | p->vst) % ce == 0,
               CV3_ERR_VALUE, "paged_attention: cache rows must start on 16-byte boundaries");
   // (a tile behind the last key must not pass 2^31 either)
-  CV3_REQUIRE(page_size <= INT32_MAX && max_blocks * page_size <= INT32_MAX - 4096 && num_pages <= INT32_MAX && batch <= INT32_MAX, CV3_ERR_VALUE,
-              "paged_attention: positions and pages are 32-bit numbers");
-  if (batch == 0) return CV3_OK;
-  const int64_t pairs = pairs_of(batch, heads, kv_heads), max_len = max_blocks * page_size;
-  const int64_t grid = grid_of(pairs, max_len);
-  CV3_REQUIRE(pairs <= INT32_MAX, CV3_ERR_VALUE, "paged_attention: too many requests and heads");
-  CV3_REQUIRE(workspace && workspace_floats >= floats_of(pairs, grid, head_dim) && ((uintptr_t)workspace & 7) == 0,
+  CV3_REQUIRE(p->page_size <= INT32_MAX && p->max_blocks <= INT32_MAX &&
+                  p->max_blocks * p->page_size <= INT32_MAX - 4096 && p->num_pages <= INT32_MAX &&
+                  p->batch <= 1 << 24 && p->heads <= 1 << 16,
+              CV3_ERR_VALUE, "paged_attention: positions, pages and pairs are 32-bit numbers");
+  if (p->batch == 0) return CV3_OK;
+  const int64_t max_len = p->max_blocks * p->page_size;
+  const Plan plan = plan_of(p->batch, p->heads, p->kv_heads, d, es, max_len);
+  CV3_REQUIRE(plan.grid <= INT32_MAX, CV3_ERR_VALUE, "paged_attention: too many requests and heads");
+  CV3_REQUIRE(plan.floats == 0 || (p->workspace && p->workspace_floats >= plan.floats && ((uintptr_t)p->workspace & 7) == 0),
               CV3_ERR_VALUE, "paged_attention: the workspace must hold cv3_paged_attention_workspace() floats");
-  // n / ps by a product: with shift s = 32 + ceil(log2 ps) the error of mul = ceil(2^s / ps) < 2^33 is too small to
-  // reach a quotient for n < 2^31; mul itself must stay below 2^32, so one step less for n < 2^31
+  // n / page_size by a product: with 2^(sh-1) < page_size <= 2^sh and mul = ceil(2^(31+sh) / page_size), the excess
+  // mul * page_size - 2^(31+sh) is below 2^sh, so n < 2^31 times it stays below 2^(31+sh): the quotient is exact
   int sh = 0;
-  while ((int64_t)1 << sh < page_size) ++sh;
-  const uint32_t mul = (uint32_t)((((uint64_t)1 << (31 + sh)) + page_size - 1) / page_size);
-  float* stat = workspace + 2 * pairs;
-  const AttnArgs a = {q, q_type, qsb, qsh, k_pages, v_pages, ksp, ksh, kst, vsp, vsh, vst, num_pages, (int)page_size, mul,
-                      (uint32_t)(31 + sh), block_tables, table_ld, (int)max_len, lens, (int)batch, (int)heads,
-                      (int)kv_heads, (int)(heads / kv_heads), (int)((heads / kv_heads + HT - 1) / HT),
-                      (int)std::min<int64_t>(window, INT32_MAX), scale, out, osb, osh, lse, bad,
-                      stat + grid * 2 * HT * 2, stat, reinterpret_cast<int2*>(workspace)};
-  const bool uni = page_size % 16 == 0;
-  const Fn fn = kv_type == CV3_TYPE_F32   ? pick<float>(head_dim, uni)
-                : kv_type == CV3_TYPE_F16 ? pick<__half>(head_dim, uni) : pick<__nv_bfloat16>(head_dim, uni);
+  while ((int64_t)1 << sh < p->page_size) ++sh;
+  const uint32_t mul = (uint32_t)((((uint64_t)1 << (31 + sh)) + p->page_size - 1) / p->page_size);
+  float* stat = p->workspace + 2 * plan.pairs;
+  const int group = (int)(p->heads / p->kv_heads);
+  const AttnArgs a = {p->q, (int)p->q_type, p->qsb, p->qsh, p->k_pages, p->v_pages, p->ksp, p->ksh, p->kst, p->vsp,
+                      p->vsh, p->vst, p->num_pages, (int)p->page_size, mul, (uint32_t)(31 + sh), p->block_tables,
+                      p->table_ld, (int)max_len, p->lens, (int)p->batch, (int)p->heads, (int)p->kv_heads, group,
+                      (group + HT - 1) / HT, (int)std::min<int64_t>(p->window, INT32_MAX), (float)p->scale, p->out,
+                      p->osb, p->osh, p->lse, p->bad, stat + plan.grid * 2 * HT * 2, stat,
+                      reinterpret_cast<int2*>(p->workspace)};
+  const bool uni = p->page_size % 16 == 0, cl = plan.cluster > 0;
+  const Fn fn = p->kv_type == CV3_TYPE_F32   ? pick<float>(d, uni, cl)
+                : p->kv_type == CV3_TYPE_F16 ? pick<__half>(d, uni, cl) : pick<__nv_bfloat16>(d, uni, cl);
   cudaStream_t st = cv3::as_stream(stream);
-  int rc = cv3::check_launch("paged_attention", cv3::launch_dep(fn, dim3((unsigned)grid), dim3(NW * 32), 0, st, a));
-  if (rc || grid == 1) return rc;
-  const bool wide = pairs <= 64;
-  return cv3::check_launch("paged_join", cv3::launch_dep(pick_join(head_dim, wide), dim3((unsigned)pairs, wide ? HT : 1),
-                                                         dim3(NW * 32), 0, st, a));
+  const dim3 grid((unsigned)plan.grid), block(NW * 32);
+  if (cl)
+    return cv3::check_launch("paged_attention", plan.cluster == 1
+                                                    ? cv3::launch_dep(fn, grid, block, 0, st, a)
+                                                    : cv3p::launch_cluster(fn, grid, block, 0, (unsigned)plan.cluster, st, a));
+  int rc = cv3::check_launch("paged_attention", cv3::launch_dep(fn, grid, block, 0, st, a));
+  if (rc) return rc;
+  const bool wide = plan.pairs <= 64;
+  return cv3::check_launch("paged_join", cv3::launch_dep(pick_join(d, wide), dim3((unsigned)plan.pairs, wide ? HT : 1),
+                                                         block, 0, st, a));
 }

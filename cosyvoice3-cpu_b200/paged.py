@@ -22,6 +22,7 @@ they read on the device (lengths, tables, flags) may change between replays.
 from __future__ import annotations
 
 import math
+import struct
 from typing import NamedTuple, Optional, Tuple
 
 import numpy as np
@@ -32,6 +33,11 @@ from ._lib import check, load
 torch = D.torch
 
 MAX_BEAMS = 32   # CV3_MAX_BEAMS
+
+# The C entries' parameter blocks (include/cv3cuda.h): 64-bit fields, packed here in one call -- a
+# third of what 20 to 35 ctypes arguments cost.
+_EXTEND, _APPEND, _ATTENTION, _BEAM, _REORDER = (struct.Struct("=" + f) for f in
+                                                 ("20q", "26q", "32qd", "20qd", "24q"))
 
 if torch is not None:
     _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -56,6 +62,11 @@ class BeamStep(NamedTuple):
     scores: object       # float32
     counts: object       # int32
     done: object         # int32
+
+
+def _new(like, shape, dtype):
+    """An uninitialised array next to ``like``."""
+    return like.new_empty(shape, dtype=dtype) if torch is not None else D.empty(shape, dtype)
 
 
 def _device(name: str, *arrays) -> int:
@@ -146,28 +157,29 @@ def paged_extend(lens, new_lens, block_tables, free_pages, free_count, page_size
     if page_size <= 0 or T < 0:
         raise ValueError(f"{name}: page_size {page_size}, max_tokens {max_tokens}")
     pl, pn = _ints(name, "lens", lens, n), _ints(name, "new_lens", new_lens, n)
-    pr = None if release is None else _ints(name, "release", release, n)
+    pr = 0 if release is None else _ints(name, "release", release, n)
     tp, ld, cols = _table(name, block_tables, n)
     cap = free_pages.numel()
     pf, pc = _ints(name, "free_pages", free_pages, cap), _ints(name, "free_count", free_count, 1)
     if out is None:
-        slots = D.empty((T,), D.I64)
+        sizes = (T, T, n + 1, n, 1, n + 1)
         if torch is not None:
-            seq, pos, offsets, lens_out, count, scratch = torch.empty(
-                2 * T + 3 * n + 3, dtype=torch.int32, device=lens.device).split((T, T, n + 1, n, 1, n + 1))
+            parts = torch.split_with_sizes(lens.new_empty((2 * T + 3 * n + 3,)), sizes)
         else:
-            seq, pos, offsets, lens_out, count, scratch = (D.empty((m,), D.I32) for m in (T, T, n + 1, n, 1, n + 1))
-        out = PagedStep(slots, seq, pos, offsets, lens_out, count)
+            parts = [D.empty((m,), D.I32) for m in sizes]
+        out = PagedStep(_new(lens, (T,), D.I64), *parts[:5])
+        scratch = parts[5]
     else:
-        _device(name, *out)
+        _device(name, lens, *out)
         _ints(name, "out.slots", out.slots, T, D.I64)
         for what, x, m in (("seq", out.seq, T), ("pos", out.pos, T), ("offsets", out.offsets, n + 1),
                            ("lens", out.lens, n), ("free_count", out.free_count, 1)):
             _ints(name, "out." + what, x, m)
-        scratch = D.empty((n + 1,), D.I32)
-    rc = load().cv3_paged_extend(pl, pn, pr, n, tp, ld, cols, page_size, pf, cap, pc, T, out.slots.data_ptr(),
-                                 out.seq.data_ptr(), out.pos.data_ptr(), out.offsets.data_ptr(), out.lens.data_ptr(),
-                                 out.free_count.data_ptr(), scratch.data_ptr(), D.raw_stream(d))
+        scratch = _new(lens, (n + 1,), D.I32)
+    rc = load().cv3_paged_extend(
+        _EXTEND.pack(_EXTEND.size, pl, pn, pr, n, tp, ld, cols, page_size, pf, cap, pc, T, out.slots.data_ptr(),
+                     out.seq.data_ptr(), out.pos.data_ptr(), out.offsets.data_ptr(), out.lens.data_ptr(),
+                     out.free_count.data_ptr(), scratch.data_ptr()), D.raw_stream(d))
     if rc:
         check(rc, name)
     return out
@@ -194,11 +206,10 @@ def paged_append(qkv, slots, pos, k_pages, v_pages, heads: int, cos=None, sin=No
     if one != 1:
         raise ValueError(f"{name}: qkv rows must be contiguous")
     pslots = _ints(name, "slots", slots, rows, D.I64)
-    pc = psn = None
-    positions = 0
+    pc = psn = positions = 0
     if (cos is None) != (sin is None) or (cos is not None and pos is None):
         raise ValueError(f"{name}: cos, sin and pos go together")
-    ppos = None if pos is None else _ints(name, "pos", pos, rows)
+    ppos = 0 if pos is None else _ints(name, "pos", pos, rows)
     if cos is not None:
         positions = cos.shape[0]
         for x in (cos, sin):
@@ -206,14 +217,14 @@ def paged_append(qkv, slots, pos, k_pages, v_pages, heads: int, cos=None, sin=No
                 raise ValueError(f"{name}: cos and sin must be contiguous float32 (positions, {dim})")
         pc, psn = cos.data_ptr(), sin.data_ptr()
     if out is None:
-        out = D.empty((rows, heads, dim), qkv.dtype)
+        out = _new(qkv, (rows, heads, dim), qkv.dtype)
     else:
         _like(name, out, (rows, heads, dim), qkv.dtype)
-    pbad = None if bad is None else _ints(name, "bad", bad, 1)
-    rc = load().cv3_paged_append(qkv.data_ptr(), t, rows, ldq if rows > 1 else qkv.shape[1], pc, psn, positions, pslots,
-                                 ppos, heads, kv, dim, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), kt, ks[0],
-                                 ks[1], ks[2], vs[0], vs[1], vs[2], pages, ps,
-                                 pbad, D.raw_stream(d))
+    pbad = 0 if bad is None else _ints(name, "bad", bad, 1)
+    rc = load().cv3_paged_append(
+        _APPEND.pack(_APPEND.size, qkv.data_ptr(), t, rows, ldq if rows > 1 else qkv.shape[1], pc, psn, positions, pslots,
+                     ppos, heads, kv, dim, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), kt, ks[0], ks[1],
+                     ks[2], vs[0], vs[1], vs[2], pages, ps, pbad), D.raw_stream(d))
     if rc:
         check(rc, name)
     return out
@@ -250,18 +261,20 @@ def paged_attention(q, k_pages, v_pages, block_tables, lens, scale: Optional[flo
     tp, ld, cols = _table(name, block_tables, B)
     plens = _ints(name, "lens", lens, B)
     if out is None:
-        out = D.empty((B, H, dim), q.dtype)
+        out = _new(q, (B, H, dim), q.dtype)
     else:
         _like(name, out, (B, H, dim), q.dtype)
-    pbad = None if bad is None else _ints(name, "bad", bad, 1)
-    lse = D.empty((B, H)) if return_lse else None
+    pbad = 0 if bad is None else _ints(name, "bad", bad, 1)
+    lse = _new(q, (B, H), D.F32) if return_lse else None
     lib = load()
-    words = lib.cv3_paged_attention_workspace(B, H, kv, dim, cols * ps)
-    ws = D.empty((words,)) if words else None
-    rc = lib.cv3_paged_attention(q.data_ptr(), qt, qsb, qsh, k_pages.data_ptr(), v_pages.data_ptr(), kt, ks[0], ks[1],
-                                 ks[2], vs[0], vs[1], vs[2], pages, ps, tp, ld, cols, plens, B, H, kv, dim, window,
-                                 1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), H * dim, dim,
-                                 None if lse is None else lse.data_ptr(), pbad, None if ws is None else ws.data_ptr(), words, D.raw_stream(d))
+    words = lib.cv3_paged_attention_workspace(B, H, kv, dim, kt, cols * ps)
+    ws = _new(q, (words,), D.F32) if words else None
+    rc = lib.cv3_paged_attention(
+        _ATTENTION.pack(_ATTENTION.size, q.data_ptr(), qt, qsb, qsh, k_pages.data_ptr(), v_pages.data_ptr(), kt, ks[0],
+                        ks[1], ks[2], vs[0], vs[1], vs[2], pages, ps, tp, ld, cols, plens, B, H, kv, dim, window,
+                        out.data_ptr(), H * dim, dim, lse.data_ptr() if return_lse else 0, pbad,
+                        ws.data_ptr() if words else 0, words, 1.0 / math.sqrt(dim) if scale is None else scale),
+        D.raw_stream(d))
     if rc:
         check(rc, name)
     return (out, lse) if return_lse else out
@@ -290,29 +303,28 @@ def beam_select(logits, scores, counts, done, stop: Optional[Tuple[int, int]] = 
     if (V > 1 and sv != 1) or (G > 1 and sg != K * sk):
         raise ValueError(f"{name}: rows of logits must be contiguous and evenly spaced")
     n = G * K
-    if scores.dtype != D.F32 or scores.numel() != n or not scores.is_contiguous():
-        raise ValueError(f"{name}: scores must be {n} contiguous float32 values")
-    pc, pd = _ints(name, "counts", counts, n), _ints(name, "done", done, n)
-    pm = None if min_len is None else _ints(name, "min_len", min_len, G)
+    for what, x, dt in (("scores", scores, D.F32), ("counts", counts, D.I32), ("done", done, D.I32)):
+        if x.dtype != dt or x.shape != (G, K) or not x.is_contiguous():
+            raise ValueError(f"{name}: {what} must be contiguous ({G}, {K}) {dt}, got {tuple(x.shape)} {x.dtype}")
+    pc, pd = counts.data_ptr(), done.data_ptr()
+    pm = 0 if min_len is None else _ints(name, "min_len", min_len, G)
     lo, hi = (0, 0) if stop is None else stop
     if not 0 <= lo <= hi <= V:
         raise ValueError(f"{name}: stop tokens {lo}..{hi} outside the vocabulary of {V}")
     if out is None:
-        if torch is not None:
-            parents, cnt, fin = torch.empty((3, G, K), dtype=torch.int32, device=logits.device).unbind(0)
-        else:
-            parents, cnt, fin = (D.empty((G, K), D.I32) for _ in range(3))
-        out = BeamStep(D.empty((G, K), D.I64), parents, D.empty((G, K)), cnt, fin)
+        out = BeamStep(_new(counts, (G, K), D.I64), D.empty_like(counts), D.empty_like(scores), D.empty_like(counts),
+                       D.empty_like(done))
     else:
         _device(name, logits, *out)
         for x, dt in zip(out, (D.I64, D.I32, D.F32, D.I32, D.I32)):
             _like(name, x, (G, K), dt)
     lib = load()
     size = lib.cv3_beam_workspace(G, K, V)
-    ws = D.empty((max(size, 8) // 8,), D.I64)
-    rc = lib.cv3_beam_select(logits.data_ptr(), t, sk if n > 1 else V, G, K, V, scores.data_ptr(), pc, pd, lo, hi, pm,
-                             length_penalty, out.tokens.data_ptr(), out.parents.data_ptr(), out.scores.data_ptr(),
-                             out.counts.data_ptr(), out.done.data_ptr(), ws.data_ptr(), size, D.raw_stream(d))
+    ws = _new(counts, (size >> 3,), D.I64) if size else None
+    rc = lib.cv3_beam_select(
+        _BEAM.pack(_BEAM.size, logits.data_ptr(), t, sk if n > 1 else V, G, K, V, scores.data_ptr(), pc, pd, lo, hi, pm,
+                   out.tokens.data_ptr(), out.parents.data_ptr(), out.scores.data_ptr(), out.counts.data_ptr(),
+                   out.done.data_ptr(), ws.data_ptr() if size else 0, size, length_penalty), D.raw_stream(d))
     if rc:
         check(rc, name)
     return out
@@ -342,8 +354,8 @@ def paged_reorder(k_pages, v_pages, block_tables, parents, lens) -> None:
     pp = _ints(name, "parents", parents, G * K)
     tp, ld, cols = _table(name, block_tables, G * K)
     plens = _ints(name, "lens", lens, G * K)
-    rc = load().cv3_paged_reorder(k_pages.data_ptr(), v_pages.data_ptr(), kt, layers, pages, kv, ps, dim, ks[0], ks[1],
-                                  ks[2], ks[3], vs[0], vs[1], vs[2], vs[3], tp, ld, cols, pp,
-                                  plens, G, K, D.raw_stream(d))
+    rc = load().cv3_paged_reorder(
+        _REORDER.pack(_REORDER.size, k_pages.data_ptr(), v_pages.data_ptr(), kt, layers, pages, kv, ps, dim, *ks[:4],
+                      *vs[:4], tp, ld, cols, pp, plens, G, K), D.raw_stream(d))
     if rc:
         check(rc, name)

@@ -393,6 +393,9 @@ int cv3_head_select(const float* logits, int64_t batch, int64_t vocab, int64_t s
 #define CV3_TYPE_F16 1
 #define CV3_TYPE_BF16 2
 
+/* The entries take one block of 64-bit fields (pointers, int64_t, double; `size` is
+ * sizeof the block and is checked), which a caller without structs can fill as an array. */
+
 /* Pages and slots for the new tokens of `batch` requests.  Request b holds lens[b]
  * tokens (with release non-NULL and release[b] != 0 it first gives its pages back and
  * holds none) and gets new_lens[b] more.  Free pages are a stack: free_pages[0 ..
@@ -405,10 +408,27 @@ int cv3_head_select(const float* logits, int64_t batch, int64_t vocab, int64_t s
  * pos 0); offsets [batch + 1], request b's rows being offsets[b] .. offsets[b+1];
  * lens_out [batch]; *free_count_out.  lens_out may be lens, free_count_out may be
  * free_count.  scratch: batch + 1 ints. */
-int cv3_paged_extend(const int* lens, const int* new_lens, const int* release, int64_t batch, int* block_tables,
-                     int64_t table_ld, int64_t max_blocks, int64_t page_size, int* free_pages, int64_t free_cap,
-                     const int* free_count, int64_t max_tokens, int64_t* slots, int* seq, int* pos, int* offsets,
-                     int* lens_out, int* free_count_out, int* scratch, void* stream);
+typedef struct cv3_paged_extend_params {
+  int64_t size;
+  const int* lens;
+  const int* new_lens;
+  const int* release;
+  int64_t batch;
+  int* block_tables;
+  int64_t table_ld, max_blocks, page_size;
+  int* free_pages;
+  int64_t free_cap;
+  const int* free_count;
+  int64_t max_tokens;
+  int64_t* slots;
+  int* seq;
+  int* pos;
+  int* offsets;
+  int* lens_out;
+  int* free_count_out;
+  int* scratch;
+} cv3_paged_extend_params;
+int cv3_paged_extend(const cv3_paged_extend_params* params, void* stream);
 
 /* cv3_rope_qkv_append into pages: rows of fused qkv [rows][ldq] (q heads, k heads, v
  * heads; element type `type`) -> q_out [rows][heads][head_dim] of that type, rotated;
@@ -417,11 +437,23 @@ int cv3_paged_extend(const int* lens, const int* new_lens, const int* release, i
  * [positions][head_dim], stores nothing and adds 1 to *bad (may be NULL).  NULL
  * tables: no rotation (pos may be NULL).  Slots of one call must differ.  head_dim a
  * multiple of 16 up to 256; rows on 16-byte boundaries. */
-int cv3_paged_append(const void* qkv, int type, int64_t rows, int64_t ldq, const float* cos_table,
-                     const float* sin_table, int64_t positions, const int64_t* slots, const int* pos, int64_t heads,
-                     int64_t kv_heads, int64_t head_dim, void* q_out, void* k_pages, void* v_pages, int kv_type,
-                     int64_t ksp, int64_t ksh, int64_t kst, int64_t vsp, int64_t vsh, int64_t vst, int64_t num_pages,
-                     int64_t page_size, int* bad, void* stream);
+typedef struct cv3_paged_append_params {
+  int64_t size;
+  const void* qkv;
+  int64_t type, rows, ldq;
+  const float* cos_table;
+  const float* sin_table;
+  int64_t positions;
+  const int64_t* slots;
+  const int* pos;
+  int64_t heads, kv_heads, head_dim;
+  void* q_out;
+  void* k_pages;
+  void* v_pages;
+  int64_t kv_type, ksp, ksh, kst, vsp, vsh, vst, num_pages, page_size;
+  int* bad;
+} cv3_paged_append_params;
+int cv3_paged_append(const cv3_paged_append_params* params, void* stream);
 
 /* One new token's attention per request over its pages: out[b][h] = softmax(scale *
  * q[b][h] . K) V over request b's cached tokens [max(0, lens[b] - window), lens[b])
@@ -432,14 +464,28 @@ int cv3_paged_append(const void* qkv, int type, int64_t rows, int64_t ldq, const
  * table entry adds 1 to *bad (may be NULL).  lse (may be NULL) [batch][heads]: the
  * logarithm of the softmax's sum (-inf without tokens).  head_dim 32, 64, 96 or 128.
  * workspace: cv3_paged_attention_workspace() floats (its max_len: max_blocks *
- * page_size), nothing kept in it between calls. */
-int cv3_paged_attention(const void* q, int q_type, int64_t qsb, int64_t qsh, const void* k_pages, const void* v_pages,
-                        int kv_type, int64_t ksp, int64_t ksh, int64_t kst, int64_t vsp, int64_t vsh, int64_t vst,
-                        int64_t num_pages, int64_t page_size, const int* block_tables, int64_t table_ld,
-                        int64_t max_blocks, const int* lens, int64_t batch, int64_t heads, int64_t kv_heads,
-                        int64_t head_dim, int64_t window, float scale, void* out, int64_t osb, int64_t osh, float* lse,
-                        int* bad, float* workspace, int64_t workspace_floats, void* stream);
-int64_t cv3_paged_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+ * page_size; 0: none is needed), nothing kept in it between calls. */
+typedef struct cv3_paged_attention_params {
+  int64_t size;
+  const void* q;
+  int64_t q_type, qsb, qsh;
+  const void* k_pages;
+  const void* v_pages;
+  int64_t kv_type, ksp, ksh, kst, vsp, vsh, vst, num_pages, page_size;
+  const int* block_tables;
+  int64_t table_ld, max_blocks;
+  const int* lens;
+  int64_t batch, heads, kv_heads, head_dim, window;
+  void* out;
+  int64_t osb, osh;
+  float* lse;
+  int* bad;
+  float* workspace;
+  int64_t workspace_floats;
+  double scale;
+} cv3_paged_attention_params;
+int cv3_paged_attention(const cv3_paged_attention_params* params, void* stream);
+int64_t cv3_paged_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int kv_type,
                                       int64_t max_len);
 
 /* Beam search's choice.  Group g's `beams` hypotheses have scores (sums of
@@ -455,10 +501,25 @@ int64_t cv3_paged_attention_workspace(int64_t batch, int64_t heads, int64_t kv_h
  * may be the input buffers.  Keys are computed in 64 bits.
  * workspace: cv3_beam_workspace() bytes, 8-byte aligned, nothing kept in it. */
 #define CV3_MAX_BEAMS 32
-int cv3_beam_select(const void* logits, int type, int64_t ld, int64_t groups, int64_t beams, int64_t vocab,
-                    const float* scores, const int* counts, const int* done, int64_t stop_lo, int64_t stop_hi,
-                    const int* min_len, double length_penalty, int64_t* tokens, int* parents, float* scores_out,
-                    int* counts_out, int* done_out, void* workspace, int64_t workspace_bytes, void* stream);
+typedef struct cv3_beam_params {
+  int64_t size;
+  const void* logits;
+  int64_t type, ld, groups, beams, vocab;
+  const float* scores;
+  const int* counts;
+  const int* done;
+  int64_t stop_lo, stop_hi;
+  const int* min_len;
+  int64_t* tokens;
+  int* parents;
+  float* scores_out;
+  int* counts_out;
+  int* done_out;
+  void* workspace;
+  int64_t workspace_bytes;
+  double length_penalty;
+} cv3_beam_params;
+int cv3_beam_select(const cv3_beam_params* params, void* stream);
 int64_t cv3_beam_workspace(int64_t groups, int64_t beams, int64_t vocab);
 
 /* The cache follows the beams: rows g*beams .. of block_tables are a group's beams, all
@@ -468,11 +529,18 @@ int64_t cv3_beam_workspace(int64_t groups, int64_t beams, int64_t vocab);
  * beam k's own row names there, which no other beam may name.  A parent outside
  * [0, beams) counts as k; a beam whose own or whose parent's last page lies outside the
  * pool keeps that page as it is.  Pools: layers s_l apart. */
-int cv3_paged_reorder(void* k_pages, void* v_pages, int kv_type, int64_t layers, int64_t num_pages, int64_t kv_heads,
-                      int64_t page_size, int64_t head_dim, int64_t ksl, int64_t ksp, int64_t ksh, int64_t kst,
-                      int64_t vsl, int64_t vsp, int64_t vsh, int64_t vst, int* block_tables, int64_t table_ld,
-                      int64_t max_blocks, const int* parents, const int* lens, int64_t groups, int64_t beams,
-                      void* stream);
+typedef struct cv3_paged_reorder_params {
+  int64_t size;
+  void* k_pages;
+  void* v_pages;
+  int64_t kv_type, layers, num_pages, kv_heads, page_size, head_dim, ksl, ksp, ksh, kst, vsl, vsp, vsh, vst;
+  int* block_tables;
+  int64_t table_ld, max_blocks;
+  const int* parents;
+  const int* lens;
+  int64_t groups, beams;
+} cv3_paged_reorder_params;
+int cv3_paged_reorder(const cv3_paged_reorder_params* params, void* stream);
 
 /* ------------------------------------------------------------------ */
 /* DiT flow estimator and Euler/CFG solve (cv3cpu/models/dit.py, flow.py) */

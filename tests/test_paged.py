@@ -2,12 +2,13 @@
 strides and alignment are rejected before anything reaches the device (the host checks run here on
 CPU tensors with the device check replaced, the C ABI on made-up addresses that it must not touch)."""
 
-import ctypes
+import os
+import re
 
 import numpy as np
 import pytest
 
-from conftest import pkg
+from conftest import REPO, pkg
 
 import oracle.paged as ref
 
@@ -139,51 +140,78 @@ def test_beam_and_reorder_refusals(ops):
             ops.paged_reorder(**{**fine, **change})
 
 
-def test_c_entries_refuse_before_any_device_work():
-    L = pkg("_lib")
-    lib = L.load()
-    P = ctypes.c_void_p
-    V, U = L.CV3_ERR_VALUE, L.CV3_ERR_UNSUPPORTED
+BLOCKS = {"cv3_paged_extend": "_EXTEND", "cv3_paged_append": "_APPEND", "cv3_paged_attention": "_ATTENTION",
+          "cv3_beam": "_BEAM", "cv3_paged_reorder": "_REORDER"}
 
-    def attention(dim=64, kv=2, heads=4, ps=16, strides=(2048, 1024, 64), k=1 << 20, kt=0, cols=3, ld=3, window=0):
-        return lib.cv3_paged_attention(P(1 << 20), 0, heads * dim, dim, P(k), P(1 << 20), kt, *strides, *strides, 9, ps,
-                                       P(1 << 20), ld, cols, P(1 << 20), 0, heads, kv, dim, window, 0.1, P(1 << 20),
-                                       heads * dim, dim, None, None, None, 0, None)
+
+def test_parameter_blocks_match_the_header():
+    """Every field of a block is 8 bytes, doubles last: the packed format has the header's fields."""
+    text = open(os.path.join(REPO, "include", "cv3cuda.h")).read()
+    p = pkg("paged")
+    for name, fmt in BLOCKS.items():
+        body = re.search(r"typedef struct %s_params \{(.*?)\} %s_params;" % (name, name), text, re.S).group(1)
+        kinds = []
+        for line in filter(None, (x.strip() for x in body.split(";"))):
+            t = "q" if "*" in line or line.startswith("int64_t") else "d" if line.startswith("double") else "?"
+            kinds += [t] * len(line.split(","))
+        f = getattr(p, fmt)
+        assert "?" not in kinds and kinds == sorted(kinds, reverse=True)
+        assert f.size == 8 * len(kinds) and f.unpack(f.pack(*([0] * len(kinds)))).count(0.0) == len(kinds)
+        assert f.format.lstrip("=") in ("%dq" % len(kinds), "%dqd" % (len(kinds) - 1))
+        assert f.format.endswith("d") == (kinds[-1] == "d")
+
+
+def test_c_entries_refuse_before_any_device_work():
+    L, p = pkg("_lib"), pkg("paged")
+    lib = L.load()
+    V, U = L.CV3_ERR_VALUE, L.CV3_ERR_UNSUPPORTED
+    at = 1 << 20
+
+    def attention(dim=64, kv=2, heads=4, ps=16, strides=(2048, 1024, 64), k=at, kt=0, cols=3, ld=3, window=0, batch=0,
+                  words=0, size=p._ATTENTION.size):
+        return lib.cv3_paged_attention(p._ATTENTION.pack(
+            size, at, 0, heads * dim, dim, k, at, kt, *strides, *strides, 9, ps, at, ld, cols, at, batch, heads, kv, dim,
+            window, at, heads * dim, dim, 0, 0, 0, words, 0.1), None)
     assert attention() == 0                                  # no requests: nothing to do
+    assert attention(size=8) == V and b"parameter block" in lib.cv3_last_error()
     assert attention(dim=80) == U and b"head_dim" in lib.cv3_last_error()
     assert attention(kv=3) == V and b"not a multiple" in lib.cv3_last_error()
     assert attention(strides=(2048, 1024, 62)) == V and b"16-byte" in lib.cv3_last_error()
-    assert attention(k=(1 << 20) + 4) == V
+    assert attention(k=at + 4) == V
     assert attention(kt=5) == V and attention(ps=0) == V and attention(ld=2) == V and attention(window=-1) == V
     assert attention(cols=1 << 28, ld=1 << 28) == V and b"32-bit" in lib.cv3_last_error()
+    assert attention(cols=5000, ld=5000, batch=2) == V and b"workspace" in lib.cv3_last_error()
+    assert lib.cv3_paged_attention(None, None) == V
 
-    def append(dim=64, ldq=8 * 64, rows=0, qkv=1 << 20, cos=None, sin=None, t=0):
-        return lib.cv3_paged_append(P(qkv), t, rows, ldq, cos, sin, 0, None, None, 4, 2, dim, P(1 << 20), P(1 << 20),
-                                    P(1 << 20), 0, 2048, 1024, 64, 2048, 1024, 64, 9, 16, None, None)
+    def append(dim=64, ldq=8 * 64, rows=0, qkv=at, cos=0, sin=0, t=0, size=p._APPEND.size):
+        return lib.cv3_paged_append(p._APPEND.pack(size, qkv, t, rows, ldq, cos, sin, 0, 0, 0, 4, 2, dim, at, at, at, 0, 2048,
+                                                   1024, 64, 2048, 1024, 64, 9, 16, 0), None)
     assert append() == 0
     assert append(dim=72) == U and append(ldq=500) == V and append(ldq=8 * 64 + 2) == V and append(t=3) == V
-    assert append(qkv=(1 << 20) + 8) == V and append(cos=P(1 << 20)) == V
+    assert append(qkv=at + 8) == V and append(cos=at) == V and append(size=0) == V
 
-    def extend(tokens=4, ps=16, cols=3, ld=3, cap=9):
-        return lib.cv3_paged_extend(None, None, None, 2, None, ld, cols, ps, None, cap, None, tokens, *[None] * 8)
+    def extend(tokens=4, ps=16, cols=3, ld=3, cap=9, size=p._EXTEND.size):
+        return lib.cv3_paged_extend(p._EXTEND.pack(size, 0, 0, 0, 2, 0, ld, cols, ps, 0, cap, 0, tokens, *[0] * 7), None)
     assert extend(ps=0) == V and extend(tokens=-1) == V and extend(ld=2) == V and extend(tokens=1 << 31) == V
-    assert extend(cols=1 << 28, ld=1 << 28) == V and extend(cap=-1) == V
+    assert extend(cols=1 << 28, ld=1 << 28) == V and extend(cap=-1) == V and extend(size=152) == V
 
-    def beam(beams=4, vocab=100, ld=100, stop=(0, 0), t=0, ws=None, size=0, groups=2):
-        return lib.cv3_beam_select(None, t, ld, groups, beams, vocab, None, None, None, *stop, None, 0.0, None, None, None,
-                                   None, None, ws, size, None)
+    def beam(beams=4, vocab=100, ld=100, stop=(0, 0), t=0, groups=2, ws=0, words=0, size=p._BEAM.size):
+        return lib.cv3_beam_select(p._BEAM.pack(size, 0, t, ld, groups, beams, vocab, 0, 0, 0, *stop, *[0] * 6, ws, words, 0.0),
+                                   None)
     assert beam(groups=0) == 0
     assert beam(beams=33) == U and beam(beams=0) == U and beam(ld=99) == V and beam(stop=(5, 4)) == V and beam(t=9) == V
-    assert beam() == V and b"workspace" in lib.cv3_last_error()
-    assert beam(ws=P(1 << 20), size=lib.cv3_beam_workspace(2, 4, 100) - 1) == V
-    assert beam(ws=P((1 << 20) + 4), size=1 << 20) == V
+    assert beam(groups=40000) == U and beam(size=1) == V
+    need = lib.cv3_beam_workspace(1, 32, 10 ** 7)
+    assert need > 0 and beam(groups=1, beams=32, vocab=10 ** 7, ld=10 ** 7, ws=at, words=need - 1) == V
+    assert b"workspace" in lib.cv3_last_error()
+    assert beam(groups=1, beams=32, vocab=10 ** 7, ld=10 ** 7, ws=at + 4, words=need) == V
 
-    def reorder(beams=4, dim=64, st=64, t=0, groups=0):
+    def reorder(beams=4, dim=64, st=64, t=0, groups=0, size=p._REORDER.size):
         s = (1 << 16, 2048, 1024, st)
-        return lib.cv3_paged_reorder(P(1 << 20), P(1 << 20), t, 2, 9, 2, 16, dim, *s, *s, None, 3, 3, None, None, groups,
-                                     beams, None)
+        return lib.cv3_paged_reorder(p._REORDER.pack(size, at, at, t, 2, 9, 2, 16, dim, *s, *s, 0, 3, 3, 0, 0, groups, beams), None)
     assert reorder() == 0 and reorder(beams=1, groups=3) == 0
     assert reorder(beams=33) == U and reorder(st=63) == V and reorder(dim=62, st=64) == V and reorder(t=4) == V
+    assert reorder(size=3) == V
     with pytest.raises(RuntimeError):
         L.check(reorder(beams=33), "cv3_paged_reorder")
 
