@@ -2,6 +2,17 @@
 //
 // key(k, v) = (score_k + log_softmax(x_k)_v) / (count_k + 1)^alpha; a finished hypothesis offers
 // itself, unchanged, as its one candidate.  Equal keys go to the lowest k * V + v.
+//
+// Bound by the logits' bytes, which are read once.  Within a hypothesis the key grows with the logit,
+// so a row gives its K largest logits (lowest token on ties) and its log-sum-exp; the K * K candidates
+// are then ordered by keys in 64 bits.  Each warp walks tiles of 512 logits with 16-byte loads and
+// keeps, lane i the i-th, the K best of them: a tile costs one vote unless it beats the K-th (of this
+// warp or, shared, of another one).
+//
+// Precision: candidates of different hypotheses may lie closer than fp32 resolves, so the log-sum-exp
+// is held to about 1e-9.  Terms within e^-5 of the running maximum are evaluated in 64 bits; the
+// others, each below 1/150 of the sum, in fp32 (relative errors of a few 2^-24, of either sign, which
+// over many terms cancel), 16 at a time, and added up in 64 bits.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -10,9 +21,7 @@ namespace {
 
 struct BeamArgs {
   const void* logits;
-  int type;
   int64_t ld;
-  int64_t groups;
   int beams;
   int64_t vocab;
   const float* scores;
@@ -24,14 +33,20 @@ struct BeamArgs {
   int* parents;
   float* scores_out;
   int *counts_out, *done_out;
-  int64_t chunks;
-  // workspace: per (row, chunk) the largest logit, the sum of exp against it, and the best candidates
-  double* sum;
-  float* top;
-  unsigned long long* cand;  // [row][chunk][beams]: ordered logit << 32 | ~token; 0: none
+  int chunks;      // of a row
+  int64_t tiles;   // of a chunk
+  char* work;      // the tasks' results of all groups (two launches)
 };
 
-constexpr int BT = 256, BE = 16;  // threads, logits per thread: a chunk has BT * BE
+typedef unsigned long long u64;
+
+constexpr int BW = 8, BT = BW * 32;
+constexpr int TILE = 512;      // logits of a warp's step, 16 a lane
+constexpr float NEAR = 5.f;
+
+// A task's (row's chunk's) result: sum of exp against the largest logit, that logit, then `beams`
+// candidates: ordered logit << 32 | ~token, 0 for none.
+__host__ __device__ constexpr int64_t task_bytes(int64_t beams) { return 16 + 8 * beams; }
 
 // floats in an order that unsigned comparison follows; -0 and +0 are one value
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -41,106 +56,230 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 __device__ __forceinline__ float unordered(uint32_t u) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
 }
-__device__ __forceinline__ unsigned long long ordered(double x) {
-  const unsigned long long u = __double_as_longlong(x + 0.0);
+__device__ __forceinline__ u64 ordered(double x) {
+  const u64 u = __double_as_longlong(x + 0.0);
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
 // A hypothesis that nothing can continue: no (or NaN) score.
 __device__ __forceinline__ bool dead(float score) { return !(score > -INFINITY); }
 
-// The warp's list of the n largest keys, lane i the i-th: puts in `key` of every lane that beats the n-th.
-__device__ __forceinline__ void list_add(unsigned long long key, unsigned long long& list, int n) {
-  const int lane = threadIdx.x & 31;
-  unsigned long long last = __shfl_sync(0xffffffffu, list, n - 1);
-  unsigned wins = __ballot_sync(0xffffffffu, key > last);
-  while (wins) {
-    const int src = __ffs(wins) - 1;
-    const unsigned long long x = __shfl_sync(0xffffffffu, key, src);
-    const int at = __popc(__ballot_sync(0xffffffffu, list > x));
-    const unsigned long long up = __shfl_up_sync(0xffffffffu, list, 1);
-    list = lane < at ? list : lane == at ? x : up;
-    if (lane >= n) list = 0;
-    last = __shfl_sync(0xffffffffu, list, n - 1);
-    if (lane == src) key = 0;
-    wins = __ballot_sync(0xffffffffu, key > last);
-  }
-}
+// Rows whose logits are not looked at: finished hypotheses and those that do not exist.
+__device__ __forceinline__ bool skipped(const BeamArgs& a, int64_t row) { return a.done[row] || dead(a.scores[row]); }
 
-__global__ void __launch_bounds__(BT) beam_scan_kernel(const BeamArgs a) {
-  __shared__ float redf[32];
-  __shared__ double redd[BT / 32];
-  __shared__ unsigned long long lists[BT / 32][32];
-  dep_wait();
-  dep_release();
-  const int64_t row = blockIdx.y, chunk = blockIdx.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (a.done[row]) return;
-  const int64_t v0 = chunk * BT * BE;
-  const bool none = dead(a.scores[row]);
-  const bool early = a.min_len && a.counts[row] < a.min_len[row / a.beams];
-  float x[BE], m = -INFINITY;
-#pragma unroll
-  for (int e = 0; e < BE; ++e) {
-    const int64_t v = v0 + e * BT + threadIdx.x;
-    x[e] = v < a.vocab ? cv3p::load_any(a.logits, a.type, row * a.ld + v) : -INFINITY;
-    if (x[e] != x[e]) x[e] = -INFINITY;  // NaN: no candidate
-    m = fmaxf(m, x[e]);
-  }
-  m = block_max(m, redf);
-  double s = 0.0;
-#pragma unroll
-  for (int e = 0; e < BE; ++e)
-    if (x[e] > -INFINITY) s += x[e] == m ? 1.0 : exp((double)x[e] - (double)m);
-  s = warp_sum_d(s);
-  if (lane == 0) redd[warp] = s;
-  unsigned long long list = 0;
-#pragma unroll 1
-  for (int e = 0; e < BE; ++e) {
-    const int64_t v = v0 + e * BT + threadIdx.x;
-    const bool out = none || (early && v >= a.stop_lo && v < a.stop_hi);
-    const unsigned long long key =
-        v < a.vocab ? (unsigned long long)ordered(out ? -INFINITY : x[e]) << 32 | (uint32_t)~(uint32_t)v : 0ull;
-    list_add(key, list, a.beams);
-  }
-  lists[warp][lane] = list;
-  __syncthreads();
-  if (warp == 0) {
-    for (int w = 1; w < BT / 32; ++w) list_add(lists[w][lane], list, a.beams);
-    const int64_t at = row * a.chunks + chunk;
-    if (lane < a.beams) a.cand[at * a.beams + lane] = list;
-    if (lane == 0) {
-      double t = 0.0;
-      for (int w = 0; w < BT / 32; ++w) t += redd[w];
-      a.sum[at] = t;
-      a.top[at] = m;
-    }
-  }
-}
-
-// a candidate: ordered key, then lowest k * V + v
+// A candidate of the choice: ordered key, then lowest k * V + v.
 struct Cand {
-  unsigned long long key;
-  unsigned long long tie;  // ~(k * V + v)
+  u64 key;
+  u64 tie;  // ~(k * V + v)
 };
 
+__device__ __forceinline__ bool better(u64 x, u64 y) { return x > y; }
 __device__ __forceinline__ bool better(const Cand& x, const Cand& y) {
   return x.key > y.key || (x.key == y.key && x.tie > y.tie);
 }
+__device__ __forceinline__ u64 from_lane(u64 x, int lane) { return __shfl_sync(0xffffffffu, x, lane); }
+__device__ __forceinline__ Cand from_lane(const Cand& x, int lane) { return {from_lane(x.key, lane), from_lane(x.tie, lane)}; }
+__device__ __forceinline__ u64 across(u64 x, int j) { return __shfl_xor_sync(0xffffffffu, x, j); }
+__device__ __forceinline__ Cand across(const Cand& x, int j) { return {across(x.key, j), across(x.tie, j)}; }
 
-__device__ __forceinline__ void list_add(Cand c, Cand& list, int n) {
+// The warp's lists: lane i holds the i-th best, zeros behind the last.  A bitonic network sorts 32
+// entries in 15 exchanges; two sorted lists give the 32 best of both in 5.
+template <typename X>
+__device__ __forceinline__ X exchange(X x, int j, bool keep_better) {
+  const X y = across(x, j);
+  return better(x, y) == keep_better ? x : y;
+}
+template <typename X>
+__device__ __forceinline__ X sorted(X x) {
   const int lane = threadIdx.x & 31;
-  for (;;) {
-    Cand last = {__shfl_sync(0xffffffffu, list.key, n - 1), __shfl_sync(0xffffffffu, list.tie, n - 1)};
-    const unsigned wins = __ballot_sync(0xffffffffu, better(c, last));
-    if (!wins) return;
-    const int src = __ffs(wins) - 1;
-    const Cand x = {__shfl_sync(0xffffffffu, c.key, src), __shfl_sync(0xffffffffu, c.tie, src)};
-    const int at = __popc(__ballot_sync(0xffffffffu, better(list, x)));
-    const Cand up = {__shfl_up_sync(0xffffffffu, list.key, 1), __shfl_up_sync(0xffffffffu, list.tie, 1)};
-    list = lane < at ? list : lane == at ? x : up;
-    if (lane >= n) list = Cand{0, 0};
-    if (lane == src) c = Cand{0, 0};
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) x = exchange(x, j, ((lane & j) == 0) == ((lane & k) == 0));
+  return x;
+}
+template <typename X>
+__device__ __forceinline__ X merged(X x, const X& other) {
+  const int lane = threadIdx.x & 31;
+  const X y = from_lane(other, 31 - lane);
+  x = better(x, y) ? x : y;
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) x = exchange(x, j, (lane & j) == 0);
+  return x;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& r, float* x) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned short u = (unsigned short)(h ? w[i] >> 16 : w[i]);
+        T v;
+        memcpy(&v, &u, 2);
+        x[2 * i + h] = cv3p::to_f32<T>(v);
+      }
+  }
+}
+
+// One task by the whole CTA.  Rows need not begin on 16-byte boundaries: a row is taken as the
+// 16-byte blocks that hold at least one of its logits, and what else they hold is masked.
+// `bar` (shared): the best K-th logit of any warp so far; nothing below it can be among the K best.
+// The result is in warp 0: list, and in every lane m and s.
+template <typename T>
+__device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, u64 (&lists)[BW][32], float (&ms)[BW],
+                     double (&ss)[BW], uint32_t& bar, u64& list, float& m, double& s) {
+  constexpr int E = 16 / sizeof(T), J = 16 / E;  // logits of a block; blocks of a lane's step
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, K = a.beams;
+  const T* x0 = static_cast<const T*>(a.logits) + row * a.ld;
+  const int off = (int)(((uintptr_t)x0 & 15) / sizeof(T));
+  const uint4* blocks = reinterpret_cast<const uint4*>(x0 - off);
+  const int64_t nb = (a.vocab + off + E - 1) / E;
+  const bool early = a.min_len && a.counts[row] < a.min_len[row / K] && a.stop_lo < a.stop_hi;
+  __syncthreads();  // (the last task's shared memory is done with)
+  if (threadIdx.x == 0) bar = 0;
+  __syncthreads();
+  list = 0;
+  u64 last = 0;  // the list's K-th
+  bool started = false;
+  m = -INFINITY;
+  s = 0.0;
+  const int64_t end = min((chunk + 1) * a.tiles * (TILE / E), nb);
+  for (int64_t i0 = chunk * a.tiles * (TILE / E) + warp * (TILE / E); i0 < end; i0 += BW * (TILE / E)) {
+    uint4 raw[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int64_t i = i0 + j * 32 + lane;
+      raw[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (i < nb)
+        asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(raw[j].x), "=r"(raw[j].y), "=r"(raw[j].z), "=r"(raw[j].w) : "l"(blocks + i));
+    }
+    float x[16];
+#pragma unroll
+    for (int j = 0; j < J; ++j) unpack<T>(raw[j], x + j * E);
+    const int64_t v0 = i0 * E - off;  // token of the step's first logit
+    auto token = [&](int e) -> int64_t { return v0 + (int64_t)((e / E) * 32 + lane) * E + e % E; };
+    unsigned valid = 0xFFFFu;
+    if (v0 < 0 || v0 + TILE > a.vocab) {
+      valid = 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const bool in = token(e) >= 0 && token(e) < a.vocab;
+        valid |= (in ? 1u : 0u) << e;
+        x[e] = in ? x[e] : -INFINITY;
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      x[e] = fmaxf(x[e], -INFINITY);  // NaN: no candidate
+      top = fmaxf(top, x[e]);
+    }
+    // the sum of exp
+    const float wtop = warp_max(top);
+    if (wtop > m) {
+      s *= m > -INFINITY ? exp((double)m - (double)wtop) : 0.0;
+      m = wtop;
+    }
+    if (m > -INFINITY) {
+      float t[16];
+      if (__any_sync(0xffffffffu, top >= m - NEAR)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const bool near = x[e] >= m - NEAR;
+          if (near) s += x[e] == m ? 1.0 : exp((double)x[e] - (double)m);  // (m may be infinite)
+          t[e] = near ? 0.f : expf(x[e] - m);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t[e] = expf(x[e] - m);
+      }
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+        for (int e = 0; e < w; ++e) t[e] += t[e + w];
+      s += (double)t[0];
+    }
+    // candidates
+    if (early) {
+      top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (token(e) >= a.stop_lo && token(e) < a.stop_hi) x[e] = -INFINITY;
+        top = fmaxf(top, x[e]);
+      }
+    }
+    const uint32_t others = *(volatile uint32_t*)&bar;
+    const uint32_t last_x = (uint32_t)(last >> 32);
+    if (last != 0 && !__any_sync(0xffffffffu, ordered(top) > last_x && ordered(top) >= others)) continue;
+    u64 key;
+    int place;
+    auto best = [&]() {  // the lane's best of what is left
+      float bx = 0.f;
+      place = -1;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if ((valid >> e & 1u) && (place < 0 || x[e] > bx)) {
+          bx = x[e];
+          place = e;
+        }
+      key = place < 0 ? 0ull : (u64)ordered(bx) << 32 | (uint32_t)~(uint32_t)token(place);
+    };
+    best();
+    if (!started) {  // the lanes' best ones, sorted, bound the rest from below
+      started = true;
+      list = sorted(key);
+      if (lane >= K) list = 0;
+      last = from_lane(list, K - 1);
+      if (key != 0 && key >= last) {
+        valid &= ~(1u << place);
+        best();
+      }
+    }
+    for (;;) {
+      const unsigned wins = __ballot_sync(0xffffffffu, key > last && (uint32_t)(key >> 32) >= others);
+      if (!wins) break;
+      const int src = __ffs(wins) - 1;
+      const u64 k = from_lane(key, src);
+      const int at = __popc(__ballot_sync(0xffffffffu, list > k));
+      const u64 up = __shfl_up_sync(0xffffffffu, list, 1);
+      list = lane < at ? list : lane == at ? k : up;
+      if (lane >= K) list = 0;
+      last = from_lane(list, K - 1);
+      if (lane == src) {
+        valid &= ~(1u << place);
+        best();
+      }
+    }
+    if (lane == 0 && last != 0 && (uint32_t)(last >> 32) > others) atomicMax(&bar, (uint32_t)(last >> 32));
+  }
+  s = warp_sum_d(s);
+  lists[warp][lane] = list;
+  if (lane == 0) { ms[warp] = m; ss[warp] = s; }
+  __syncthreads();
+#pragma unroll
+  for (int w = BW / 2; w > 0; w >>= 1) {
+    if (warp < w) {
+      list = merged(list, lists[warp + w][lane]);
+      if (lane >= K) list = 0;
+      lists[warp][lane] = list;
+    }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    m = -INFINITY;
+    s = 0.0;
+#pragma unroll
+    for (int w = 0; w < BW; ++w) m = fmaxf(m, ms[w]);
+#pragma unroll
+    for (int w = 0; w < BW; ++w)
+      if (ms[w] > -INFINITY) s += ss[w] * (ms[w] == m ? 1.0 : exp((double)ms[w] - (double)m));
   }
 }
 
@@ -151,25 +290,27 @@ __device__ __forceinline__ double continued(double base, float x, float top, dou
   return c == c ? c : -(double)INFINITY;  // (an infinite score and an impossible token)
 }
 
-__global__ void __launch_bounds__(BT) beam_pick_kernel(const BeamArgs a) {
+// The group's choice by one CTA, from its tasks' results (global or shared memory).
+template <typename T>
+__device__ void choose(const BeamArgs& a, int64_t g, const char* work) {
   __shared__ double lsum[CV3_MAX_BEAMS], base[CV3_MAX_BEAMS], norm[CV3_MAX_BEAMS];
   __shared__ float tops[CV3_MAX_BEAMS];
-  __shared__ Cand lists[BT / 32][32];
-  dep_wait();
-  dep_release();
-  const int64_t g = blockIdx.x;
+  __shared__ int fins[CV3_MAX_BEAMS];
+  __shared__ Cand lists[BW][32];
   const int K = a.beams, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int k = warp; k < K; k += BT / 32) {
+  const int64_t tb = task_bytes(K);
+  for (int k = warp; k < K; k += BW) {
     const int64_t row = g * K + k;
-    const bool fin = a.done[row] != 0;
+    const bool fin = a.done[row] != 0, skip = skipped(a, row);
     float m = -INFINITY;
     double s = 0.0;
-    if (!fin) {
-      for (int64_t c = lane; c < a.chunks; c += 32) m = fmaxf(m, a.top[row * a.chunks + c]);
+    if (!skip) {
+      const char* w = work + (int64_t)k * a.chunks * tb;
+      for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, *reinterpret_cast<const float*>(w + c * tb + 8));
       m = warp_max(m);
-      for (int64_t c = lane; c < a.chunks; c += 32) {
-        const float t = a.top[row * a.chunks + c];
-        if (t > -INFINITY) s += a.sum[row * a.chunks + c] * (t == m ? 1.0 : exp((double)t - (double)m));
+      for (int c = lane; c < a.chunks; c += 32) {
+        const float t = *reinterpret_cast<const float*>(w + c * tb + 8);
+        if (t > -INFINITY) s += *reinterpret_cast<const double*>(w + c * tb) * (t == m ? 1.0 : exp((double)t - (double)m));
       }
       s = warp_sum_d(s);
     }
@@ -180,45 +321,53 @@ __global__ void __launch_bounds__(BT) beam_pick_kernel(const BeamArgs a) {
       lsum[k] = log(s);
       base[k] = dead(sc) ? -INFINITY : (double)sc;
       norm[k] = a.alpha == 0.0 ? 1.0 : pow((double)max(n, 1), a.alpha);
+      fins[k] = fin ? 2 : skip;
     }
   }
   __syncthreads();
   Cand list = {0, 0};
-  const int64_t per = a.chunks * K, all = per * K;
-  for (int64_t i0 = warp * 32; i0 < all; i0 += BT) {
-    const int64_t i = i0 + lane;
+  const int per = a.chunks * K, all = per * K;
+  for (int i0 = warp * 32; i0 < all; i0 += BT) {
+    const int i = i0 + lane;
     Cand c = {0, 0};
     if (i < all) {
-      const int k = (int)(i / per);
-      const int64_t row = g * K + k;
-      if (a.done[row]) {
-        const int64_t v = i - (int64_t)k * per;  // itself, then what stands in where nothing is left
-        if (v < K && v < a.vocab)
-          c = Cand{ordered(v == 0 ? base[k] / norm[k] : -(double)INFINITY), ~(unsigned long long)(k * a.vocab + v)};
+      const int k = i / per, r = i - k * per;
+      if (fins[k]) {  // a finished one itself, then what stands in where nothing is left
+        if (r < K && r < a.vocab)
+          c = Cand{ordered(r == 0 && fins[k] == 2 ? base[k] / norm[k] : -(double)INFINITY), ~(u64)(k * a.vocab + r)};
       } else {
-        const unsigned long long u = a.cand[row * per + (i - (int64_t)k * per)];
-        if (u) {
-          const float x = unordered((uint32_t)(u >> 32));
-          const uint32_t v = ~(uint32_t)u;
-          c = Cand{ordered(continued(base[k], x, tops[k], lsum[k]) / norm[k]), ~(unsigned long long)(k * a.vocab + v)};
-        }
+        const u64 u = *reinterpret_cast<const u64*>(work + (int64_t)(k * a.chunks + r / K) * tb + 16 + r % K * 8);
+        if (u)
+          c = Cand{ordered(continued(base[k], unordered((uint32_t)(u >> 32)), tops[k], lsum[k]) / norm[k]),
+                   ~(u64)(k * a.vocab + (uint32_t)~(uint32_t)u)};
       }
     }
-    list_add(c, list, K);
+    const Cand last = from_lane(list, K - 1);
+    if (!__any_sync(0xffffffffu, better(c, last))) continue;
+    list = merged(list, sorted(c));
+    if (lane >= K) list = Cand{0, 0};
   }
   lists[warp][lane] = list;
   __syncthreads();
-  if (warp) return;
-  for (int w = 1; w < BT / 32; ++w) list_add(lists[w][lane], list, K);
-  if (lane >= K) return;
+#pragma unroll
+  for (int w = BW / 2; w > 0; w >>= 1) {
+    if (warp < w && w * 32 < all) {  // (warps beyond the candidates have empty lists)
+      list = merged(list, lists[warp + w][lane]);
+      if (lane >= K) list = Cand{0, 0};
+      lists[warp][lane] = list;
+    }
+    __syncthreads();
+  }
+  if (warp || lane >= K) return;
   const int64_t id = (int64_t)~list.tie;
   const int k = (int)(id / a.vocab);
   const int64_t v = id - (int64_t)k * a.vocab, row = g * K + k, to = g * K + lane;
-  const bool fin = a.done[row] != 0;
+  const bool fin = fins[k] == 2;
   double cum = -(double)INFINITY;
-  if (list.key > ordered(-(double)INFINITY)) {
-    cum = fin ? base[k] : continued(base[k], cv3p::load_any(a.logits, a.type, row * a.ld + v), tops[k], lsum[k]);
-  }
+  if (list.key > ordered(-(double)INFINITY))
+    cum = fin ? base[k]
+              : continued(base[k], fmaxf(cv3p::to_f32<T>(static_cast<const T*>(a.logits)[row * a.ld + v]), -INFINITY), tops[k],
+                          lsum[k]);
   const int count = a.counts[row] + (fin ? 0 : 1);
   __syncwarp(0xffffffffu >> (32 - K));  // the outputs may be the inputs' own buffers
   a.tokens[to] = fin ? 0 : v;
@@ -228,12 +377,123 @@ __global__ void __launch_bounds__(BT) beam_pick_kernel(const BeamArgs a) {
   a.done_out[to] = fin || (v >= a.stop_lo && v < a.stop_hi) ? 1 : 0;
 }
 
-int64_t chunks_of(int64_t vocab) { return (vocab + BT * BE - 1) / (BT * BE); }
+// two launches: a CTA per task, then one per group
+template <typename T>
+__global__ void __launch_bounds__(BT, 4) beam_scan_kernel(const BeamArgs a) {
+  __shared__ u64 lists[BW][32];
+  __shared__ float ms[BW];
+  __shared__ double ss[BW];
+  __shared__ uint32_t bar;
+  dep_wait();
+  dep_release();
+  const int64_t row = blockIdx.y;
+  if (skipped(a, row)) return;
+  u64 list;
+  float m;
+  double s;
+  scan<T>(a, row, blockIdx.x, lists, ms, ss, bar, list, m, s);
+  if (threadIdx.x < 32) {
+    char* w = a.work + (row * a.chunks + blockIdx.x) * task_bytes(a.beams);
+    if (threadIdx.x < a.beams) reinterpret_cast<u64*>(w + 16)[threadIdx.x] = list;
+    if (threadIdx.x == 0) {
+      *reinterpret_cast<double*>(w) = s;
+      *reinterpret_cast<float*>(w + 8) = m;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(BT) beam_pick_kernel(const BeamArgs a) {
+  dep_wait();
+  dep_release();
+  const int64_t g = blockIdx.x;
+  choose<T>(a, g, a.work + g * a.beams * a.chunks * task_bytes(a.beams));
+}
+
+__device__ __forceinline__ void put8(uint32_t at, u64 x) {
+  asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(at), "l"(x) : "memory");
+}
+
+// one launch: a cluster per group shares its tasks; the results go to the first CTA's shared memory
+template <typename T>
+__global__ void __launch_bounds__(BT) beam_cluster_kernel(const BeamArgs a, int cluster) {
+  extern __shared__ __align__(16) char work[];
+  __shared__ u64 lists[BW][32];
+  __shared__ float ms[BW];
+  __shared__ double ss[BW];
+  __shared__ uint32_t bar;
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  dep_wait();
+  dep_release();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA of the cluster runs
+  const int64_t g = blockIdx.x / cluster;
+  const int rank = blockIdx.x % cluster;
+  uint32_t first;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(first) : "r"((uint32_t)__cvta_generic_to_shared(work)));
+  for (int i = rank; i < a.beams * a.chunks; i += cluster) {
+    const int64_t row = g * a.beams + i / a.chunks;
+    if (skipped(a, row)) continue;
+    u64 list;
+    float m;
+    double s;
+    scan<T>(a, row, i % a.chunks, lists, ms, ss, bar, list, m, s);
+    if (threadIdx.x < 32) {
+      const uint32_t at = first + (uint32_t)(i * task_bytes(a.beams));
+      if (threadIdx.x < a.beams) put8(at + 16 + threadIdx.x * 8, list);
+      if (threadIdx.x == 0) {
+        put8(at, __double_as_longlong(s));
+        put8(at + 8, __float_as_uint(m));
+      }
+    }
+  }
+  cv3p::cluster_sync();
+  if (rank == 0) choose<T>(a, g, work);
+}
+
+// How a call is cut.  One launch where every warp of a cluster then walks at most CLUSTER_TILES tiles
+// of its group; else two, with chunks enough for four CTAs on every SM, a tile per warp at least.
+struct Plan {
+  int64_t cluster, chunks, tiles, bytes;  // cluster 0: two launches; bytes of results
+};
+constexpr int64_t CLUSTER = 8, CLUSTER_TILES = 16;  // (at most 32 tasks: 9 KB of results in shared memory)
+
+Plan plan_of(int64_t groups, int64_t beams, int64_t vocab) {
+  Plan p = {};
+  const int64_t row = (vocab + 7 + TILE - 1) / TILE;  // tiles of a row, its first block's share included
+  auto cut = [&](int64_t chunks) {
+    p.tiles = (std::max<int64_t>(1, (row + chunks - 1) / chunks) + BW - 1) / BW * BW;
+    p.chunks = (row + p.tiles - 1) / p.tiles;
+  };
+  if (beams * ((row + BW - 1) / BW) <= CLUSTER * CLUSTER_TILES) {
+    cut(std::max<int64_t>(1, CLUSTER / beams));
+    p.cluster = std::min<int64_t>(CLUSTER, beams * p.chunks);
+    while (p.cluster & (p.cluster - 1)) ++p.cluster;  // a power of two
+  } else {
+    cut(std::max<int64_t>(1, 4 * cv3::sm_count() / (groups * beams)));
+  }
+  p.bytes = (p.cluster ? 1 : groups) * beams * p.chunks * task_bytes(beams);
+  return p;
+}
+
+template <typename T>
+int launch(const BeamArgs& a, const Plan& plan, int64_t groups, cudaStream_t st) {
+  if (plan.cluster) {
+    return cv3::check_launch("beam_select",
+                             cv3p::launch_cluster(beam_cluster_kernel<T>, dim3((unsigned)(groups * plan.cluster)), dim3(BT),
+                                                  (size_t)plan.bytes, (unsigned)plan.cluster, st, a, (int)plan.cluster));
+  }
+  int rc = cv3::check_launch("beam_scan", cv3::launch_dep(beam_scan_kernel<T>, dim3((unsigned)plan.chunks, (unsigned)(groups * a.beams)),
+                                                          dim3(BT), 0, st, a));
+  if (rc) return rc;
+  return cv3::check_launch("beam_pick", cv3::launch_dep(beam_pick_kernel<T>, dim3((unsigned)groups), dim3(BT), 0, st, a));
+}
 
 }  // namespace
 
 extern "C" int64_t cv3_beam_workspace(int64_t groups, int64_t beams, int64_t vocab) {
-  return groups * beams * chunks_of(vocab) * (16 + 8 * beams);
+  if (groups <= 0 || beams <= 0 || beams > CV3_MAX_BEAMS || vocab <= 0) return 0;
+  const Plan p = plan_of(groups, beams, vocab);
+  return p.cluster ? 0 : p.bytes;
 }
 
 extern "C" int cv3_beam_select(const cv3_beam_params* p, void* stream) {
@@ -245,19 +505,16 @@ extern "C" int cv3_beam_select(const cv3_beam_params* p, void* stream) {
   CV3_REQUIRE(cv3p::type_ok(p->type), CV3_ERR_VALUE, "beam_select: unknown element type");
   CV3_REQUIRE(p->groups <= 65535 && p->groups * p->beams <= 65535, CV3_ERR_UNSUPPORTED,
               "beam_select: more than 65535 hypotheses");
+  CV3_REQUIRE((uintptr_t)p->logits % cv3p::type_size(p->type) == 0, CV3_ERR_VALUE, "beam_select: misaligned logits");
   if (p->groups == 0) return CV3_OK;
-  const int64_t chunks = chunks_of(p->vocab), n = p->groups * p->beams * chunks;
-  CV3_REQUIRE(p->workspace && p->workspace_bytes >= cv3_beam_workspace(p->groups, p->beams, p->vocab) &&
-                  ((uintptr_t)p->workspace & 7) == 0,
+  const Plan plan = plan_of(p->groups, p->beams, p->vocab);
+  CV3_REQUIRE(plan.cluster || (p->workspace && p->workspace_bytes >= plan.bytes && ((uintptr_t)p->workspace & 7) == 0),
               CV3_ERR_VALUE, "beam_select: the workspace must hold cv3_beam_workspace() bytes");
-  char* w = static_cast<char*>(p->workspace);
-  const BeamArgs a = {p->logits, (int)p->type, p->ld, p->groups, (int)p->beams, p->vocab, p->scores, p->counts, p->done,
-                      p->stop_lo, p->stop_hi, p->min_len, p->length_penalty, p->tokens, p->parents, p->scores_out,
-                      p->counts_out, p->done_out, chunks, reinterpret_cast<double*>(w), reinterpret_cast<float*>(w + 8 * n),
-                      reinterpret_cast<unsigned long long*>(w + 16 * n)};
+  const BeamArgs a = {p->logits, p->ld, (int)p->beams, p->vocab, p->scores, p->counts, p->done, p->stop_lo, p->stop_hi,
+                      p->min_len, p->length_penalty, p->tokens, p->parents, p->scores_out, p->counts_out, p->done_out,
+                      (int)plan.chunks, plan.tiles, static_cast<char*>(p->workspace)};
   cudaStream_t st = cv3::as_stream(stream);
-  int rc = cv3::check_launch("beam_scan", cv3::launch_dep(beam_scan_kernel, dim3((unsigned)chunks, (unsigned)(p->groups * p->beams)),
-                                                          dim3(BT), 0, st, a));
-  if (rc) return rc;
-  return cv3::check_launch("beam_pick", cv3::launch_dep(beam_pick_kernel, dim3((unsigned)p->groups), dim3(BT), 0, st, a));
+  if (p->type == CV3_TYPE_F32) return launch<float>(a, plan, p->groups, st);
+  if (p->type == CV3_TYPE_F16) return launch<__half>(a, plan, p->groups, st);
+  return launch<__nv_bfloat16>(a, plan, p->groups, st);
 }
