@@ -10,8 +10,8 @@
 // warp or, shared, of another one).
 //
 // Precision: candidates of different hypotheses may lie closer than fp32 resolves, so the log-sum-exp
-// is held to about 1e-9.  Terms within e^-5 of the running maximum are evaluated in 64 bits; the
-// others, each below 1/150 of the sum, in fp32 (relative errors of a few 2^-24, of either sign, which
+// is held to about 1e-8.  Terms within e^-4 of the running maximum are evaluated in 64 bits; the
+// others, each below 1/54 of the sum, in fp32 (relative errors of about 2^-22, of either sign, which
 // over many terms cancel), 16 at a time, and added up in 64 bits.
 #include <algorithm>
 
@@ -42,7 +42,7 @@ typedef unsigned long long u64;
 
 constexpr int BW = 8, BT = BW * 32;
 constexpr int TILE = 512;      // logits of a warp's step, 16 a lane
-constexpr float NEAR = 5.f;
+constexpr float NEAR = 4.f;
 
 // A task's (row's chunk's) result: sum of exp against the largest logit, that logit, then `beams`
 // candidates: ordered logit << 32 | ~token, 0 for none.
@@ -106,6 +106,13 @@ __device__ __forceinline__ X merged(X x, const X& other) {
 #pragma unroll
   for (int j = 16; j > 0; j >>= 1) x = exchange(x, j, (lane & j) == 0);
   return x;
+}
+
+// e^d for d <= 0; log2(e) in two parts, since an error of it would not cancel over the terms
+__device__ __forceinline__ float exp_far(float d) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(d, 1.925963033e-8f, d * 1.442695022f)));
+  return y;
 }
 
 template <typename T>
@@ -175,12 +182,13 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, u64 (&lists)
         x[e] = in ? x[e] : -INFINITY;
       }
     }
-    float top = -INFINITY;
+    float top = -INFINITY;  // (fmaxf passes over NaN)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      x[e] = fmaxf(x[e], -INFINITY);  // NaN: no candidate
-      top = fmaxf(top, x[e]);
-    }
+    for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
+    auto no_nan = [&]() {  // a NaN logit is no candidate and no term
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = fmaxf(x[e], -INFINITY);
+    };
     // the sum of exp
     const float wtop = warp_max(top);
     if (wtop > m) {
@@ -188,23 +196,39 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, u64 (&lists)
       m = wtop;
     }
     if (m > -INFINITY) {
-      float t[16];
-      if (__any_sync(0xffffffffu, top >= m - NEAR)) {
+      const bool close = __any_sync(0xffffffffu, top >= m - NEAR);
+      unsigned near = 0;
+      if (close) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const bool near = x[e] >= m - NEAR;
-          if (near) s += x[e] == m ? 1.0 : exp((double)x[e] - (double)m);  // (m may be infinite)
-          t[e] = near ? 0.f : expf(x[e] - m);
+        for (int e = 0; e < 16; ++e) near |= (x[e] >= m - NEAR ? 1u : 0u) << e;
+        for (unsigned left = near; __any_sync(0xffffffffu, left != 0); left &= left - 1) {
+          float y = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) y = (left & (0u - left)) == 1u << e ? x[e] : y;
+          if (left) s += y == m ? 1.0 : exp((double)y - (double)m);  // (m may be infinite)
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) t[e] = expf(x[e] - m);
       }
+      auto rest = [&]() -> float {
+        float t[16];
+        if (close) {
 #pragma unroll
-      for (int w = 8; w > 0; w >>= 1)
+          for (int e = 0; e < 16; ++e) t[e] = near >> e & 1u ? 0.f : exp_far(x[e] - m);
+        } else {
 #pragma unroll
-        for (int e = 0; e < w; ++e) t[e] += t[e + w];
-      s += (double)t[0];
+          for (int e = 0; e < 16; ++e) t[e] = exp_far(x[e] - m);
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+          for (int e = 0; e < w; ++e) t[e] += t[e + w];
+        return t[0];
+      };
+      float r = rest();
+      if (__any_sync(0xffffffffu, r != r)) {
+        no_nan();
+        r = rest();
+      }
+      s += (double)r;
     }
     // candidates
     if (early) {
@@ -218,6 +242,7 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, u64 (&lists)
     const uint32_t others = *(volatile uint32_t*)&bar;
     const uint32_t last_x = (uint32_t)(last >> 32);
     if (last != 0 && !__any_sync(0xffffffffu, ordered(top) > last_x && ordered(top) >= others)) continue;
+    no_nan();
     u64 key;
     int place;
     auto best = [&]() {  // the lane's best of what is left
