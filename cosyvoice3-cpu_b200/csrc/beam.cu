@@ -3,15 +3,16 @@
 // key(k, v) = (score_k + log_softmax(x_k)_v) / (count_k + 1)^alpha; a finished hypothesis offers
 // itself, unchanged, as its one candidate.  Equal keys go to the lowest k * V + v.
 //
-// Bound by the logits' bytes, which are read once.  Within a hypothesis the key grows with the logit,
-// so a row gives its K largest logits (lowest token on ties) and its log-sum-exp; the K * K candidates
-// are then ordered by keys in 64 bits.  Each warp walks tiles of 512 logits with 16-byte loads and
-// keeps, lane i the i-th, the K best of them: a tile costs one vote unless it beats the K-th (of this
-// warp or, shared, of another one).
+// Bound by the logits' bytes.  Within a hypothesis the key grows with the logit, so a row gives its K
+// largest logits (lowest token on ties) and its log-sum-exp; the K * K candidates are then ordered by
+// keys in 64 bits.  A CTA reads its chunk of a row in tiles of 512 logits, once for the sum and the
+// tiles' maxima; the K-th largest of these maxima bounds the K-th logit from below, so only the tiles
+// that reach it -- K of them, but for ties -- are read again (from L2) for candidates.  (Lists kept
+// while reading cost more than all the rest: 32 x 8 rows over 151936 tokens took 94 us.)
 //
 // Precision: candidates of different hypotheses may lie closer than fp32 resolves, so the log-sum-exp
-// is held to about 1e-8.  Terms within e^-4 of the running maximum are evaluated in 64 bits; the
-// others, each below 1/54 of the sum, in fp32 (relative errors of about 2^-22, of either sign, which
+// is held to about 2e-8.  Terms within e^-2 of the running maximum are evaluated in 64 bits; the
+// others, each below 1/7 of the sum, in fp32 (relative errors of about 2^-23, of either sign, which
 // over many terms cancel), 16 at a time, and added up in 64 bits.
 #include <algorithm>
 
@@ -42,7 +43,8 @@ typedef unsigned long long u64;
 
 constexpr int BW = 8, BT = BW * 32;
 constexpr int TILE = 512;      // logits of a warp's step, 16 a lane
-constexpr float NEAR = 4.f;
+constexpr float NEAR = 2.f;
+constexpr int TILES_MOST = 1024;  // of a task (a multiple of the warps)
 
 // A task's (row's chunk's) result: sum of exp against the largest logit, that logit, then `beams`
 // candidates: ordered logit << 32 | ~token, 0 for none.
@@ -59,6 +61,10 @@ __device__ __forceinline__ float unordered(uint32_t u) {
 __device__ __forceinline__ u64 ordered(double x) {
   const u64 u = __double_as_longlong(x + 0.0);
   return u >> 63 ? ~u : u | (1ull << 63);
+}
+
+__device__ __forceinline__ double unordered(u64 u) {
+  return __longlong_as_double(u >> 63 ? u & ~(1ull << 63) : ~u);
 }
 
 // A hypothesis that nothing can continue: no (or NaN) score.
@@ -115,88 +121,81 @@ __device__ __forceinline__ float exp_far(float d) {
   return y;
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack(const uint4& r, float* x) {
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const unsigned short u = (unsigned short)(h ? w[i] >> 16 : w[i]);
-        T v;
-        memcpy(&v, &u, 2);
-        x[2 * i + h] = cv3p::to_f32<T>(v);
-      }
-  }
-}
+// The CTA's shared memory for a task.
+struct Scratch {
+  u64 held[BW][64];  // candidates on their way into a warp's list
+  u64 lists[BW][32];
+  double ss[BW];
+  float ms[BW];
+  uint32_t tops[TILES_MOST];  // ordered maxima of the tiles (stop ids left out where they are none)
+  uint32_t bar;
+};
 
-// One task by the whole CTA.  Rows need not begin on 16-byte boundaries: a row is taken as the
-// 16-byte blocks that hold at least one of its logits, and what else they hold is masked.
-// `bar` (shared): the best K-th logit of any warp so far; nothing below it can be among the K best.
+// One task by the whole CTA.  A lane takes every 32nd logit of a tile, so rows may begin anywhere and
+// alike rows give the same bits wherever they lie; nothing depends on the warps' timing either.
 // The result is in warp 0: list, and in every lane m and s.
 template <typename T>
-__device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, u64 (&lists)[BW][32], float (&ms)[BW],
-                     double (&ss)[BW], uint32_t& bar, u64& list, float& m, double& s) {
-  constexpr int E = 16 / sizeof(T), J = 16 / E;  // logits of a block; blocks of a lane's step
+__device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh, u64& list, float& m, double& s) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, K = a.beams;
-  const T* x0 = static_cast<const T*>(a.logits) + row * a.ld;
-  const int off = (int)(((uintptr_t)x0 & 15) / sizeof(T));
-  const uint4* blocks = reinterpret_cast<const uint4*>(x0 - off);
-  const int64_t nb = (a.vocab + off + E - 1) / E;
+  const T* logits = static_cast<const T*>(a.logits) + row * a.ld;
+  const int begin = (int)(chunk * a.tiles * TILE);
+  const int tiles = (int)((min((chunk + 1) * a.tiles * TILE, a.vocab) - begin + TILE - 1) / TILE);
   const bool early = a.min_len && a.counts[row] < a.min_len[row / K] && a.stop_lo < a.stop_hi;
-  __syncthreads();  // (the last task's shared memory is done with)
-  if (threadIdx.x == 0) bar = 0;
-  __syncthreads();
-  list = 0;
-  u64 last = 0;  // the list's K-th
-  bool started = false;
-  m = -INFINITY;
-  s = 0.0;
-  const int64_t end = min((chunk + 1) * a.tiles * (TILE / E), nb);
-  for (int64_t i0 = chunk * a.tiles * (TILE / E) + warp * (TILE / E); i0 < end; i0 += BW * (TILE / E)) {
-    uint4 raw[J];
+  float x[16];
+  int v0 = 0;  // token of the lane's first logit; the others follow in steps of 32
+  auto inside = [&](int e) -> bool { return v0 + e * 32 < a.vocab; };
+  auto stopped = [&](int e) -> bool { return v0 + e * 32 >= a.stop_lo && v0 + e * 32 < a.stop_hi; };
+  auto load = [&](int tile) {
+    v0 = begin + tile * TILE + lane;
+    const T* p = logits + v0;
+    if (v0 - lane + TILE <= a.vocab) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int64_t i = i0 + j * 32 + lane;
-      raw[j] = make_uint4(0u, 0u, 0u, 0u);
-      if (i < nb)
-        asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(raw[j].x), "=r"(raw[j].y), "=r"(raw[j].z), "=r"(raw[j].w) : "l"(blocks + i));
+      for (int e = 0; e < 16; ++e) x[e] = cv3p::to_f32<T>(p[e * 32]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = inside(e) ? cv3p::to_f32<T>(p[e * 32]) : -INFINITY;
     }
-    float x[16];
+  };
+  auto no_nan = [&]() {  // a NaN logit is no term, and as good as -inf
 #pragma unroll
-    for (int j = 0; j < J; ++j) unpack<T>(raw[j], x + j * E);
-    const int64_t v0 = i0 * E - off;  // token of the step's first logit
-    auto token = [&](int e) -> int64_t { return v0 + (int64_t)((e / E) * 32 + lane) * E + e % E; };
-    unsigned valid = 0xFFFFu;
-    if (v0 < 0 || v0 + TILE > a.vocab) {
-      valid = 0;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const bool in = token(e) >= 0 && token(e) < a.vocab;
-        valid |= (in ? 1u : 0u) << e;
-        x[e] = in ? x[e] : -INFINITY;
-      }
-    }
-    float top = -INFINITY;  // (fmaxf passes over NaN)
+    for (int e = 0; e < 16; ++e) x[e] = fmaxf(x[e], -INFINITY);
+  };
+  auto maximum = [&]() -> float {  // (fmaxf passes over NaN)
+    float top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
-    auto no_nan = [&]() {  // a NaN logit is no candidate and no term
+    return warp_max(top);
+  };
+
+  // first reading: the sum of exp against a running maximum that begins with the first BW tiles', and
+  // the tiles' maxima
+  float wtop = -INFINITY;
+  if (warp < tiles) {
+    load(warp);
+    wtop = maximum();
+  }
+  __syncthreads();  // (the last task's shared memory is done with)
+  if (lane == 0) sh.ms[warp] = wtop;
+  __syncthreads();
+  m = -INFINITY;
+  s = 0.0;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = fmaxf(x[e], -INFINITY);
-    };
-    // the sum of exp
-    const float wtop = warp_max(top);
+  for (int w = 0; w < BW; ++w) m = fmaxf(m, sh.ms[w]);
+  for (int tile = warp; tile < tiles;) {
     if (wtop > m) {
-      s *= m > -INFINITY ? exp((double)m - (double)wtop) : 0.0;
+      if (s != 0.0) s *= exp((double)m - (double)wtop);
       m = wtop;
     }
+    float allowed = wtop;
+    if (early && v0 - lane < a.stop_hi && v0 - lane + TILE > a.stop_lo) {
+      allowed = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) allowed = stopped(e) ? allowed : fmaxf(allowed, x[e]);
+      allowed = warp_max(allowed);
+    }
+    if (lane == 0) sh.tops[tile] = ordered(allowed);
     if (m > -INFINITY) {
-      const bool close = __any_sync(0xffffffffu, top >= m - NEAR);
+      const bool close = wtop >= m - NEAR;
       unsigned near = 0;
       if (close) {
 #pragma unroll
@@ -230,81 +229,84 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, u64 (&lists)
       }
       s += (double)r;
     }
-    // candidates
-    if (early) {
-      top = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if (token(e) >= a.stop_lo && token(e) < a.stop_hi) x[e] = -INFINITY;
-        top = fmaxf(top, x[e]);
-      }
+    tile += BW;
+    if (tile < tiles) {
+      load(tile);
+      wtop = maximum();
     }
-    const uint32_t others = *(volatile uint32_t*)&bar;
-    const uint32_t last_x = (uint32_t)(last >> 32);
-    if (last != 0 && !__any_sync(0xffffffffu, ordered(top) > last_x && ordered(top) >= others)) continue;
-    no_nan();
-    u64 key;
-    int place;
-    auto best = [&]() {  // the lane's best of what is left
-      float bx = 0.f;
-      place = -1;
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if ((valid >> e & 1u) && (place < 0 || x[e] > bx)) {
-          bx = x[e];
-          place = e;
-        }
-      key = place < 0 ? 0ull : (u64)ordered(bx) << 32 | (uint32_t)~(uint32_t)token(place);
-    };
-    best();
-    if (!started) {  // the lanes' best ones, sorted, bound the rest from below
-      started = true;
-      list = sorted(key);
-      if (lane >= K) list = 0;
-      last = from_lane(list, K - 1);
-      if (key != 0 && key >= last) {
-        valid &= ~(1u << place);
-        best();
-      }
-    }
-    for (;;) {
-      const unsigned wins = __ballot_sync(0xffffffffu, key > last && (uint32_t)(key >> 32) >= others);
-      if (!wins) break;
-      const int src = __ffs(wins) - 1;
-      const u64 k = from_lane(key, src);
-      const int at = __popc(__ballot_sync(0xffffffffu, list > k));
-      const u64 up = __shfl_up_sync(0xffffffffu, list, 1);
-      list = lane < at ? list : lane == at ? k : up;
-      if (lane >= K) list = 0;
-      last = from_lane(list, K - 1);
-      if (lane == src) {
-        valid &= ~(1u << place);
-        best();
-      }
-    }
-    if (lane == 0 && last != 0 && (uint32_t)(last >> 32) > others) atomicMax(&bar, (uint32_t)(last >> 32));
   }
+  __syncthreads();
+
+  // the bar: the K-th largest of the tiles' maxima (none where there are fewer tiles)
+  if (warp == 0) {
+    u64 best = 0;
+    for (int i = 0; i < tiles; i += 32) {
+      const u64 key = i + lane < tiles ? (u64)sh.tops[i + lane] : 0ull;
+      if (__any_sync(0xffffffffu, key > from_lane(best, K - 1))) best = merged(best, sorted(key));
+    }
+    const uint32_t bar = (uint32_t)from_lane(best, K - 1);
+    if (lane == 0) sh.bar = bar;
+  }
+  __syncthreads();
+
+  // second reading: what reaches the bar, merged into the warp's list 32 at a time
+  const uint32_t bar = sh.bar;
+  const float least = bar ? unordered(bar) : -INFINITY;
+  u64* held = sh.held[warp];
+  int count = 0, turn = 0;
+  list = 0;
+  auto flush = [&]() {
+    __syncwarp();
+    const u64 key = lane < count ? held[lane] : 0ull, rest = lane + 32 < count ? held[lane + 32] : 0ull;
+    __syncwarp();
+    held[lane] = rest;
+    count = max(count - 32, 0);
+    list = merged(list, sorted(key));
+    if (lane >= K) list = 0;
+  };
+  for (int t0 = 0; t0 < tiles; t0 += 32) {
+    unsigned reach = __ballot_sync(0xffffffffu, t0 + lane < tiles && sh.tops[t0 + lane] >= bar);
+    for (; reach; reach &= reach - 1) {
+      if (turn++ % BW != warp) continue;
+      load(t0 + __ffs(reach) - 1);
+      no_nan();
+      unsigned mine = 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mine |= (x[e] >= least && inside(e) ? 1u : 0u) << e;
+      for (unsigned left = __reduce_or_sync(0xffffffffu, mine); left; left &= left - 1) {
+        const int e = __ffs(left) - 1;
+        float y = 0.f;
+#pragma unroll
+        for (int f = 0; f < 16; ++f) y = f == e ? x[f] : y;
+        if (early && stopped(e)) y = -INFINITY;
+        const u64 key = (u64)ordered(y) << 32 | (uint32_t)~(uint32_t)(v0 + e * 32);
+        const u64 last = from_lane(list, K - 1);  // (by all lanes: not within a condition)
+        const bool pass = (mine >> e & 1u) && y >= least && key > last;
+        const unsigned who = __ballot_sync(0xffffffffu, pass);
+        if (pass) held[count + __popc(who & ((1u << lane) - 1u))] = key;
+        count += __popc(who);
+        if (count >= 32) flush();
+      }
+    }
+  }
+  if (count) flush();
   s = warp_sum_d(s);
-  lists[warp][lane] = list;
-  if (lane == 0) { ms[warp] = m; ss[warp] = s; }
+  sh.lists[warp][lane] = list;
+  if (lane == 0) { sh.ms[warp] = m; sh.ss[warp] = s; }
   __syncthreads();
 #pragma unroll
   for (int w = BW / 2; w > 0; w >>= 1) {
     if (warp < w) {
-      list = merged(list, lists[warp + w][lane]);
+      list = merged(list, sh.lists[warp + w][lane]);
       if (lane >= K) list = 0;
-      lists[warp][lane] = list;
+      sh.lists[warp][lane] = list;
     }
     __syncthreads();
   }
   if (warp == 0) {
-    m = -INFINITY;
-    s = 0.0;
-#pragma unroll
-    for (int w = 0; w < BW; ++w) m = fmaxf(m, ms[w]);
-#pragma unroll
-    for (int w = 0; w < BW; ++w)
-      if (ms[w] > -INFINITY) s += ss[w] * (ms[w] == m ? 1.0 : exp((double)ms[w] - (double)m));
+    const float mine = lane < BW ? sh.ms[lane] : -INFINITY;
+    m = warp_max(mine);
+    s = warp_sum_d(mine == -INFINITY ? 0.0 : sh.ss[lane] * (mine == m ? 1.0 : exp((double)mine - (double)m)));
   }
 }
 
@@ -320,7 +322,7 @@ template <typename T>
 __device__ void choose(const BeamArgs& a, int64_t g, const char* work) {
   __shared__ double lsum[CV3_MAX_BEAMS], base[CV3_MAX_BEAMS], norm[CV3_MAX_BEAMS];
   __shared__ float tops[CV3_MAX_BEAMS];
-  __shared__ int fins[CV3_MAX_BEAMS];
+  __shared__ int fins[CV3_MAX_BEAMS], lengths[CV3_MAX_BEAMS];
   __shared__ Cand lists[BW][32];
   const int K = a.beams, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t tb = task_bytes(K);
@@ -341,12 +343,13 @@ __device__ void choose(const BeamArgs& a, int64_t g, const char* work) {
     }
     if (lane == 0) {
       const float sc = a.scores[row];
-      const int n = max(a.counts[row], 0) + (fin ? 0 : 1);
+      const int held = a.counts[row], n = max(held, 0) + (fin ? 0 : 1);
       tops[k] = m;
       lsum[k] = log(s);
       base[k] = dead(sc) ? -INFINITY : (double)sc;
       norm[k] = a.alpha == 0.0 ? 1.0 : pow((double)max(n, 1), a.alpha);
       fins[k] = fin ? 2 : skip;
+      lengths[k] = held + (fin ? 0 : 1);
     }
   }
   __syncthreads();
@@ -386,29 +389,22 @@ __device__ void choose(const BeamArgs& a, int64_t g, const char* work) {
   if (warp || lane >= K) return;
   const int64_t id = (int64_t)~list.tie;
   const int k = (int)(id / a.vocab);
-  const int64_t v = id - (int64_t)k * a.vocab, row = g * K + k, to = g * K + lane;
+  const int64_t v = id - (int64_t)k * a.vocab, to = g * K + lane;
   const bool fin = fins[k] == 2;
-  double cum = -(double)INFINITY;
-  if (list.key > ordered(-(double)INFINITY))
-    cum = fin ? base[k]
-              : continued(base[k], fmaxf(cv3p::to_f32<T>(static_cast<const T*>(a.logits)[row * a.ld + v]), -INFINITY), tops[k],
-                          lsum[k]);
-  const int count = a.counts[row] + (fin ? 0 : 1);
-  __syncwarp(0xffffffffu >> (32 - K));  // the outputs may be the inputs' own buffers
+  // the key times the length's power is the score again (to the last bits of 64); the outputs may be
+  // the inputs' own buffers, of which nothing is read any more
+  const double cum = list.key > ordered(-(double)INFINITY) ? (fin ? base[k] : unordered(list.key) * norm[k]) : -(double)INFINITY;
   a.tokens[to] = fin ? 0 : v;
   a.parents[to] = k;
   a.scores_out[to] = (float)cum;
-  a.counts_out[to] = count;
+  a.counts_out[to] = lengths[k];
   a.done_out[to] = fin || (v >= a.stop_lo && v < a.stop_hi) ? 1 : 0;
 }
 
 // two launches: a CTA per task, then one per group
 template <typename T>
 __global__ void __launch_bounds__(BT, 4) beam_scan_kernel(const BeamArgs a) {
-  __shared__ u64 lists[BW][32];
-  __shared__ float ms[BW];
-  __shared__ double ss[BW];
-  __shared__ uint32_t bar;
+  __shared__ Scratch sh;
   dep_wait();
   dep_release();
   const int64_t row = blockIdx.y;
@@ -416,7 +412,7 @@ __global__ void __launch_bounds__(BT, 4) beam_scan_kernel(const BeamArgs a) {
   u64 list;
   float m;
   double s;
-  scan<T>(a, row, blockIdx.x, lists, ms, ss, bar, list, m, s);
+  scan<T>(a, row, blockIdx.x, sh, list, m, s);
   if (threadIdx.x < 32) {
     char* w = a.work + (row * a.chunks + blockIdx.x) * task_bytes(a.beams);
     if (threadIdx.x < a.beams) reinterpret_cast<u64*>(w + 16)[threadIdx.x] = list;
@@ -443,10 +439,7 @@ __device__ __forceinline__ void put8(uint32_t at, u64 x) {
 template <typename T>
 __global__ void __launch_bounds__(BT) beam_cluster_kernel(const BeamArgs a, int cluster) {
   extern __shared__ __align__(16) char work[];
-  __shared__ u64 lists[BW][32];
-  __shared__ float ms[BW];
-  __shared__ double ss[BW];
-  __shared__ uint32_t bar;
+  __shared__ Scratch sh;
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   dep_wait();
   dep_release();
@@ -461,7 +454,7 @@ __global__ void __launch_bounds__(BT) beam_cluster_kernel(const BeamArgs a, int 
     u64 list;
     float m;
     double s;
-    scan<T>(a, row, i % a.chunks, lists, ms, ss, bar, list, m, s);
+    scan<T>(a, row, i % a.chunks, sh, list, m, s);
     if (threadIdx.x < 32) {
       const uint32_t at = first + (uint32_t)(i * task_bytes(a.beams));
       if (threadIdx.x < a.beams) put8(at + 16 + threadIdx.x * 8, list);
@@ -484,8 +477,9 @@ constexpr int64_t CLUSTER = 8, CLUSTER_TILES = 16;  // (at most 32 tasks: 9 KB o
 
 Plan plan_of(int64_t groups, int64_t beams, int64_t vocab) {
   Plan p = {};
-  const int64_t row = (vocab + 7 + TILE - 1) / TILE;  // tiles of a row, its first block's share included
+  const int64_t row = (vocab + TILE - 1) / TILE;  // tiles of a row
   auto cut = [&](int64_t chunks) {
+    chunks = std::max(chunks, (row + TILES_MOST - 1) / TILES_MOST);
     p.tiles = (std::max<int64_t>(1, (row + chunks - 1) / chunks) + BW - 1) / BW * BW;
     p.chunks = (row + p.tiles - 1) / p.tiles;
   };
@@ -503,6 +497,8 @@ Plan plan_of(int64_t groups, int64_t beams, int64_t vocab) {
 template <typename T>
 int launch(const BeamArgs& a, const Plan& plan, int64_t groups, cudaStream_t st) {
   if (plan.cluster) {
+    int rc = cv3::allow_smem((const void*)beam_cluster_kernel<T>, (int)plan.bytes);
+    if (rc) return rc;
     return cv3::check_launch("beam_select",
                              cv3p::launch_cluster(beam_cluster_kernel<T>, dim3((unsigned)(groups * plan.cluster)), dim3(BT),
                                                   (size_t)plan.bytes, (unsigned)plan.cluster, st, a, (int)plan.cluster));
@@ -523,7 +519,7 @@ extern "C" int64_t cv3_beam_workspace(int64_t groups, int64_t beams, int64_t voc
 
 extern "C" int cv3_beam_select(const cv3_beam_params* p, void* stream) {
   CV3_REQUIRE(p && p->size == (int64_t)sizeof(*p), CV3_ERR_VALUE, "beam_select: bad parameter block");
-  CV3_REQUIRE(p->groups >= 0 && p->vocab > 0 && p->vocab <= INT32_MAX && p->ld >= p->vocab && p->stop_lo <= p->stop_hi,
+  CV3_REQUIRE(p->groups >= 0 && p->vocab > 0 && p->vocab <= 1 << 30 && p->ld >= p->vocab && p->stop_lo <= p->stop_hi,
               CV3_ERR_VALUE, "beam_select: bad shape");
   CV3_REQUIRE(p->beams > 0 && p->beams <= CV3_MAX_BEAMS, CV3_ERR_UNSUPPORTED, "beam_select: %lld beams (1 to %d)",
               (long long)p->beams, CV3_MAX_BEAMS);
