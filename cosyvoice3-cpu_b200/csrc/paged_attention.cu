@@ -7,9 +7,8 @@
 // it.  Three choices follow.
 //
 // 1. Work is cut evenly, whatever the lengths.  A pair (request, group of up to 8 heads of a kv head)
-//    has ceil(keys / TK) tiles; all pairs' tiles in order form one line, of which each of the grid's
-//    CTAs takes an equal piece (found from the lengths on the device, so a captured launch follows
-//    them).  A CTA meets at most two pairs that it does not hold whole -- the one that began before
+//    has ceil(keys / TK) tiles; all pairs' tiles in order form one line, of which the grid's CTAs take
+//    equal pieces (found from the lengths on the device, so a captured launch follows them).  A CTA meets at most two pairs that it does not hold whole -- the one that began before
 //    its piece and the one that goes on behind it -- and leaves their partial results (running
 //    maximum, sum, unnormalised output) in two slots; a second launch joins the slots of every pair
 //    that was cut, in CTA order, so the result does not depend on timing.  Short caches, whose cost
@@ -23,6 +22,8 @@
 //    most 8 heads, so rows 0..7 hold the upper tf32 part of q (then of p) and rows 8..15 the lower
 //    part: 22 bits of both at no cost.  The matrix pipe truncates when it adds, so only one tile's
 //    p.v is summed there; tiles are added in fp32 registers, the softmax's rescaling on the way.
+//    Queries of the cache's own 16-bit type need less: 16-bit products, exact for q.k, and p in two
+//    16-bit parts, whose 2^-16 is far below the result's rounding.
 #include <algorithm>
 #include <type_traits>
 
@@ -63,13 +64,45 @@ constexpr float TINY = 1e-37f;         // stands for a lower part of 0, so that 
 // keeps enough loads in flight.
 template <typename KT, int D>
 constexpr int keys_per_step() {
-  return D * (int)sizeof(KT) <= 128 ? 32 : D * (int)sizeof(KT) <= 256 ? 16 : 8;
+  return D * (int)sizeof(KT) <= 64 ? 32 : D * (int)sizeof(KT) <= 256 ? 16 : 8;
 }
 
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename KT>
+__device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<KT, __nv_bfloat16>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// two probabilities as 16-bit parts: the upper ones, and what these leave (never 0, see TINY; 6e-8, the
+// smallest fp16, is below the arithmetic's own rounding)
+template <typename KT>
+__device__ __forceinline__ void split_16(float x, float y, uint32_t& hi, uint32_t& lo) {
+  if constexpr (std::is_same<KT, __nv_bfloat16>::value) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    const float rx = x - __uint_as_float(hi << 16), ry = y - __uint_as_float(hi & 0xFFFF0000u);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(rx == 0.f ? TINY : rx, ry == 0.f ? TINY : ry);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+  } else {
+    const __half2 h = __floats2half2_rn(x, y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    const float2 back = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - back.x, y - back.y);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+    lo |= (lo & 0x7FFFu ? 0u : 1u) | (lo & 0x7FFF0000u ? 0u : 0x10000u);
+  }
 }
 
 __device__ __forceinline__ uint32_t tf32_hi(uint32_t x) { return x & 0xFFFFE000u; }
@@ -85,7 +118,19 @@ struct Raw;
 template <>
 struct Raw<16> { uint32_t r[4]; };
 template <>
+struct Raw<32> { uint32_t r[8]; };
+template <>
 struct Raw<8> { uint32_t r[2]; };
+
+__device__ __forceinline__ void fetch(Raw<32>& x, const void* p, bool ok) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x.r[i] = 0u;
+  if (ok)
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(x.r[0]), "=r"(x.r[1]), "=r"(x.r[2]), "=r"(x.r[3]), "=r"(x.r[4]), "=r"(x.r[5]), "=r"(x.r[6]),
+                   "=r"(x.r[7])
+                 : "l"(p));
+}
 
 __device__ __forceinline__ void fetch(Raw<16>& x, const void* p, bool ok) {
   x.r[0] = x.r[1] = x.r[2] = x.r[3] = 0u;
@@ -111,11 +156,11 @@ __device__ __forceinline__ uint32_t element(const Raw<B>& x, int e) {
   }
 }
 
-// what the upper tf32 part leaves of x (0 of an infinity)
+// what the upper tf32 part leaves of x (NaN of an infinity: sums of such products count as 0)
 __device__ __forceinline__ uint32_t tf32_rest(uint32_t x) {
-  const float f = __uint_as_float(x), r = f - __uint_as_float(tf32_hi(x));
-  return fabsf(f) == INFINITY ? 0u : __float_as_uint(r);
+  return __float_as_uint(__uint_as_float(x) - __uint_as_float(tf32_hi(x)));
 }
+__device__ __forceinline__ float or_zero(float x) { return x == x ? x : 0.f; }
 
 __device__ __forceinline__ int page_index(const AttnArgs& a, int key) {
   return (int)(((uint64_t)(uint32_t)key * a.ps_mul) >> a.ps_shift);
@@ -128,18 +173,22 @@ __device__ __forceinline__ void visible(const AttnArgs& a, int b, int& lo, int& 
 }
 
 // UNI: page_size is a multiple of 16, so 16 (or 8) keys from a multiple of 16 share a page.
+// H16: the queries have the cache's 16-bit type.
 // CL: clusters of gridDim / pairs CTAs, one per pair, instead of even pieces of the line.
-template <typename KT, int D, bool UNI, bool CL>
+template <typename KT, int D, bool UNI, bool H16, bool CL>
 __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnArgs a) {
   constexpr int KI = keys_per_step<KT, D>(), NT = KI / 8, TK = NW * KI;
   constexpr bool WIDE = sizeof(KT) == 4;          // keys and values need a lower part
-  constexpr int KE = 16 / sizeof(KT);             // elements of a key piece; 4 lanes cover 4 * KE dimensions
+  // a key piece: 32 bytes where 4 lanes' pieces fill whole rows (a 128-byte line per key and load), else 16
+  constexpr int KB = D * (int)sizeof(KT) % 128 == 0 ? 32 : 16;
+  constexpr int KE = KB / (int)sizeof(KT);        // its elements; 4 lanes cover 4 * KE dimensions
   constexpr int KC = D / (4 * KE);
   constexpr int VE = sizeof(KT) == 2 && D % 64 == 0 ? 8 : 4;  // of a value piece; 8 lanes cover 8 * VE
   constexpr int VC = D / (8 * VE);
   constexpr int VB = VE * (int)sizeof(KT);
   constexpr int GK = UNI ? (KI >= 16 ? KI / 16 : 1) : NT;  // page lookups of a step: per 16 keys, or per 8 and row
-  __shared__ __align__(16) uint32_t sq[D / 8][32][4];      // q as product operands, lower parts in rows 8..15
+  constexpr int QS = H16 ? D / 16 : D / 8, QW = H16 ? 2 : 4;  // steps of q.k, words of a lane's operand
+  __shared__ __align__(16) uint32_t sq[QS][32][QW];  // q as product operands; H16: rows 0..7, else lower parts in 8..15
   __shared__ float so[NW][HT][D];
   __shared__ float sm[NW][HT], sl[NW][HT];
   dep_wait();
@@ -151,20 +200,28 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
   // tiles [t0, t1) of a pair: the warps' maxima, sums and unnormalised outputs to shared memory
   auto attend = [&](int b, int pair, int lo, int hi, int g, int h0, int nh, int t0, int t1) {
     __syncthreads();  // the last pair's shared memory is done with
-    for (int i = tid; i < D / 8 * 32; i += NW * 32) {
+    for (int i = tid; i < QS * 32; i += NW * 32) {
       const int s = i >> 5, ln = i & 31, row = ln >> 2;
-      const int d = s / (KE / 2) * 4 * KE + (ln & 3) * KE + s % (KE / 2) * 2;
-      uint32_t v[4] = {0u, 0u, 0u, 0u};
-      if (row < nh) {
+      const int64_t at = b * a.qsb + (h0 + row) * a.qsh;
+      if constexpr (H16) {  // four dimensions of a key piece per step, two in a word
+        const int d = s / (KE / 4) * 4 * KE + (ln & 3) * KE + s % (KE / 4) * 4;
+        const unsigned short* q = static_cast<const unsigned short*>(a.q) + at + d;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float x = cv3p::load_any(a.q, a.q_type, b * a.qsb + (h0 + row) * a.qsh + d + e) * (a.scale * LOG2E);
-          const uint32_t r = tf32_rest(__float_as_uint(x));
-          v[2 * e] = tf32_hi(__float_as_uint(x));
-          v[2 * e + 1] = (r & 0x7FFFFFFFu) ? r : __float_as_uint(copysignf(TINY, x));
+        for (int e = 0; e < 2; ++e) sq[s][ln][e] = row < nh ? q[2 * e] | (uint32_t)q[2 * e + 1] << 16 : 0u;
+      } else {
+        const int d = s / (KE / 2) * 4 * KE + (ln & 3) * KE + s % (KE / 2) * 2;
+        uint32_t v[4] = {0u, 0u, 0u, 0u};
+        if (row < nh) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = cv3p::load_any(a.q, a.q_type, at + d + e) * (a.scale * LOG2E);
+            const uint32_t r = __float_as_uint(or_zero(__uint_as_float(tf32_rest(__float_as_uint(x)))));
+            v[2 * e] = tf32_hi(__float_as_uint(x));
+            v[2 * e + 1] = (r & 0x7FFFFFFFu) ? r : __float_as_uint(copysignf(TINY, x));
+          }
         }
+        *reinterpret_cast<uint4*>(&sq[s][ln][0]) = make_uint4(v[0], v[1], v[2], v[3]);
       }
-      *reinterpret_cast<uint4*>(&sq[s][ln][0]) = make_uint4(v[0], v[1], v[2], v[3]);
     }
     __syncthreads();
 
@@ -186,7 +243,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
       return ok ? p : -1;
     };
 
-    Raw<16> kr[NT][KC];
+    Raw<KB> kr[NT][KC];
     Raw<VB> vr[NT][2][VC];
     const int first = (lo & -KI) + t0 * TK + warp * KI, end = min(hi, (lo & -KI) + t1 * TK);
     // pages of a step: UNI: of its 16-key groups (any visible key of one names it); else of the rows
@@ -254,19 +311,32 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s0[i][e] = s1[i][e] = 0.f;
+      if constexpr (H16) {
 #pragma unroll
-      for (int s = 0; s < D / 8; ++s) {
-        const uint4 q4 = *reinterpret_cast<const uint4*>(&sq[s][lane][0]);
-        const uint32_t qa[4] = {q4.x, q4.y, q4.z, q4.w};
+        for (int s = 0; s < QS; ++s) {
+          const uint2 q2 = *reinterpret_cast<const uint2*>(&sq[s][lane][0]);
+          const uint32_t qa[4] = {q2.x, 0u, q2.y, 0u};
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const uint32_t b0 = element<KT>(kr[i][s / (KE / 2)], s % (KE / 2) * 2);
-          const uint32_t b1 = element<KT>(kr[i][s / (KE / 2)], s % (KE / 2) * 2 + 1);
-          if constexpr (WIDE) {
-            mma_tf32(s0[i], qa, tf32_hi(b0), tf32_hi(b1));
-            mma_tf32(s1[i], qa, tf32_rest(b0), tf32_rest(b1));
-          } else {
-            mma_tf32(s & 1 ? s1[i] : s0[i], qa, b0, b1);
+          for (int i = 0; i < NT; ++i) {
+            const auto& piece = kr[i][s / (KE / 4)];
+            mma_16<KT>(s & 1 ? s1[i] : s0[i], qa, piece.r[s % (KE / 4) * 2], piece.r[s % (KE / 4) * 2 + 1]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < D / 8; ++s) {
+          const uint4 q4 = *reinterpret_cast<const uint4*>(&sq[s][lane][0]);
+          const uint32_t qa[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            const uint32_t b0 = element<KT>(kr[i][s / (KE / 2)], s % (KE / 2) * 2);
+            const uint32_t b1 = element<KT>(kr[i][s / (KE / 2)], s % (KE / 2) * 2 + 1);
+            if constexpr (WIDE) {
+              mma_tf32(s0[i], qa, tf32_hi(b0), tf32_hi(b1));
+              mma_tf32(s1[i], qa, tf32_rest(b0), tf32_rest(b1));
+            } else {
+              mma_tf32(s & 1 ? s1[i] : s0[i], qa, b0, b1);
+            }
           }
         }
       }
@@ -276,7 +346,9 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float x = (s0[i][r] + s1[i][r]) + (s0[i][2 + r] + s1[i][2 + r]);
+          const float rest = s1[i][r] + s1[i][2 + r];
+          const float x = H16 ? (s0[i][r] + s1[i][r]) * (a.scale * LOG2E)
+                              : (s0[i][r] + s0[i][2 + r]) + (WIDE ? or_zero(rest) : rest);
           s0[i][r] = seen[i][r] ? x : -INFINITY;
           top = fmaxf(top, s0[i][r]);
         }
@@ -286,31 +358,61 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
       const float fade = exp2_fast(m - ref);
       m = top;
       l *= fade;
-      uint32_t p[NT][4];
+      float pr[NT][2];
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float x = exp2_fast(s0[i][r] - ref);
-          l += x;
-          p[i][2 * r] = tf32_hi(__float_as_uint(x));
-          p[i][2 * r + 1] = __float_as_uint(fmaxf(x - __uint_as_float(p[i][2 * r]), TINY));
+          pr[i][r] = exp2_fast(s0[i][r] - ref);
+          l += pr[i][r];
         }
+      if constexpr (H16) {
+        uint32_t p[NT / 2][4];
 #pragma unroll
-      for (int j = 0; j < D / 8; ++j) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < NT; ++i) split_16<KT>(pr[i][0], pr[i][1], p[i / 2][i % 2 * 2], p[i / 2][i % 2 * 2 + 1]);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const uint32_t b0 = element<KT>(vr[i][0][j / VE], j % VE), b1 = element<KT>(vr[i][1][j / VE], j % VE);
-          if constexpr (WIDE) {
-            mma_tf32(acc, p[i], tf32_hi(b0), tf32_hi(b1));
-            mma_tf32(acc, p[i], tf32_rest(b0), tf32_rest(b1));
-          } else {
-            mma_tf32(acc, p[i], b0, b1);
+        for (int j = 0; j < D / 8; ++j) {
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < NT; i += 2) {
+            const int x = j / VE, w = j % VE / 2;
+            const uint32_t half = j % 2 ? 0x7632u : 0x5410u;  // a column's values of two keys in a word
+            mma_16<KT>(acc, p[i / 2], __byte_perm(vr[i][0][x].r[w], vr[i][1][x].r[w], half),
+                       __byte_perm(vr[i + 1][0][x].r[w], vr[i + 1][1][x].r[w], half));
           }
+          o[j][0] = fmaf(o[j][0], fade, acc[0] + acc[2]);
+          o[j][1] = fmaf(o[j][1], fade, acc[1] + acc[3]);
         }
-        o[j][0] = fmaf(o[j][0], fade, acc[0] + acc[2]);
-        o[j][1] = fmaf(o[j][1], fade, acc[1] + acc[3]);
+      } else {
+        uint32_t p[NT][4];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            p[i][2 * r] = tf32_hi(__float_as_uint(pr[i][r]));
+            p[i][2 * r + 1] = __float_as_uint(fmaxf(pr[i][r] - __uint_as_float(p[i][2 * r]), TINY));
+          }
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+          float acc[4] = {0.f, 0.f, 0.f, 0.f}, low[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            const uint32_t b0 = element<KT>(vr[i][0][j / VE], j % VE), b1 = element<KT>(vr[i][1][j / VE], j % VE);
+            if constexpr (WIDE) {
+              mma_tf32(acc, p[i], tf32_hi(b0), tf32_hi(b1));
+              mma_tf32(low, p[i], tf32_rest(b0), tf32_rest(b1));
+            } else {
+              mma_tf32(acc, p[i], b0, b1);
+            }
+          }
+          float y0 = acc[0] + acc[2], y1 = acc[1] + acc[3];
+          if constexpr (WIDE) {
+            y0 += or_zero(low[0] + low[2]);
+            y1 += or_zero(low[1] + low[3]);
+          }
+          o[j][0] = fmaf(o[j][0], fade, y0);
+          o[j][1] = fmaf(o[j][1], fade, y1);
+        }
       }
     }
 
@@ -404,7 +506,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
     }
     cv3p::cluster_sync();  // no CTA leaves while another reads its shared memory
     return;
-  }
+  } else {
 
   // requests without keys: zeros, nothing to join
   for (int b = c; b < a.batch; b += gridDim.x) {
@@ -419,10 +521,10 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) W += __shfl_xor_sync(0xffffffffu, W, o);
   W *= per;
-  const int64_t C = min((int64_t)gridDim.x, W);  // every CTA that works has a tile
-  if (c >= C) return;
-  int64_t u = W * c / C;
-  const int64_t u_end = W * (c + 1) / C;
+  const int64_t share = (W + gridDim.x - 1) / gridDim.x;
+  int64_t u = c * share;
+  const int64_t u_end = min(u + share, W);
+  if (u >= u_end) return;
   int b = 0;
   int64_t before = 0;  // tiles of the requests before b (one pair each)
   for (int b0 = 0;; b0 += 32) {
@@ -471,10 +573,11 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
         if (e == 0) { a.stat[at * 2] = M; a.stat[at * 2 + 1] = L; }
       }
     }
-    if (t0 == 0 && tid == 0) {  // who holds the pair: CTA x has the tiles from W * x / C on
-      const int last = (int)(((u0 + tiles) * C - 1) / W);
+    if (t0 == 0 && tid == 0) {  // who holds the pair: CTA x has the tiles from x * share on
+      const int last = (int)((u0 + tiles - 1) / share);
       a.cut[(int64_t)b * per + pair] = whole ? make_int2(0, 0) : make_int2(c, last - c + 1);
     }
+  }
   }
 }
 
@@ -548,19 +651,25 @@ __global__ void __launch_bounds__(NW * 32) paged_join_kernel(const AttnArgs a) {
 
 using Fn = void (*)(const AttnArgs);
 
+template <typename KT, int D, bool UNI, bool H16>
+Fn pick(bool cl) {
+  return cl ? paged_attention_kernel<KT, D, UNI, H16, true> : paged_attention_kernel<KT, D, UNI, H16, false>;
+}
+
 template <typename KT, int D>
-Fn pick(bool uni, bool cl) {
-  if (cl) return uni ? paged_attention_kernel<KT, D, true, true> : paged_attention_kernel<KT, D, false, true>;
-  return uni ? paged_attention_kernel<KT, D, true, false> : paged_attention_kernel<KT, D, false, false>;
+Fn pick(bool uni, bool h16, bool cl) {
+  if constexpr (sizeof(KT) == 2)
+    if (h16) return uni ? pick<KT, D, true, true>(cl) : pick<KT, D, false, true>(cl);
+  return uni ? pick<KT, D, true, false>(cl) : pick<KT, D, false, false>(cl);
 }
 
 template <typename KT>
-Fn pick(int64_t d, bool uni, bool cl) {
+Fn pick(int64_t d, bool uni, bool h16, bool cl) {
   switch (d) {
-    case 32: return pick<KT, 32>(uni, cl);
-    case 64: return pick<KT, 64>(uni, cl);
-    case 96: return pick<KT, 96>(uni, cl);
-    default: return pick<KT, 128>(uni, cl);
+    case 32: return pick<KT, 32>(uni, h16, cl);
+    case 64: return pick<KT, 64>(uni, h16, cl);
+    case 96: return pick<KT, 96>(uni, h16, cl);
+    default: return pick<KT, 128>(uni, h16, cl);
   }
 }
 
@@ -574,7 +683,7 @@ Fn pick_join(int64_t d, bool wide) {
 }
 
 // Keys of a CTA's tile (keys_per_step of the type and head dimension).
-int64_t tile_of(int64_t d, int64_t size) { return NW * (d * size <= 128 ? 32 : d * size <= 256 ? 16 : 8); }
+int64_t tile_of(int64_t d, int64_t size) { return NW * (d * size <= 64 ? 32 : d * size <= 256 ? 16 : 8); }
 
 struct Plan {
   int64_t pairs, grid, cluster, floats;  // cluster 0: even pieces and a join
@@ -622,10 +731,10 @@ extern "C" int cv3_paged_attention(const cv3_paged_attention_params* p, void* st
               "paged_attention: head_dim %lld (built for 32, 64, 96 and 128)", (long long)d);
   CV3_REQUIRE(cv3p::type_ok(p->q_type) && cv3p::type_ok(p->kv_type), CV3_ERR_VALUE,
               "paged_attention: unknown element type");
-  const int es = cv3p::type_size(p->kv_type), ce = 16 / es;
-  CV3_REQUIRE(cv3p::aligned16(p->k_pages) && cv3p::aligned16(p->v_pages) &&
+  const int es = cv3p::type_size(p->kv_type), ce = 32 / es;
+  CV3_REQUIRE(((uintptr_t)p->k_pages & 31) == 0 && ((uintptr_t)p->v_pages & 31) == 0 &&
                   (p->ksp | p->ksh | p->kst | p->vsp | p->vsh | p->vst) % ce == 0,
-              CV3_ERR_VALUE, "paged_attention: cache rows must start on 16-byte boundaries");
+              CV3_ERR_VALUE, "paged_attention: cache rows must start on 32-byte boundaries");
   // (a tile behind the last key must not pass 2^31 either)
   CV3_REQUIRE(p->page_size <= INT32_MAX && p->max_blocks <= INT32_MAX &&
                   p->max_blocks * p->page_size <= INT32_MAX - 4096 && p->num_pages <= INT32_MAX &&
@@ -650,9 +759,9 @@ extern "C" int cv3_paged_attention(const cv3_paged_attention_params* p, void* st
                       (group + HT - 1) / HT, (int)std::min<int64_t>(p->window, INT32_MAX), (float)p->scale, p->out,
                       p->osb, p->osh, p->lse, p->bad, stat + plan.grid * 2 * HT * 2, stat,
                       reinterpret_cast<int2*>(p->workspace)};
-  const bool uni = p->page_size % 16 == 0, cl = plan.cluster > 0;
-  const Fn fn = p->kv_type == CV3_TYPE_F32   ? pick<float>(d, uni, cl)
-                : p->kv_type == CV3_TYPE_F16 ? pick<__half>(d, uni, cl) : pick<__nv_bfloat16>(d, uni, cl);
+  const bool uni = p->page_size % 16 == 0, h16 = es == 2 && p->q_type == p->kv_type, cl = plan.cluster > 0;
+  const Fn fn = p->kv_type == CV3_TYPE_F32   ? pick<float>(d, uni, h16, cl)
+                : p->kv_type == CV3_TYPE_F16 ? pick<__half>(d, uni, h16, cl) : pick<__nv_bfloat16>(d, uni, h16, cl);
   cudaStream_t st = cv3::as_stream(stream);
   const dim3 grid((unsigned)plan.grid), block(NW * 32);
   if (cl)

@@ -462,7 +462,8 @@ int cv3_paged_append(const cv3_paged_append_params* params, void* stream);
  * GQA: query head h uses kv head h / (heads / kv_heads).  A request without tokens
  * gives zeros.  Tokens of a page number outside the pool are left out, and each such
  * table entry adds 1 to *bad (may be NULL).  lse (may be NULL) [batch][heads]: the
- * logarithm of the softmax's sum (-inf without tokens).  head_dim 32, 64, 96 or 128.
+ * logarithm of the softmax's sum (-inf without tokens).  head_dim 32, 64, 96 or 128;
+ * cache rows on 32-byte boundaries.
  * workspace: cv3_paged_attention_workspace() floats (its max_len: max_blocks *
  * page_size; 0: none is needed), nothing kept in it between calls. */
 typedef struct cv3_paged_attention_params {

@@ -176,8 +176,8 @@ def test_c_entries_refuse_before_any_device_work():
     assert attention(size=8) == V and b"parameter block" in lib.cv3_last_error()
     assert attention(dim=80) == U and b"head_dim" in lib.cv3_last_error()
     assert attention(kv=3) == V and b"not a multiple" in lib.cv3_last_error()
-    assert attention(strides=(2048, 1024, 62)) == V and b"16-byte" in lib.cv3_last_error()
-    assert attention(k=at + 4) == V
+    assert attention(strides=(2048, 1024, 62)) == V and b"32-byte" in lib.cv3_last_error()
+    assert attention(k=at + 16) == V
     assert attention(kt=5) == V and attention(ps=0) == V and attention(ld=2) == V and attention(window=-1) == V
     assert attention(cols=1 << 28, ld=1 << 28) == V and b"32-bit" in lib.cv3_last_error()
     assert attention(cols=5000, ld=5000, batch=2) == V and b"workspace" in lib.cv3_last_error()
