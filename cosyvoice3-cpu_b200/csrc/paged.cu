@@ -139,7 +139,8 @@ __device__ __forceinline__ void extend_rows(const ExtendArgs& a, int i, int n) {
   }
 }
 
-// One CTA: pages given back, sums over the requests, lengths and counts (and, fused, the rows).
+// Pages given back, sums over the requests, lengths and counts (and, fused, the rows) by one CTA.  Many
+// requests' pages are given back by a cluster of them (512 requests, a third of them done: 8 CTAs).
 constexpr int OWN = 4;  // new tokens up to which a request's thread writes its rows itself
 
 __global__ void __launch_bounds__(ET) extend_scan_kernel(const ExtendArgs a, int fused) {
@@ -153,7 +154,7 @@ __global__ void __launch_bounds__(ET) extend_scan_kernel(const ExtendArgs a, int
   int64_t have = min((int64_t)max(*a.count, 0), a.cap);
   if (a.release) {
     __shared__ int give[ET], place[ET];
-    const int warp = tid >> 5, lane = tid & 31, warps = T >> 5;
+    const int lane = tid & 31, ranks = gridDim.x, warps = ranks * (T >> 5), warp = blockIdx.x * (T >> 5) + (tid >> 5);
     int64_t carry = 0;
     for (int64_t b0 = 0; b0 < a.batch; b0 += T) {
       const int64_t b = b0 + tid;
@@ -189,6 +190,10 @@ __global__ void __launch_bounds__(ET) extend_scan_kernel(const ExtendArgs a, int
       __syncthreads();
     }
     have = min(have + carry, a.cap);
+    if (ranks > 1) {
+      cv3p::cluster_sync();
+      if (blockIdx.x) return;
+    }
   }
   Sum2 asked = {0, 0};  // pages and rows asked for by the requests before this tile
   int64_t taken = 0;    // pages of the requests that are served
@@ -465,7 +470,10 @@ extern "C" int cv3_paged_extend(const cv3_paged_extend_params* p, void* stream) 
   const int fused = p->max_tokens <= 4 * ET;
   const int64_t work = std::max(p->batch, fused ? (p->max_tokens + RV - 1) / RV : 0);
   const unsigned threads = (unsigned)std::min<int64_t>(ET, std::max<int64_t>(64, (work + 31) / 32 * 32));
-  int rc = cv3::check_launch("paged_extend", cv3::launch_dep(extend_scan_kernel, dim3(1), dim3(threads), 0, st, a, fused));
+  const bool cluster = p->release && p->batch >= 64;
+  int rc = cv3::check_launch("paged_extend",
+                             cluster ? cv3p::launch_cluster(extend_scan_kernel, dim3(8), dim3(threads), 0, 8u, st, a, fused)
+                                     : cv3::launch_dep(extend_scan_kernel, dim3(1), dim3(threads), 0, st, a, fused));
   if (rc || fused) return rc;
   const int64_t grid = (p->max_tokens + 256 * RV - 1) / (256 * RV);
   return cv3::check_launch("paged_extend_rows",
