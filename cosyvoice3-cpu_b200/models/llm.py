@@ -29,15 +29,21 @@ ENDOFPROMPT_ID = 151646
 
 
 class SamplingConfig:
-    """Sampling knobs of cv3cpu/models/llm.py:19-34 (host-side sampler)."""
+    """Sampling knobs of cv3cpu/models/llm.py:19-34 (host-side sampler).
+
+    ``beams`` > 0 (device extension): beam search with that many hypotheses instead of sampling;
+    ``length_penalty`` divides a hypothesis's score by its length to that power.  The token/text
+    ratios bound the length as in sampling, no stop id being taken below the minimum."""
 
     def __init__(self, top_p: float = 0.8, top_k: int = 25, win_size: int = 10, tau_r: float = 0.1,
                  seed: Optional[int] = None, max_token_text_ratio: float = 20.0,
-                 min_token_text_ratio: float = 2.0, strict_min_len: bool = False):
+                 min_token_text_ratio: float = 2.0, strict_min_len: bool = False, beams: int = 0,
+                 length_penalty: float = 0.0):
         self.top_p, self.top_k, self.win_size, self.tau_r = top_p, top_k, win_size, tau_r
         self.max_token_text_ratio = max_token_text_ratio
         self.min_token_text_ratio = min_token_text_ratio
         self.strict_min_len = strict_min_len
+        self.beams, self.length_penalty = int(beams), float(length_penalty)
         self.rng = np.random.default_rng(seed)
 
 
@@ -74,6 +80,7 @@ class CosyVoice3LM:
         self.endofprompt_id = int(weights.meta.get("endofprompt_id", ENDOFPROMPT_ID))
         self._engines = {}
         self._sampling_engines = {}
+        self._beam_engines = {}
 
     # -- pieces (llm.py:68-78) -------------------------------------------------
     def _speech_emb(self, ids):
@@ -120,6 +127,13 @@ class CosyVoice3LM:
         min_len = int(n_new * sampling.min_token_text_ratio)
         max_len = int(n_new * sampling.max_token_text_ratio)
         if max_len <= 0:
+            return
+        if getattr(sampling, "beams", 0) > 0:
+            toks = self.generate_beam([x], sampling.beams, max_len, min_len, sampling.length_penalty)[0][0][0]
+            for i, t in enumerate(toks):
+                yield t
+                if progress is not None:
+                    progress(i, t)
             return
         if device_sampler and 1 <= int(sampling.top_k) <= SAMPLER_MAX_TOP_K and sampling.top_p > 0:
             # graph-replayed decode steps with the device sampler: the same tokens and the
@@ -201,6 +215,46 @@ class CosyVoice3LM:
                                              "state": {"state": state[0], "inc": state[1]},
                                              "has_uint32": st["has_uint32"], "uinteger": st["uinteger"]}
         return out
+
+    # -- beam search ------------------------------------------------------------
+    def generate_beam(self, prompts, beams: int, max_len: int, min_len=0, length_penalty: float = 0.0,
+                      page_size: int = 16, cache_dtype=None, use_graph: bool = True):
+        """Beam search over every prompt embedding ``(T_b, H)``: per prompt the hypotheses best first, as
+        (tokens without the stop id, sum of log-probabilities).
+
+        Hypotheses end at a stop id (none below ``min_len`` tokens, one number or one per prompt) or at
+        ``max_len`` tokens.  Their keys and values live in pages that hypotheses share (``cache_dtype``
+        float32, float16 or bfloat16); ``MAX_DECODE_BATCH // beams`` prompts are searched together.
+        """
+        B, K = len(prompts), int(beams)
+        if B == 0:
+            return []
+        if not 1 <= K <= MAX_DECODE_BATCH or max_len < 1:
+            raise ValueError(f"{beams} beams (1 to {MAX_DECODE_BATCH}) of up to {max_len} tokens (1 at least)")
+        mins = [int(min_len)] * B if np.ndim(min_len) == 0 else [int(m) for m in min_len]
+        if len(mins) != B:
+            raise ValueError(f"{len(mins)} minimum lengths for {B} prompts")
+        group = MAX_DECODE_BATCH // K
+        out = []
+        for b in range(0, B, group):
+            part = prompts[b:b + group]
+            longest = -(-max(int(np.shape(p)[0]) for p in part) // 256) * 256
+            eng = self.beam_engine(len(part), K, longest, -(-max_len // 256) * 256, page_size, cache_dtype, length_penalty)
+            out += eng.run(part, mins[b:b + group], max_len, use_graph)
+        return out
+
+    def beam_engine(self, groups: int, beams: int, max_prompt: int, max_steps: int, page_size: int, cache_dtype,
+                    length_penalty: float):
+        from .paged import BeamEngine
+        key = (groups, beams, max_prompt, max_steps, page_size, cache_dtype, float(length_penalty))
+        if key not in self._beam_engines:
+            name = self.prefix + "llm_decoder.bias"
+            self._beam_engines[key] = BeamEngine(
+                self.body, self.w.weight(self.prefix + "llm_decoder.weight"), self.w.f32(name) if name in self.w else None,
+                self.w.weight(self.prefix + "speech_embedding"),
+                (self.speech_token_size, max(self.stop_token_ids) + 1), groups, beams, max_prompt, max_steps, page_size,
+                cache_dtype, length_penalty)
+        return self._beam_engines[key]
 
     # -- batched greedy decode ------------------------------------------------
     def engine(self, batch: int, cap: int, max_steps: int) -> DecodeEngine:

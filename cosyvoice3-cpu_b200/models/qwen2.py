@@ -254,6 +254,25 @@ def pk_sm_count() -> int:
     return int(torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count)
 
 
+def decode_gemvs(model: Qwen2Model, qkv_splits: int) -> list:
+    """Per layer the fused q8 decode GEMVs (RMSNorm in, residual / SwiGLU out: qkv, o, gate|up, down),
+    or None where the layer is not q8."""
+    c, fast = model.cfg, []
+    for i, L in enumerate(model.layers()):
+        p = f"layers.{i}."
+        ws = [L.qkv._keep[0], L.o._keep[0], model._t(p + "mlp.gate_proj.weight"),
+              model._t(p + "mlp.up_proj.weight"), L.down._keep[0]]
+        if all(isinstance(w, QTensor) and w.kind == "q8" for w in ws):   # (q4 layers: generic path)
+            gu = model.w.cache((model.prefix + p + "gate_up_interleaved",), lambda ws=ws: interleave_rows(ws[2], ws[3]))
+            fast.append((DecodeGemv(ws[0], L.qkv._keep[1], L.ln1, c.rms_norm_eps, mma_splits=qkv_splits),
+                         DecodeGemv(ws[1]),
+                         DecodeGemv(gu, norm_w=L.ln2, eps=c.rms_norm_eps, swiglu=True),
+                         DecodeGemv(ws[4], mma_splits=5)))
+        else:
+            fast.append(None)
+    return fast
+
+
 class DecodeEngine:
     """Batched greedy decode, one CUDA graph per step.
 
@@ -302,20 +321,7 @@ class DecodeEngine:
         self.graph = None
         self.keep_logp = False
         self.sampling = None  # (top_p, top_k, win_size, tau_r, strict): device sampler instead of greedy
-        # fused q8 decode GEMVs (RMSNorm in, residual / SwiGLU out) where the layer is q8
-        self.fast = []
-        for i, L in enumerate(model.layers()):
-            p = f"layers.{i}."
-            ws = [L.qkv._keep[0], L.o._keep[0], model._t(p + "mlp.gate_proj.weight"),
-                  model._t(p + "mlp.up_proj.weight"), L.down._keep[0]]
-            if all(isinstance(w, QTensor) and w.kind == "q8" for w in ws):   # (q4 layers: generic path)
-                gu = model.w.cache((model.prefix + p + "gate_up_interleaved",), lambda ws=ws: interleave_rows(ws[2], ws[3]))
-                self.fast.append((DecodeGemv(ws[0], L.qkv._keep[1], L.ln1, c.rms_norm_eps, mma_splits=self.QKV_SPLITS),
-                                  DecodeGemv(ws[1]),
-                                  DecodeGemv(gu, norm_w=L.ln2, eps=c.rms_norm_eps, swiglu=True),
-                                  DecodeGemv(ws[4], mma_splits=5)))
-            else:
-                self.fast.append(None)
+        self.fast = decode_gemvs(model, self.QKV_SPLITS)
         self.fast_head = DecodeGemv(head_w, norm_w=model.norm_w(), eps=c.rms_norm_eps) \
             if isinstance(head_w, QTensor) and head_w.kind == "q8" else None
         self._mk = self._persistent_setup()
