@@ -1,5 +1,8 @@
 """Compile ``csrc/*.cu`` into the in-tree ``libcv3cuda.so`` for sm_100a.
 
+``csrc/bind/*.cpp`` become Python extension modules next to it, for hosts with PyTorch (the short
+way of its callers to some entries; the library itself needs no GPU framework).
+
 Each translation unit is compiled by nvcc (in parallel, skipped when its object
 is newer than its sources and headers) and linked with ``nvcc -shared``.  The
 library lands next to this file so it travels with the source tree; the
@@ -46,6 +49,31 @@ def _compile(src: str, force: bool, hdr_time: float, extra) -> str:
     return obj
 
 
+def bind_path(src: str) -> str:
+    return os.path.join(HERE, "_" + os.path.basename(src)[:-4] + ".so")
+
+
+def _bind(src: str, force: bool) -> None:
+    """One extension module against the installed PyTorch (skipped where there is none)."""
+    import importlib.util
+    import sysconfig
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        return
+    out, torch_dir = bind_path(src), spec.submodule_search_locations[0]
+    header = os.path.join(INCLUDE, "cv3cuda.h")
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), os.path.getmtime(header)):
+        return
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=1",
+           "-I", os.path.join(torch_dir, "include"), "-I", os.path.join(cuda, "include"),
+           "-I", sysconfig.get_paths()["include"], src, "-o", out, "-L", os.path.join(torch_dir, "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {os.path.basename(src)}:\n{r.stdout}\n{r.stderr}")
+
+
 def build(force: bool = False, jobs: int = 0, extra=()) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
@@ -54,7 +82,10 @@ def build(force: bool = False, jobs: int = 0, extra=()) -> str:
     hdr = _deps()
     jobs = jobs or min(len(srcs), os.cpu_count() or 4)
     with ThreadPoolExecutor(jobs) as ex:
+        binds = [ex.submit(_bind, s, force) for s in sorted(glob.glob(os.path.join(CSRC, "bind", "*.cpp")))]
         objs = list(ex.map(lambda s: _compile(s, force, hdr, list(extra)), srcs))
+        for b in binds:
+            b.result()
     if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < max(os.path.getmtime(o) for o in objs):
         cmd = [NVCC, *ARCH, "-shared", "-o", LIB, *objs, "-lcudart"]
         r = subprocess.run(cmd, capture_output=True, text=True)

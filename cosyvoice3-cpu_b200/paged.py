@@ -21,14 +21,17 @@ they read on the device (lengths, tables, flags) may change between replays.
 
 from __future__ import annotations
 
+import ctypes
+import importlib.util
 import math
+import os
 import struct
 from typing import NamedTuple, Optional, Tuple
 
 import numpy as np
 
 from . import _dev as D
-from ._lib import check, load
+from ._lib import HERE, check, load
 
 torch = D.torch
 
@@ -62,6 +65,28 @@ class BeamStep(NamedTuple):
     scores: object       # float32
     counts: object       # int32
     done: object         # int32
+
+
+_bound = None   # the short way (csrc/bind/paged_bind.cpp), False where there is none
+
+
+def _bind():
+    """The extension module that takes plain calls of PyTorch tensors; False without PyTorch or without
+    the built module (every call then goes the long way, which gives the same results)."""
+    global _bound
+    if _bound is None:
+        path = os.path.join(HERE, "_paged_bind.so")
+        _bound = False
+        if torch is not None and os.path.exists(path):
+            spec = importlib.util.spec_from_file_location("_paged_bind", path)
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+            lib = load()
+            mod.setup(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in
+                        ("cv3_paged_extend", "cv3_paged_append", "cv3_paged_attention", "cv3_paged_attention_workspace",
+                         "cv3_beam_select", "cv3_beam_workspace", "cv3_paged_reorder")), PagedStep, BeamStep)
+            _bound = mod
+    return _bound
 
 
 def _new(like, shape, dtype):
@@ -150,6 +175,10 @@ def paged_extend(lens, new_lens, block_tables, free_pages, free_count, page_size
     Returns a :class:`PagedStep`; ``out`` gives it its tensors (``out.lens`` may be ``lens`` and
     ``out.free_count`` may be ``free_count``: the state then advances in place).
     """
+    if out is None and (_bound or _bind()):
+        r = _bound.extend(lens, new_lens, block_tables, free_pages, free_count, page_size, max_tokens, release)
+        if r is not None:
+            return r
     name = "paged_extend"
     arrays = (lens, new_lens, block_tables, free_pages, free_count)
     d = _device(name, *(arrays if release is None else arrays + (release,)))
@@ -195,6 +224,10 @@ def paged_append(qkv, slots, pos, k_pages, v_pages, heads: int, cos=None, sin=No
     may be None.  A slot outside the pool, or a position outside the tables, stores nothing and counts
     into ``bad`` (int32, one value).  The slots of one call must differ.
     """
+    if _bound or _bind():
+        r = _bound.append(qkv, slots, pos, k_pages, v_pages, heads, cos, sin, out, bad)
+        if r is not None:
+            return r
     name = "paged_append"
     d = _device(name, qkv, slots, k_pages, v_pages, *(x for x in (pos, cos, sin, out, bad) if x is not None))
     kt, shape, ks, vs = _pools(name, k_pages, v_pages, 4)
@@ -242,6 +275,10 @@ def paged_attention(q, k_pages, v_pages, block_tables, lens, scale: Optional[flo
     separate caches are joined.  Tokens of a page number outside the pool are left out and counted
     (per table entry) into ``bad``.
     """
+    if _bound or _bind():
+        r = _bound.attention(q, k_pages, v_pages, block_tables, lens, scale, window, out, return_lse, bad)
+        if r is not None:
+            return r
     name = "paged_attention"
     d = _device(name, q, k_pages, v_pages, block_tables, lens, *(x for x in (out, bad) if x is not None))
     kt, shape, ks, vs = _pools(name, k_pages, v_pages, 4)
@@ -293,6 +330,10 @@ def beam_select(logits, scores, counts, done, stop: Optional[Tuple[int, int]] = 
     first at the start.  NaN logits are no candidates.  Keys are computed in 64 bits.  ``out`` gives the
     :class:`BeamStep` its tensors, which may be the input state.
     """
+    if out is None and (_bound or _bind()):
+        r = _bound.beam(logits, scores, counts, done, stop, min_len, length_penalty)
+        if r is not None:
+            return r
     name = "beam_select"
     d = _device(name, logits, scores, counts, done, *((min_len,) if min_len is not None else ()))
     t = _type(name, logits)
@@ -339,6 +380,8 @@ def paged_reorder(k_pages, v_pages, block_tables, parents, lens) -> None:
     ``parents[g][k]`` was: full pages are shared through the table, the tokens of the last, partly
     filled page are copied into the page that beam k's own row names there (and no other beam's).
     """
+    if (_bound or _bind()) and _bound.reorder(k_pages, v_pages, block_tables, parents, lens):
+        return
     name = "paged_reorder"
     d = _device(name, k_pages, v_pages, block_tables, parents, lens)
     dims = len(k_pages.shape)

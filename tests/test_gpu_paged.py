@@ -647,3 +647,84 @@ def test_graph_replay_on_a_side_stream():
         torch.cuda.synchronize()
         for (g, q, lens, out), (fq, fl) in zip(graphs, feeds):
             assert torch.equal(out, ops.paged_attention(fq, k, v, tables, fl))
+
+
+# ---------------------------------------------------------------------------
+# the two ways of a call
+# ---------------------------------------------------------------------------
+
+def test_short_and_long_way_agree(monkeypatch):
+    """The extension module takes the plain calls and gives what the Python way gives, bit for bit; the
+    calls it does not take are refused with the Python way's messages."""
+    import torch
+    ops, P = _ops(), pkg("paged")
+    mod = P._bind()
+    assert mod, "the extension module was not built"
+    rng = np.random.default_rng(31)
+    tables, Pn, rest = _tables(rng, [40, 0, 333], 16, 24)
+    stack = np.zeros(Pn, np.int32)
+    stack[:len(rest)] = rest
+    k, v = (_cuda(rng.normal(size=(2, Pn, 2, 16, 64)).astype(np.float32)) for _ in range(2))
+    lens, new = _cuda(np.array([40, 0, 333], np.int32)), _cuda(np.array([1, 1, 1], np.int32))
+    qkv = _cuda(rng.normal(size=(3, 18 * 64)).astype(np.float32))
+    tab = _cuda(rng.normal(size=(400, 64)).astype(np.float32))
+    logits = _cuda(rng.normal(size=(1, 3, 777)).astype(np.float32))
+    scores, z = _cuda(rng.normal(size=(1, 3)).astype(np.float32)), torch.zeros(1, 3, dtype=torch.int32, device="cuda")
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def all_of_them():
+        kk, vv, td, sd = k.clone(), v.clone(), _cuda(tables), _cuda(stack)
+        cd = _cuda(np.array([len(rest)], np.int32))
+        r = ops.paged_extend(lens, new, td, sd, cd, 16, 4, release=_cuda(np.array([0, 1, 0], np.int32)))
+        q = ops.paged_append(qkv, r.slots[:3], r.pos[:3], kk[1], vv[1], 14, tab, tab, bad=bad)
+        q2 = ops.paged_append(qkv, r.slots[:3], None, kk[0], vv[0], 14, out=torch.empty_like(q))
+        o, lse = ops.paged_attention(q, kk[1], vv[1], td, r.lens, scale=0.2, window=100, return_lse=True, bad=bad)
+        o2 = ops.paged_attention(q, kk[1], vv[1], td, r.lens)
+        b = ops.beam_select(logits, scores, z, z, stop=(700, 777), length_penalty=0.5)
+        ops.paged_reorder(kk, vv, td, b.parents, r.lens)
+        ops.paged_reorder(kk[0], vv[0], td, b.parents, r.lens)
+        assert type(r) is ops.PagedStep and type(b) is ops.BeamStep
+        return [*r, q, q2, o, lse, o2, *b, kk, vv, td, sd]
+
+    taken = []
+    for name in ("extend", "append", "attention", "beam", "reorder"):
+        def spy(*a, f=getattr(mod, name), name=name):
+            r = f(*a)
+            taken.append((name, r is not None))
+            return r
+        monkeypatch.setattr(mod, name, spy)
+    short = all_of_them()
+    assert len(taken) == 8 and all(t for _, t in taken)
+    monkeypatch.setattr(P, "_bound", False)
+    monkeypatch.setattr(P, "_bind", lambda: False)
+    for a, b in zip(short, all_of_them()):
+        assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
+
+
+def test_refusals_on_the_device():
+    import torch
+    ops = _ops()
+    k = torch.zeros(3, 2, 16, 64, device="cuda")
+    q = torch.zeros(2, 4, 64, device="cuda")
+    t, n = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    ops.paged_attention(q, k, k, t, n)
+    for a in ((q.cpu(), k, k, t, n), (q, k.cpu(), k, t, n), (q, k, k, t, n.long()), (q[:, :3], k, k, t, n), (q, k, k, t.T, n),
+              (q, k, k.half(), t, n), (q.double(), k, k, t, n), (q, k[..., :32], k[..., :32], t, n)):
+        with pytest.raises(ValueError):
+            ops.paged_attention(*a)
+    with pytest.raises(ValueError):
+        ops.paged_attention(q, k, k, t, n, window=-1)
+    with pytest.raises(ValueError):
+        ops.paged_attention(q, k.view(3, 2, 16, 64)[..., 1:], k[..., 1:], t, n)
+    with pytest.raises(RuntimeError, match="head_dim"):
+        ops.paged_attention(torch.zeros(2, 4, 80, device="cuda"), torch.zeros(3, 2, 16, 80, device="cuda"),
+                            torch.zeros(3, 2, 16, 80, device="cuda"), t, n)
+    off = torch.zeros(3 * 2 * 16 * 64 + 4, device="cuda")[4:].view(3, 2, 16, 64)
+    with pytest.raises(ValueError, match="32-byte"):
+        ops.paged_attention(q, off, off, t, n)
+    with pytest.raises(RuntimeError, match="beams"):
+        ops.beam_select(torch.zeros(1, 33, 9, device="cuda"), torch.zeros(1, 33, device="cuda"),
+                        *(torch.zeros(1, 33, dtype=torch.int32, device="cuda") for _ in range(2)))
+    with pytest.raises(ValueError):
+        ops.beam_select(torch.zeros(1, 3, 9, device="cuda"), torch.zeros(1, 3, device="cuda"),
+                        *(torch.zeros(1, 3, dtype=torch.int32, device="cuda") for _ in range(2)), stop=(0, 10))
