@@ -145,16 +145,22 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
   int v0 = 0;  // token of the lane's first logit; the others follow in steps of 32
   auto inside = [&](int e) -> bool { return v0 + e * 32 < a.vocab; };
   auto stopped = [&](int e) -> bool { return v0 + e * 32 >= a.stop_lo && v0 + e * 32 < a.stop_hi; };
-  auto load = [&](int tile) {
-    v0 = begin + tile * TILE + lane;
-    const T* p = logits + v0;
-    if (v0 - lane + TILE <= a.vocab) {
+  T raw[16];
+  auto fetch = [&](int tile) {
+    const int at = begin + tile * TILE + lane;
+    const T* p = logits + at;
+    if (at - lane + TILE <= a.vocab) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = cv3p::to_f32<T>(p[e * 32]);
+      for (int e = 0; e < 16; ++e) raw[e] = p[e * 32];
     } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = inside(e) ? cv3p::to_f32<T>(p[e * 32]) : -INFINITY;
+      for (int e = 0; e < 16; ++e) raw[e] = at + e * 32 < a.vocab ? p[e * 32] : cv3p::from_f32<T>(-INFINITY);
     }
+  };
+  auto take = [&](int tile) {
+    v0 = begin + tile * TILE + lane;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = cv3p::to_f32<T>(raw[e]);
   };
   auto no_nan = [&]() {  // a NaN logit is no term, and as good as -inf
 #pragma unroll
@@ -171,7 +177,8 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
   // the tiles' maxima
   float wtop = -INFINITY;
   if (warp < tiles) {
-    load(warp);
+    fetch(warp);
+    take(warp);
     wtop = maximum();
   }
   __syncthreads();  // (the last task's shared memory is done with)
@@ -182,6 +189,7 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
 #pragma unroll
   for (int w = 0; w < BW; ++w) m = fmaxf(m, sh.ms[w]);
   for (int tile = warp; tile < tiles;) {
+    if (tile + BW < tiles) fetch(tile + BW);  // on its way while this one is worked on
     if (wtop > m) {
       if (s != 0.0) s *= exp((double)m - (double)wtop);
       m = wtop;
@@ -231,7 +239,7 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
     }
     tile += BW;
     if (tile < tiles) {
-      load(tile);
+      take(tile);
       wtop = maximum();
     }
   }
@@ -242,7 +250,7 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
     u64 best = 0;
     for (int i = 0; i < tiles; i += 32) {
       const u64 key = i + lane < tiles ? (u64)sh.tops[i + lane] : 0ull;
-      if (__any_sync(0xffffffffu, key > from_lane(best, K - 1))) best = merged(best, sorted(key));
+      if (__any_sync(0xffffffffu, key > from_lane(best, K - 1))) best = i ? merged(best, sorted(key)) : sorted(key);
     }
     const uint32_t bar = (uint32_t)from_lane(best, K - 1);
     if (lane == 0) sh.bar = bar;
@@ -254,6 +262,7 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
   const float least = bar ? unordered(bar) : -INFINITY;
   u64* held = sh.held[warp];
   int count = 0, turn = 0;
+  bool listed = false;
   list = 0;
   auto flush = [&]() {
     __syncwarp();
@@ -261,14 +270,16 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
     __syncwarp();
     held[lane] = rest;
     count = max(count - 32, 0);
-    list = merged(list, sorted(key));
+    list = listed ? merged(list, sorted(key)) : sorted(key);
+    listed = true;
     if (lane >= K) list = 0;
   };
   for (int t0 = 0; t0 < tiles; t0 += 32) {
     unsigned reach = __ballot_sync(0xffffffffu, t0 + lane < tiles && sh.tops[t0 + lane] >= bar);
     for (; reach; reach &= reach - 1) {
       if (turn++ % BW != warp) continue;
-      load(t0 + __ffs(reach) - 1);
+      fetch(t0 + __ffs(reach) - 1);
+      take(t0 + __ffs(reach) - 1);
       no_nan();
       unsigned mine = 0;
 #pragma unroll
@@ -372,7 +383,7 @@ __device__ void choose(const BeamArgs& a, int64_t g, const char* work) {
     }
     const Cand last = from_lane(list, K - 1);
     if (!__any_sync(0xffffffffu, better(c, last))) continue;
-    list = merged(list, sorted(c));
+    list = i0 < BT ? sorted(c) : merged(list, sorted(c));
     if (lane >= K) list = Cand{0, 0};
   }
   lists[warp][lane] = list;
@@ -403,7 +414,7 @@ __device__ void choose(const BeamArgs& a, int64_t g, const char* work) {
 
 // two launches: a CTA per task, then one per group
 template <typename T>
-__global__ void __launch_bounds__(BT, 4) beam_scan_kernel(const BeamArgs a) {
+__global__ void __launch_bounds__(BT, 3) beam_scan_kernel(const BeamArgs a) {
   __shared__ Scratch sh;
   dep_wait();
   dep_release();
