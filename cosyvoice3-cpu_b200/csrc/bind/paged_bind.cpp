@@ -116,12 +116,14 @@ void table_of(Call& c, int i, int64_t rows, int*& p, int64_t& ld, int64_t& cols)
 }
 
 // a pair of page pools with contiguous rows
-void pools_of(Call& c, const Tensor& k, const Tensor& v, int dims) {
+void pools_of(Call& c, const Tensor& k, const Tensor& v, int dims, bool written = false) {
   if (!c.ok) return;
   c.need(k.dim() == dims && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && type_of(k) >= 0);
   if (!c.ok) return;
   c.need(k.stride(dims - 1) == 1 && v.stride(dims - 1) == 1 && k.size(dims - 2) > 0 && k.size(dims - 3) > 0 &&
          k.size(dims - 1) > 0);
+  if (written)  // (no expanded views)
+    for (int i = 0; i < dims; ++i) c.need(k.size(i) <= 1 || (k.stride(i) && v.stride(i)));
 }
 
 bool alike(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
@@ -181,7 +183,7 @@ PyObject* extend(PyObject*, PyObject* const* args, Py_ssize_t) {
 PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t) {
   Call c(args);
   const Tensor &qkv = c.tensor(0), &k = c.tensor(3), &v = c.tensor(4);
-  pools_of(c, k, v, 4);
+  pools_of(c, k, v, 4, true);
   cv3_paged_append_params p = {sizeof(p)};
   p.heads = c.integer(5);
   if (!c.ok || qkv.dim() != 2 || type_of(qkv) < 0 || p.heads <= 0) Py_RETURN_NONE;
@@ -329,7 +331,7 @@ PyObject* reorder(PyObject*, PyObject* const* args, Py_ssize_t) {
   const Tensor &k = c.tensor(0), &v = c.tensor(1), &parents = c.tensor(3);
   if (!c.ok || (k.dim() != 4 && k.dim() != 5) || parents.dim() != 2) Py_RETURN_NONE;
   const int d = (int)k.dim() - 4;
-  pools_of(c, k, v, 4 + d);
+  pools_of(c, k, v, 4 + d, true);
   cv3_paged_reorder_params p = {sizeof(p)};
   p.groups = parents.size(0), p.beams = parents.size(1);
   const int64_t n = p.groups * p.beams;

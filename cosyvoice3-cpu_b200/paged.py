@@ -144,7 +144,7 @@ def _type(name: str, x) -> int:
     return t
 
 
-def _pools(name: str, k, v, dims: int):
+def _pools(name: str, k, v, dims: int, written: bool = False):
     """(type, shape, k strides, v strides) of a pair of page pools with contiguous rows."""
     shape, ks, vs = k.shape, k.stride(), v.stride()
     if len(shape) != dims or tuple(v.shape) != tuple(shape) or v.dtype != k.dtype:
@@ -154,6 +154,8 @@ def _pools(name: str, k, v, dims: int):
         raise ValueError(f"{name}: the rows of head_dim elements must be contiguous")
     if min(ks) < 0 or min(vs) < 0 or shape[-2] == 0 or shape[-3] == 0:
         raise ValueError(f"{name}: empty or reversed page dimensions")
+    if written and any(n > 1 and (a == 0 or b == 0) for n, a, b in zip(shape, ks, vs)):
+        raise ValueError(f"{name}: pools that are written cannot be expanded views")
     return _type(name, k), shape, ks, vs
 
 
@@ -230,7 +232,7 @@ def paged_append(qkv, slots, pos, k_pages, v_pages, heads: int, cos=None, sin=No
             return r
     name = "paged_append"
     d = _device(name, qkv, slots, k_pages, v_pages, *(x for x in (pos, cos, sin, out, bad) if x is not None))
-    kt, shape, ks, vs = _pools(name, k_pages, v_pages, 4)
+    kt, shape, ks, vs = _pools(name, k_pages, v_pages, 4, True)
     pages, kv, ps, dim = shape
     t = _type(name, qkv)
     if qkv.dim() != 2 or heads <= 0 or qkv.shape[1] != (heads + 2 * kv) * dim:
@@ -387,7 +389,7 @@ def paged_reorder(k_pages, v_pages, block_tables, parents, lens) -> None:
     dims = len(k_pages.shape)
     if dims not in (4, 5):
         raise ValueError(f"{name}: pools of 4 or 5 dimensions expected, got {tuple(k_pages.shape)}")
-    kt, shape, ks, vs = _pools(name, k_pages, v_pages, dims)
+    kt, shape, ks, vs = _pools(name, k_pages, v_pages, dims, True)
     if dims == 4:
         shape, ks, vs = (1,) + tuple(shape), (0,) + tuple(ks), (0,) + tuple(vs)
     layers, pages, kv, ps, dim = shape

@@ -143,6 +143,29 @@ def test_extend_in_place_and_wide_table():
     assert bool((wide[:, :3] == -9).all()) and bool((wide[:, 15:] == -9).all())
 
 
+def test_extend_many_requests_in_place():
+    """Hundreds of requests that come, grow and go, the state advanced in place; twice the same bits."""
+    import torch
+    ops = _ops()
+    rng = np.random.default_rng(40)
+    B, ps, cols, P = 300, 4, 40, 9000
+    for repeat in range(2):
+        rng = np.random.default_rng(40)
+        tables, stack = np.full((B, cols), -1, np.int32), np.arange(P, dtype=np.int32)
+        lens, count = np.zeros(B, np.int32), P
+        td, sd, ld, cd = _cuda(tables), _cuda(stack), _cuda(lens), _cuda(np.array([count], np.int32))
+        out = ops.PagedStep(*(torch.empty(n, dtype=t, device="cuda") for n, t in
+                              ((5000, torch.int64), (5000, torch.int32), (5000, torch.int32), (B + 1, torch.int32))), ld, cd)
+        for step in range(6):
+            new = rng.integers(0, 30, B).astype(np.int32)
+            rel = (rng.random(B) < 0.3).astype(np.int32)
+            tables, stack, slots, seq, pos, offsets, lens, count = ref.extend(lens, new, tables, stack, count, ps, 5000, rel)
+            ops.paged_extend(ld, _cuda(new), td, sd, cd, ps, 5000, release=_cuda(rel), out=out)
+            for a, b in ((td, tables), (ld, lens), (out.slots, slots), (out.seq, seq), (out.pos, pos), (out.offsets, offsets)):
+                assert np.array_equal(_np(a), b), step
+            assert int(cd) == count and np.array_equal(_np(sd)[:count], stack[:count])
+
+
 # ---------------------------------------------------------------------------
 # RoPE and store
 # ---------------------------------------------------------------------------
@@ -728,3 +751,64 @@ def test_refusals_on_the_device():
     with pytest.raises(ValueError):
         ops.beam_select(torch.zeros(1, 3, 9, device="cuda"), torch.zeros(1, 3, device="cuda"),
                         *(torch.zeros(1, 3, dtype=torch.int32, device="cuda") for _ in range(2)), stop=(0, 10))
+
+
+def test_numpy_host():
+    """The operators on the library's own device arrays, PyTorch blocked: the chain's results equal the
+    64-bit restatement's (tolerances as above)."""
+    import subprocess
+    import sys
+    from conftest import REPO
+    child = r"""
+import importlib, sys
+sys.modules["torch"] = None
+sys.path.insert(0, sys.argv[1])
+import numpy as np
+import oracle.paged as ref
+P = "cosyvoice3-cpu_b200."
+ops, D = importlib.import_module(P + "ops"), importlib.import_module(P + "_dev")
+assert D.BACKEND == "numpy"
+up = D.DeviceArray.from_numpy
+rng = np.random.default_rng(0)
+B, H, Hk, d, ps, cols, pages = 3, 6, 2, 64, 16, 6, 24
+k, v = np.zeros((2, pages, Hk, ps, d), np.float32), np.zeros((2, pages, Hk, ps, d), np.float32)
+tables, stack = np.full((B, cols), -1, np.int32), np.arange(pages, dtype=np.int32)
+lens, new = np.zeros(B, np.int32), np.array([40, 0, 90], np.int32)
+kd, vd, td, sd = up(k), up(v), up(tables), up(stack)
+r = ops.paged_extend(up(lens), up(new), td, sd, up(np.array([pages], np.int32)), ps, 131)
+tables, stack, slots, seq, pos, offsets, lens, count = ref.extend(lens, new, tables, stack, pages, ps, 131)
+for a, b in zip(r, (slots, seq, pos, offsets, lens, np.array([count], np.int32))):
+    assert np.array_equal(a.numpy(), b)
+qkv = rng.normal(size=(131, (H + 2 * Hk) * d)).astype(np.float32)
+cos, sin = rng.normal(size=(2, 100, d)).astype(np.float32)
+q = ops.paged_append(up(qkv), r.slots, r.pos, kd[1], vd[1], H, up(cos), up(sin))
+x = qkv.reshape(131, H + 2 * Hk, d)
+turned = ref.rope_rows(x[:, :H + Hk], cos[pos], sin[pos])
+assert np.abs(q.numpy() - turned[:, :H]).max() < 3e-6
+k[1][slots[:130] // ps, :, slots[:130] % ps] = turned[:130, H:]
+v[1][slots[:130] // ps, :, slots[:130] % ps] = x[:130, H + Hk:]
+assert np.abs(kd.numpy() - k).max() < 3e-6 and np.array_equal(vd.numpy(), v)
+qq = rng.normal(size=(B, H, d)).astype(np.float32)
+o, lse = ops.paged_attention(up(qq), kd[1], vd[1], td, r.lens, return_lse=True)
+want, wl = ref.attention(qq, kd.numpy()[1], v[1], tables, lens, d ** -0.5)
+assert np.abs(o.numpy() - want).max() < 1e-5 * np.abs(want).max() and not o.numpy()[1].any()
+logits = rng.normal(size=(1, 3, 500)).astype(np.float32)
+s, z = rng.normal(size=(1, 3)).astype(np.float32), np.zeros((1, 3), np.int32)
+b = ops.beam_select(up(logits), up(s), up(z), up(z), stop=(490, 500))
+w = ref.beam(logits, s, z, z, (490, 500))
+assert np.array_equal(b.tokens.numpy(), w[0]) and np.array_equal(b.parents.numpy(), w[1])
+par = np.array([[2, 0, 0]], np.int32)
+n = np.full(3, 21, np.int32)
+t3 = np.arange(18, dtype=np.int32).reshape(3, 6)
+t3d = up(t3)
+kk, vv = kd.numpy(), vd.numpy()
+ops.paged_reorder(kd, vd, t3d, up(par), up(n))
+wk, wv, wt = ref.reorder(kk, vv, t3, par, n)
+assert np.array_equal(kd.numpy(), wk) and np.array_equal(vd.numpy(), wv) and np.array_equal(t3d.numpy(), wt)
+try:
+    ops.paged_attention(qq, kd[1], vd[1], td, r.lens)
+except ValueError:
+    print("numpy host ok")
+"""
+    r = subprocess.run([sys.executable, "-c", child, REPO], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "numpy host ok" in r.stdout, r.stderr[-2000:]

@@ -97,7 +97,8 @@ def test_append_refusals(ops):
                    dict(v_pages=pool.half()), dict(v_pages=pool[:2]), dict(k_pages=pool[0], v_pages=pool[0]),
                    dict(k_pages=pool.transpose(2, 3), v_pages=pool.transpose(2, 3)),
                    dict(qkv=torch.zeros(4, 8 * 64, dtype=torch.int32)), dict(qkv=torch.zeros(8 * 64, 4).T),
-                   dict(out=torch.zeros(4, 4, 32)), dict(bad=_i32(2)), dict(qkv=torch.zeros(4, 8, 64))):
+                   dict(out=torch.zeros(4, 4, 32)), dict(bad=_i32(2)), dict(qkv=torch.zeros(4, 8, 64)),
+                   dict(k_pages=pool[:1].expand(3, 2, 16, 64))):
         with pytest.raises(ValueError):
             ops.paged_append(**{**good, **change})
 
@@ -135,7 +136,8 @@ def test_beam_and_reorder_refusals(ops):
     with pytest.raises(AssertionError, match="accepted"):
         ops.paged_reorder(**fine)
     for change in (dict(k_pages=pool[0, 0]), dict(v_pages=pool[0]), dict(block_tables=_i32(5, 3)), dict(parents=_i32(6)),
-                   dict(lens=_i32(2)), dict(parents=torch.zeros(2, 3)), dict(k_pages=pool.int(), v_pages=pool.int())):
+                   dict(lens=_i32(2)), dict(parents=torch.zeros(2, 3)), dict(k_pages=pool.int(), v_pages=pool.int()),
+                   dict(v_pages=pool[:1].expand(2, 9, 2, 16, 64))):
         with pytest.raises(ValueError):
             ops.paged_reorder(**{**fine, **change})
 
