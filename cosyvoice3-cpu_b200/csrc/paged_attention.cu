@@ -197,9 +197,8 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
   const int per = a.kv_heads * a.groups;  // pairs of a request
   const int c = blockIdx.x;
 
-  // tiles [t0, t1) of a pair: the warps' maxima, sums and unnormalised outputs to shared memory
-  auto attend = [&](int b, int pair, int lo, int hi, int g, int h0, int nh, int t0, int t1) {
-    __syncthreads();  // the last pair's shared memory is done with
+  // a pair's queries as product operands in shared memory
+  auto queries = [&](int b, int h0, int nh) {
     for (int i = tid; i < QS * 32; i += NW * 32) {
       const int s = i >> 5, ln = i & 31, row = ln >> 2;
       const int64_t at = b * a.qsb + (h0 + row) * a.qsh;
@@ -223,8 +222,29 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
         *reinterpret_cast<uint4*>(&sq[s][ln][0]) = make_uint4(v[0], v[1], v[2], v[3]);
       }
     }
-    __syncthreads();
+  };
 
+  // Table entries that a step's lookups need: UNI: of its 16-key groups; else of the rows that this lane
+  // reads: key n, values 2t and 2t + 1 of each 8 keys.  Only the table's own bounds are looked at, so the
+  // first step's entries may be fetched before the request's length is known.
+  int ent[GK][UNI ? 1 : 3];
+  auto peek = [&](const int* table, int key0) {
+    auto entry = [&](int key) -> int { return key < a.max_keys ? table[page_index(a, key)] : -1; };
+#pragma unroll
+    for (int i = 0; i < GK; ++i) {
+      if constexpr (UNI) {
+        ent[i][0] = entry(key0 + i * 16);
+      } else {
+        ent[i][0] = entry(key0 + i * 8 + n);
+        ent[i][1] = entry(key0 + i * 8 + 2 * t);
+        ent[i][2] = entry(key0 + i * 8 + 2 * t + 1);
+      }
+    }
+  };
+
+  // Tiles t0, t0 + every, ... below t1 of a pair (the first's entries peeked at): the warps' maxima, sums and
+  // unnormalised outputs to shared memory.  The queries are there, but for the barrier.
+  auto attend = [&](int b, int pair, int lo, int hi, int g, int t0, int t1, int every) {
     const KT* kb = static_cast<const KT*>(a.k) + g * a.ksh;
     const KT* vb = static_cast<const KT*>(a.v) + g * a.vsh;
     const int* table = a.tables + b * a.ld;
@@ -233,32 +253,28 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = 0.f;
 
-    // the page of a key, -1 for none; `mine`: this lane counts a bad one
-    auto page_of = [&](int key, bool mine) -> int {
-      if (key < lo || key >= hi) return -1;
-      const int blk = page_index(a, key);
-      const int p = table[blk];
-      const bool ok = (unsigned)p < (unsigned)a.pages;
-      if (!ok && counts && mine && (key == lo || key == blk * a.ps)) atomicAdd(a.bad, 1);
-      return ok ? p : -1;
-    };
-
     Raw<KB> kr[NT][KC];
     Raw<VB> vr[NT][2][VC];
-    const int first = (lo & -KI) + t0 * TK + warp * KI, end = min(hi, (lo & -KI) + t1 * TK);
-    // pages of a step: UNI: of its 16-key groups (any visible key of one names it); else of the rows
-    // that this lane reads: key n, values 2t and 2t + 1 of each 8 keys
+    const int base = lo & -KI, first = base + t0 * TK + warp * KI, end = min(hi, base + t1 * TK), ahead = every * TK;
+    // the pages of a step from its table entries, -1 for none
     int pg[GK][UNI ? 1 : 3];
-    auto look = [&](int key0) {
+    auto settle = [&](int key0) {
+      // key: the first that this lookup stands for; mine: this lane counts a bad entry
+      auto page = [&](int entry, int key, bool mine) -> int {
+        if (key < lo || key >= hi) return -1;
+        const bool ok = (unsigned)entry < (unsigned)a.pages;
+        if (!ok && counts && mine && (key == lo || key == page_index(a, key) * a.ps)) atomicAdd(a.bad, 1);
+        return ok ? entry : -1;
+      };
 #pragma unroll
       for (int i = 0; i < GK; ++i) {
         if constexpr (UNI) {
           const int k0 = key0 + i * 16;
-          pg[i][0] = k0 < hi && k0 + min(KI, 16) > lo ? page_of(max(k0, lo), lane == 0) : -1;
+          pg[i][0] = k0 + min(KI, 16) > lo ? page(ent[i][0], max(k0, lo), lane == 0) : -1;
         } else {
-          pg[i][0] = page_of(key0 + i * 8 + n, false);
-          pg[i][1] = page_of(key0 + i * 8 + 2 * t, n == 0);
-          pg[i][2] = page_of(key0 + i * 8 + 2 * t + 1, n == 0);
+          pg[i][0] = page(ent[i][0], key0 + i * 8 + n, false);
+          pg[i][1] = page(ent[i][1], key0 + i * 8 + 2 * t, n == 0);
+          pg[i][2] = page(ent[i][2], key0 + i * 8 + 2 * t + 1, n == 0);
         }
       }
     };
@@ -290,22 +306,14 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
     };
 
     if (first < end) {
-      look(first);
+      settle(first);
       load_k(first);
     }
-    for (int key0 = first; key0 < end; key0 += TK) {
+    __syncthreads();  // the queries are in shared memory; what it held before is done with
+    for (int key0 = first; key0 < end; key0 += ahead) {
       load_v(key0);
-      // which of this lane's scores (keys 2t, 2t + 1 of each 8) count
-      bool seen[NT][2];
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int key = key0 + i * 8 + 2 * t + r;
-          seen[i][r] = (UNI ? pg[i / 2][0] : pg[i][1 + r]) >= 0 && key >= lo && key < hi;
-        }
-      const int next = key0 + TK;
-      if (next < end) look(next);
+      const int next = key0 + ahead;
+      if (next < end) peek(table, next);
       float s0[NT][4], s1[NT][4];  // two chains: even and odd steps, or upper and lower parts of the keys
 #pragma unroll
       for (int i = 0; i < NT; ++i)
@@ -340,8 +348,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
           }
         }
       }
-      if (next < end) load_k(next);
-      float top = m;
+      float top = m, sc[NT][2];  // this lane's scores: keys 2t, 2t + 1 of each 8
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -349,9 +356,15 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
           const float rest = s1[i][r] + s1[i][2 + r];
           const float x = H16 ? (s0[i][r] + s1[i][r]) * (a.scale * LOG2E)
                               : (s0[i][r] + s0[i][2 + r]) + (WIDE ? or_zero(rest) : rest);
-          s0[i][r] = seen[i][r] ? x : -INFINITY;
-          top = fmaxf(top, s0[i][r]);
+          const int key = key0 + i * 8 + 2 * t + r;
+          const bool seen = (UNI ? pg[i / 2][0] : pg[i][1 + r]) >= 0 && key >= lo && key < hi;
+          sc[i][r] = seen ? x : -INFINITY;
+          top = fmaxf(top, sc[i][r]);
         }
+      if (next < end) {
+        settle(next);
+        load_k(next);
+      }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const float ref = top == -INFINITY ? 0.f : top;
@@ -363,7 +376,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          pr[i][r] = exp2_fast(s0[i][r] - ref);
+          pr[i][r] = exp2_fast(sc[i][r] - ref);
           l += pr[i][r];
         }
       if constexpr (H16) {
@@ -429,23 +442,32 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
       }
     __syncthreads();
   };
-  // the warps' shares of output element (h, e) together
-  auto gather = [&](int h, int e, float& M, float& L, float& x) {
-    M = -INFINITY;
-    L = x = 0.f;
+  // Warp w puts head w's shares together: the lane's D / 32 outputs (every 32nd), in every lane M and L.
+  constexpr int E = D / 32;
+  auto gather = [&](float& M, float& L, float (&x)[E]) {
+    const int h = warp;
+    const float m = sm[lane % NW][h], l = sl[lane % NW][h];  // (a warp's sum is NaN where it met a NaN score)
+    M = m;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w][h]);
+    for (int o = NW / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float f = l == 0.f ? 0.f : exp2_fast(m - M);
+    L = l * f;
+#pragma unroll
+    for (int o = NW / 2; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      if (sl[w][h] == 0.f) continue;  // saw nothing (a NaN score leaves a NaN sum)
-      const float f = exp2_fast(sm[w][h] - M);
-      L = fmaf(sl[w][h], f, L);
-      x = fmaf(so[w][h][e], f, x);
+      const float fw = __shfl_sync(0xffffffffu, f, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = fmaf(so[w][h][e * 32 + lane], fw, x[e]);
     }
   };
-  auto finish = [&](int b, int h, int e, float M, float L, float x) {
-    cv3p::store_any(a.out, a.q_type, b * a.osb + h * a.osh + e, L == 0.f ? 0.f : x / L);
-    if (a.lse && e == 0) a.lse[(int64_t)b * a.heads + h] = L == 0.f ? -INFINITY : (M + log2f(L)) / LOG2E;
+  auto finish = [&](int b, int h, float M, float L, const float (&x)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      cv3p::store_any(a.out, a.q_type, b * a.osb + h * a.osh + e * 32 + lane, L == 0.f ? 0.f : x[e] / L);
+    if (a.lse && lane == 0) a.lse[(int64_t)b * a.heads + h] = L == 0.f ? -INFINITY : (M + log2f(L)) / LOG2E;
   };
   auto heads_of = [&](int pair, int& g, int& h0, int& nh) {
     g = pair / a.groups;
@@ -462,47 +484,47 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
     const int S = gridDim.x / (a.batch * per), rank = c % S;
     const int b = c / S / per, pair = c / S - b * per;
     int lo, hi, g, h0, nh;
-    visible(a, b, lo, hi);
     heads_of(pair, g, h0, nh);
-    const int tiles = tiles_of(b);
-    const int t0 = (int)((int64_t)tiles * rank / S), t1 = (int)((int64_t)tiles * (rank + 1) / S);
-    attend(b, pair, lo, hi, g, h0, nh, t0, t1);
+    // CTA `rank` has the tiles rank, rank + S, ...: without a window the first one's entries and the queries are
+    // on their way before the length is known
+    const int* table = a.tables + b * a.ld;
+    if (a.window == 0) peek(table, rank * TK + warp * KI);
+    queries(b, h0, nh);
+    visible(a, b, lo, hi);
+    if (a.window != 0) peek(table, (lo & -KI) + rank * TK + warp * KI);
+    attend(b, pair, lo, hi, g, rank, tiles_of(b), S);
+    float M, L, x[E];
+    gather(M, L, x);
     if (S == 1) {
-      for (int i = tid; i < nh * D; i += NW * 32) {
-        float M, L, x;
-        gather(i / D, i % D, M, L, x);
-        finish(b, h0 + i / D, i % D, M, L, x);
-      }
+      if (warp < nh) finish(b, h0 + warp, M, L, x);
       return;
     }
     __shared__ float stat[HT][2];
-    for (int i = tid; i < nh * D; i += NW * 32) {
-      float M, L, x;
-      gather(i / D, i % D, M, L, x);
-      so[0][i / D][i % D] = x;  // (read and written by this thread alone)
-      if (i % D == 0) { stat[i / D][0] = M; stat[i / D][1] = L; }
-    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) so[0][warp][e * 32 + lane] = x[e];  // (read by this lane alone so far)
+    if (lane == 0) { stat[warp][0] = M; stat[warp][1] = L; }
     cv3p::cluster_sync();
-    for (int i = tid + rank * NW * 32; i < nh * D; i += S * NW * 32) {
-      const int h = i / D, e = i - h * D;
-      float M = -INFINITY, L = 0.f, x = 0.f, m[8], l[8], o[8];
+    if (warp % S == rank && warp < nh) {  // the heads are dealt to the CTAs
+      const bool there = lane < S;
+      const float m = there ? cv3p::cluster_load(&stat[warp][0], lane) : -INFINITY;
+      const float l = there ? cv3p::cluster_load(&stat[warp][1], lane) : 0.f;
+      float o[8][E];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[r][e] = r < S ? cv3p::cluster_load(&so[0][warp][e * 32 + lane], r) : 0.f;
+      M = warp_max(m);
+      const float f = l == 0.f ? 0.f : exp2_fast(m - M);
+      L = warp_sum(l * f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = 0.f;
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        if (r >= S) break;
-        m[r] = cv3p::cluster_load(&stat[h][0], r);
-        l[r] = cv3p::cluster_load(&stat[h][1], r);
-        o[r] = cv3p::cluster_load(&so[0][h][e], r);
-        M = fmaxf(M, m[r]);
-      }
+        const float fr = __shfl_sync(0xffffffffu, f, r);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        if (r >= S) break;
-        if (l[r] == 0.f) continue;
-        const float f = exp2_fast(m[r] - M);
-        L = fmaf(l[r], f, L);
-        x = fmaf(o[r], f, x);
+        for (int e = 0; e < E; ++e) x[e] = fmaf(o[r][e], fr, x[e]);
       }
-      finish(b, h0 + h, e, M, L, x);
+      finish(b, h0 + warp, M, L, x);
     }
     cv3p::cluster_sync();  // no CTA leaves while another reads its shared memory
     return;
@@ -511,7 +533,8 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
   // requests without keys: zeros, nothing to join
   for (int b = c; b < a.batch; b += gridDim.x) {
     if (tiles_of(b)) continue;
-    for (int i = tid; i < a.heads * D; i += NW * 32) finish(b, i / D, i % D, -INFINITY, 0.f, 0.f);
+    const float zero[E] = {};
+    for (int h = warp; h < a.heads; h += NW) finish(b, h, -INFINITY, 0.f, zero);
     for (int i = tid; i < per; i += NW * 32) a.cut[(int64_t)b * per + i] = make_int2(0, 0);
   }
 
@@ -545,37 +568,53 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
 
-  while (u < u_end) {
-    // the pair that u lies in
-    int lo, hi, g, h0, nh;
-    visible(a, b, lo, hi);
-    const int tiles = tiles_of(b);
-    if (tiles == 0) { ++b; continue; }
-    const int64_t u_b = before * per;
-    const int pair = (int)((u - u_b) / tiles);
-    if (pair >= per) { before += tiles; ++b; continue; }
-    heads_of(pair, g, h0, nh);
-    const int64_t u0 = u_b + (int64_t)pair * tiles;
-    const int t0 = (int)(u - u0), t1 = (int)min((int64_t)tiles, u_end - u0);
-    const bool whole = t0 == 0 && t1 == tiles;
-    u = u0 + t1;
-    attend(b, pair, lo, hi, g, h0, nh, t0, t1);
-    const int slot = t0 > 0 ? 0 : 1;
-    for (int i = tid; i < nh * D; i += NW * 32) {
-      const int h = i / D, e = i - h * D;
-      float M, L, x;
-      gather(h, e, M, L, x);
-      if (whole) {
-        finish(b, h0 + h, e, M, L, x);
-      } else {
-        const int64_t at = ((int64_t)c * 2 + slot) * HT + h;
-        a.part[at * D + e] = x;
-        if (e == 0) { a.stat[at * 2] = M; a.stat[at * 2 + 1] = L; }
+  // (the walk's state waits in shared memory while the registers serve a pair)
+  __shared__ struct { int64_t u, before; int b; } walk;
+  __shared__ struct { int b, h0, nh, slot; } now;  // slot -1: a whole pair
+  if (tid == 0) { walk.u = u; walk.before = before; walk.b = b; }
+  for (;;) {
+    __syncthreads();  // the last pair's shared memory is done with
+    u = walk.u;
+    if (u >= u_end) break;
+    before = walk.before;
+    b = walk.b;
+    int lo, hi, g, h0, nh, pair, tiles;
+    for (;;) {  // the pair that u lies in
+      tiles = tiles_of(b);
+      const int64_t past = u - before * per;
+      if (tiles && past < (int64_t)tiles * per) {
+        pair = (int)(past / tiles);
+        break;
       }
+      before += tiles;
+      ++b;
     }
-    if (t0 == 0 && tid == 0) {  // who holds the pair: CTA x has the tiles from x * share on
-      const int last = (int)((u0 + tiles - 1) / share);
-      a.cut[(int64_t)b * per + pair] = whole ? make_int2(0, 0) : make_int2(c, last - c + 1);
+    visible(a, b, lo, hi);
+    heads_of(pair, g, h0, nh);
+    const int64_t u0 = before * per + (int64_t)pair * tiles;
+    const int t0 = (int)(u - u0), t1 = (int)min((int64_t)tiles, u_end - u0);
+    peek(a.tables + b * a.ld, (lo & -KI) + t0 * TK + warp * KI);
+    queries(b, h0, nh);
+    __syncthreads();  // everyone has read the walk's state
+    if (tid == 0) {
+      const bool whole = t0 == 0 && t1 == tiles;
+      walk = {u0 + t1, before, b};
+      now = {b, h0, nh, whole ? -1 : t0 > 0 ? 0 : 1};
+      if (t0 == 0)  // who holds the pair: CTA x has the tiles from x * share on
+        a.cut[(int64_t)b * per + pair] = whole ? make_int2(0, 0) : make_int2(c, (int)((u0 + tiles - 1) / share) - c + 1);
+    }
+    attend(b, pair, lo, hi, g, t0, t1, 1);
+    float M, L, x[E];
+    gather(M, L, x);
+    if (warp < now.nh) {
+      if (now.slot < 0) {
+        finish(now.b, now.h0 + warp, M, L, x);
+      } else {
+        const int64_t at = ((int64_t)c * 2 + now.slot) * HT + warp;
+#pragma unroll
+        for (int e = 0; e < E; ++e) a.part[at * D + e * 32 + lane] = x[e];
+        if (lane == 0) { a.stat[at * 2] = M; a.stat[at * 2 + 1] = L; }
+      }
     }
   }
   }
