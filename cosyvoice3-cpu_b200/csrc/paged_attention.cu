@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
   constexpr int GK = UNI ? (KI >= 16 ? KI / 16 : 1) : NT;  // page lookups of a step: per 16 keys, or per 8 and row
   constexpr int QS = H16 ? D / 16 : D / 8, QW = H16 ? 2 : 4;  // steps of q.k, words of a lane's operand
   __shared__ __align__(16) uint32_t sq[QS][32][QW];  // q as product operands; H16: rows 0..7, else lower parts in 8..15
-  __shared__ float so[NW][HT][D];
+  __shared__ float so[NW][HT][D + 1];  // (rows apart by 1 bank: the 8 heads of a store fall into different ones)
   __shared__ float sm[NW][HT], sl[NW][HT];
   dep_wait();
   dep_release();
