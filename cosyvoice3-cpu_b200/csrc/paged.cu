@@ -51,15 +51,15 @@ __device__ __forceinline__ Sum2 block_scan(Sum2 v, Sum2* red, Sum2& total) {
   __syncthreads();
   if (lane == 31) red[wid] = v;
   __syncthreads();
-  Sum2 before = {0, 0};
-  total = {0, 0};
-  for (int w = 0; w < warps; ++w) {
-    if (w == wid) before = total;
-    total.x += red[w].x;
-    total.y += red[w].y;
+  Sum2 w = lane < warps ? red[lane] : Sum2{0, 0};  // every warp sums the warps' totals by itself
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, w.x, o), y = __shfl_up_sync(0xffffffffu, w.y, o);
+    if (lane >= o) { w.x += x; w.y += y; }
   }
-  v.x += before.x;
-  v.y += before.y;
+  total = {__shfl_sync(0xffffffffu, w.x, 31), __shfl_sync(0xffffffffu, w.y, 31)};
+  const int64_t bx = __shfl_sync(0xffffffffu, w.x, max(wid - 1, 0)), by = __shfl_sync(0xffffffffu, w.y, max(wid - 1, 0));
+  v.x += wid ? bx : 0;
+  v.y += wid ? by : 0;
   return v;
 }
 
