@@ -245,8 +245,8 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
   // Tiles t0, t0 + every, ... below t1 of a pair (the first's entries peeked at): the warps' maxima, sums and
   // unnormalised outputs to shared memory.  The queries are there, but for the barrier.
   auto attend = [&](int b, int pair, int lo, int hi, int g, int t0, int t1, int every) {
-    const KT* kb = static_cast<const KT*>(a.k) + g * a.ksh;
-    const KT* vb = static_cast<const KT*>(a.v) + g * a.vsh;
+    const KT* kb = static_cast<const KT*>(a.k) + g * a.ksh + t * KE + (UNI ? n * a.kst : 0);
+    const KT* vb = static_cast<const KT*>(a.v) + g * a.vsh + n * VE + (UNI ? 2 * t * a.vst : 0);
     const int* table = a.tables + b * a.ld;
     const bool counts = a.bad && pair == 0;
     float o[D / 8][2], m = -INFINITY, l = 0.f;
@@ -279,29 +279,55 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
       }
     };
     auto row_of = [&](int key) -> int { return key - page_index(a, key) * a.ps; };
+    // UNI: kb and vb point at this lane's first row and piece of a 16-key group, which lies in one page
     auto load_k = [&](int key0) {
+      if constexpr (UNI) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const int key = key0 + i * 8 + n;
-        const int p = UNI ? pg[i / 2][0] : pg[i][0];
-        const bool ok = p >= 0 && key >= lo && key < hi;
-        const KT* src = kb + (int64_t)p * a.ksp + (int64_t)row_of(key) * a.kst + t * KE;
+        for (int x = 0; x < GK; ++x) {
+          const KT* src = kb + (int64_t)pg[x][0] * a.ksp + (int64_t)row_of(key0 + x * 16) * a.kst;
 #pragma unroll
-        for (int x = 0; x < KC; ++x) fetch(kr[i][x], src + x * 4 * KE, ok);
+          for (int i = 0; i < (NT < 2 ? NT : 2); ++i) {
+            const int key = key0 + x * 16 + i * 8 + n;
+            const bool ok = pg[x][0] >= 0 && key >= lo && key < hi;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) fetch(kr[2 * x + i][c], src + i * 8 * a.kst + c * 4 * KE, ok);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const int key = key0 + i * 8 + n;
+          const KT* src = kb + (int64_t)pg[i][0] * a.ksp + (int64_t)row_of(key) * a.kst;
+#pragma unroll
+          for (int c = 0; c < KC; ++c) fetch(kr[i][c], src + c * 4 * KE, pg[i][0] >= 0);
+        }
       }
     };
     auto load_v = [&](int key0) {
+      if constexpr (UNI) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
+        for (int x = 0; x < GK; ++x) {
+          const KT* src = vb + (int64_t)pg[x][0] * a.vsp + (int64_t)row_of(key0 + x * 16) * a.vst;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int key = key0 + i * 8 + 2 * t + r;
-          const int p = UNI ? pg[i / 2][0] : pg[i][1 + r];
-          const bool ok = p >= 0 && key >= lo && key < hi;
-          const KT* src = vb + (int64_t)p * a.vsp + (int64_t)row_of(key) * a.vst + n * VE;
+          for (int i = 0; i < (NT < 2 ? NT : 2); ++i)
 #pragma unroll
-          for (int x = 0; x < VC; ++x) fetch(vr[i][r][x], src + x * 8 * VE, ok);
+            for (int r = 0; r < 2; ++r) {
+              const int key = key0 + x * 16 + i * 8 + 2 * t + r;
+              const bool ok = pg[x][0] >= 0 && key >= lo && key < hi;
+#pragma unroll
+              for (int c = 0; c < VC; ++c) fetch(vr[2 * x + i][r][c], src + (i * 8 + r) * a.vst + c * 8 * VE, ok);
+            }
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int key = key0 + i * 8 + 2 * t + r;
+            const KT* src = vb + (int64_t)pg[i][1 + r] * a.vsp + (int64_t)row_of(key) * a.vst;
+#pragma unroll
+            for (int c = 0; c < VC; ++c) fetch(vr[i][r][c], src + c * 8 * VE, pg[i][1 + r] >= 0);
+          }
       }
     };
 
