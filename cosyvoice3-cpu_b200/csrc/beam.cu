@@ -8,7 +8,8 @@
 // keys in 64 bits.  A CTA reads its chunk of a row in tiles of 512 logits, once for the sum and the
 // tiles' maxima; the K-th largest of these maxima bounds the K-th logit from below, so only the tiles
 // that reach it -- K of them, but for ties -- are read again (from L2) for candidates.  (Lists kept
-// while reading cost more than all the rest: 32 x 8 rows over 151936 tokens took 94 us.)
+// while reading cost more than all the rest: 32 x 8 rows over 151936 tokens, 156 MB, took 94 us; so they
+// take 48 us, 3.2 TB/s: the sum's arithmetic and the waits of the two readings bound it.)
 //
 // Precision: candidates of different hypotheses may lie closer than fp32 resolves, so the log-sum-exp
 // is held to about 2e-8.  Terms within e^-2 of the running maximum are evaluated in 64 bits; the
@@ -479,12 +480,15 @@ __global__ void __launch_bounds__(BT) beam_cluster_kernel(const BeamArgs a, int 
   if (rank == 0) choose<T>(a, g, work);
 }
 
-// How a call is cut.  One launch where every warp of a cluster then walks at most CLUSTER_TILES tiles
-// of its group; else two, with chunks enough for four CTAs on every SM, a tile per warp at least.
+// How a call is cut.  One launch with a cluster per group where every warp then walks few tiles -- 4, or
+// 16 if the groups' clusters fill the GPU --, else two, with chunks for four CTAs on every SM and a tile
+// per warp at least.  Measured, one / two launches (fp32, us): 4 hypotheses of 6761 tokens 9.9 / 10.2, 32 x
+// 8 of them 14.0 / 22.3; 4 of 50000 15.9 / 14.0, of 151936 28.8 / 16.6.  (Chunks for three or eight CTAs
+// instead of four: 60 and 52 instead of 47 us for 32 x 8 rows of 151936.)
 struct Plan {
   int64_t cluster, chunks, tiles, bytes;  // cluster 0: two launches; bytes of results
 };
-constexpr int64_t CLUSTER = 8, CLUSTER_TILES = 16;  // (at most 32 tasks: 9 KB of results in shared memory)
+constexpr int64_t CLUSTER = 8, CLUSTER_TILES = 4, CLUSTER_TILES_FULL = 16;  // (at most 32 tasks: 9 KB of results)
 
 Plan plan_of(int64_t groups, int64_t beams, int64_t vocab) {
   Plan p = {};
@@ -494,7 +498,8 @@ Plan plan_of(int64_t groups, int64_t beams, int64_t vocab) {
     p.tiles = (std::max<int64_t>(1, (row + chunks - 1) / chunks) + BW - 1) / BW * BW;
     p.chunks = (row + p.tiles - 1) / p.tiles;
   };
-  if (beams * ((row + BW - 1) / BW) <= CLUSTER * CLUSTER_TILES) {
+  const int64_t most = groups * CLUSTER >= cv3::sm_count() ? CLUSTER_TILES_FULL : CLUSTER_TILES;
+  if (beams * ((row + BW - 1) / BW) <= CLUSTER * most) {
     cut(std::max<int64_t>(1, CLUSTER / beams));
     p.cluster = std::min<int64_t>(CLUSTER, beams * p.chunks);
     while (p.cluster & (p.cluster - 1)) ++p.cluster;  // a power of two
