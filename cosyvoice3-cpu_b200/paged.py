@@ -174,7 +174,7 @@ def paged_extend(lens, new_lens, block_tables, free_pages, free_count, page_size
     the next one in the same call.  ``free_pages[:free_count]`` is the stack of free page numbers
     (updated in place, as is ``block_tables``).  Requests are served in order; from the first whose
     pages, rows (``max_tokens`` over all) or table columns do not suffice on, none gets new tokens.
-    Returns a :class:`PagedStep`; ``out`` gives it its tensors (``out.lens`` may be ``lens`` and
+    Returns a :class:`PagedStep`, whose rows behind the last token have slot -1; ``out`` gives it its tensors (``out.lens`` may be ``lens`` and
     ``out.free_count`` may be ``free_count``: the state then advances in place).
     """
     if out is None and (_bound or _bind()):
@@ -184,6 +184,8 @@ def paged_extend(lens, new_lens, block_tables, free_pages, free_count, page_size
     name = "paged_extend"
     arrays = (lens, new_lens, block_tables, free_pages, free_count)
     d = _device(name, *(arrays if release is None else arrays + (release,)))
+    if len(lens.shape) != 1:
+        raise ValueError(f"{name}: lens must be (requests,), got {tuple(lens.shape)}")
     n, T = lens.shape[0], int(max_tokens)
     if page_size <= 0 or T < 0:
         raise ValueError(f"{name}: page_size {page_size}, max_tokens {max_tokens}")

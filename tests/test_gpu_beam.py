@@ -127,6 +127,38 @@ def test_synthesis_with_beams(small_weights):
     assert len(out.audio) == 960 * len(out.speech_tokens[0]) and np.isfinite(out.audio).all()
 
 
+def test_paged_cache_serves_requests_that_come_and_go():
+    """PagedKVCache over two layers: requests of unequal lengths admitted into the places of finished ones; each
+    one's attention equals the operator's over a cache that holds nothing else."""
+    import torch
+    ops = pkg("ops")
+    cache = pkg("models.paged").PagedKVCache(2, 2, 64, requests=4, max_len=64, pages=20, page_size=8)
+    rng = np.random.default_rng(3)
+    cos, sin = (torch.from_numpy(t).cuda() for t in pkg("models.qwen2").rope_tables(64, 64, 1e6))
+    rows = [[] for _ in range(4)]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for new, rel in (([20, 3, 0, 9], None), ([1, 1, 1, 1], None), ([1, 30, 1, 1], [0, 1, 0, 0]), ([1, 1, 1, 17], [0, 0, 1, 1])):
+        step = cache.extend(torch.tensor(new, **i32), sum(new) + 2, None if rel is None else torch.tensor(rel, **i32))
+        qkv = torch.from_numpy(rng.normal(size=(2, sum(new) + 2, 6 * 64)).astype(np.float32)).cuda()
+        q = [cache.append(layer, qkv[layer], step, 2, cos, sin) for layer in range(2)]
+        at = 0
+        for b in range(4):
+            rows[b] = ([] if rel and rel[b] else rows[b]) + [qkv[:, at + i] for i in range(new[b])]
+            at += new[b]
+        assert cache.lens.tolist() == [len(r) for r in rows]
+        for layer in range(2):
+            x = q[layer][:4].contiguous()
+            got = cache.attention(layer, x, 0.125)
+            for b in range(4):
+                n = len(rows[b])
+                alone = pkg("models.paged").PagedKVCache(1, 2, 64, requests=1, max_len=64, pages=8, page_size=8)
+                if n:
+                    s = alone.extend(torch.tensor([n], **i32), n)
+                    alone.append(0, torch.stack([r[layer] for r in rows[b]]), s, 2, cos, sin)
+                assert torch.equal(got[b:b + 1], alone.attention(0, x[b:b + 1], 0.125)), (layer, b)
+    assert int(cache.bad) == 0 and int(cache.free_count) == 20 - sum(-(-len(r) // 8) for r in rows)
+
+
 def test_beam_refusals(small_weights):
     W = small_weights["balanced"]
     lm, olm = _models(W)

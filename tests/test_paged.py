@@ -77,7 +77,7 @@ def test_extend_refusals(ops):
     for change in (dict(new_lens=_i32(2)), dict(lens=torch.zeros(3, dtype=torch.int64)), dict(block_tables=_i32(2, 5)),
                    dict(block_tables=_i32(5, 3).T), dict(free_count=_i32(2)), dict(page_size=0), dict(max_tokens=-1),
                    dict(release=_i32(4)), dict(lens=_i32(6)[::2]), dict(free_pages=torch.zeros(9)),
-                   dict(out=ops.PagedStep(*[_i32(4)] * 6)),
+                   dict(out=ops.PagedStep(*[_i32(4)] * 6)), dict(lens=torch.tensor(3, dtype=torch.int32)),
                    dict(block_tables=torch.zeros(3, 5))):
         with pytest.raises(ValueError):
             ops.paged_extend(**{**good, **change})
