@@ -71,8 +71,6 @@ __device__ __forceinline__ double unordered(u64 u) {
 // A hypothesis that nothing can continue: no (or NaN) score.
 __device__ __forceinline__ bool dead(float score) { return !(score > -INFINITY); }
 
-// Rows whose logits are not looked at: finished hypotheses and those that do not exist.
-__device__ __forceinline__ bool skipped(const BeamArgs& a, int64_t row) { return a.done[row] || dead(a.scores[row]); }
 
 // A candidate of the choice: ordered key, then lowest k * V + v.
 struct Cand {
@@ -132,16 +130,16 @@ struct Scratch {
   uint32_t bar;
 };
 
-// One task by the whole CTA.  A lane takes every 32nd logit of a tile, so rows may begin anywhere and
-// alike rows give the same bits wherever they lie; nothing depends on the warps' timing either.
+// One task by the whole CTA; false for rows whose logits do not count (finished hypotheses and those that
+// do not exist).  A lane takes every 32nd logit of a tile, so rows may begin anywhere and alike rows give
+// the same bits wherever they lie; nothing depends on the warps' timing either.
 // The result is in warp 0: list, and in every lane m and s.
 template <typename T>
-__device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh, u64& list, float& m, double& s) {
+__device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh, u64& list, float& m, double& s) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, K = a.beams;
   const T* logits = static_cast<const T*>(a.logits) + row * a.ld;
   const int begin = (int)(chunk * a.tiles * TILE);
   const int tiles = (int)((min((chunk + 1) * a.tiles * TILE, a.vocab) - begin + TILE - 1) / TILE);
-  const bool early = a.min_len && a.counts[row] < a.min_len[row / K] && a.stop_lo < a.stop_hi;
   float x[16];
   int v0 = 0;  // token of the lane's first logit; the others follow in steps of 32
   auto inside = [&](int e) -> bool { return v0 + e * 32 < a.vocab; };
@@ -174,11 +172,18 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
     return warp_max(top);
   };
 
+  // the first tile and the row's state on their way together
+  if (warp < tiles) fetch(warp);
+  const bool fin = a.done[row] != 0;
+  const float score = a.scores[row];
+  const int count_so_far = a.counts[row], least_count = a.min_len ? a.min_len[row / K] : 0;
+  if (fin || dead(score)) return false;
+  const bool early = a.min_len && count_so_far < least_count && a.stop_lo < a.stop_hi;
+
   // first reading: the sum of exp against a running maximum that begins with the first BW tiles', and
   // the tiles' maxima
   float wtop = -INFINITY;
   if (warp < tiles) {
-    fetch(warp);
     take(warp);
     wtop = maximum();
   }
@@ -320,6 +325,7 @@ __device__ void scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
     m = warp_max(mine);
     s = warp_sum_d(mine == -INFINITY ? 0.0 : sh.ss[lane] * (mine == m ? 1.0 : exp((double)mine - (double)m)));
   }
+  return true;
 }
 
 // score + log-probability of a token, from its logit, its row's largest and log(sum of exp against it)
@@ -329,39 +335,46 @@ __device__ __forceinline__ double continued(double base, float x, float top, dou
   return c == c ? c : -(double)INFINITY;  // (an infinite score and an impossible token)
 }
 
+// What the choice needs of a group's hypotheses, read while the logits are on their way.
+struct Group {
+  double base[CV3_MAX_BEAMS], norm[CV3_MAX_BEAMS], lsum[CV3_MAX_BEAMS];  // score, length's power, log of the sum
+  float tops[CV3_MAX_BEAMS];
+  int fins[CV3_MAX_BEAMS], lengths[CV3_MAX_BEAMS];  // 2: finished, 1: does not exist; length of a continuation
+};
+
+__device__ void prepare(const BeamArgs& a, int64_t g, Group& w) {
+  const int k = threadIdx.x;
+  if (k >= a.beams) return;
+  const int64_t row = g * a.beams + k;
+  const bool fin = a.done[row] != 0;
+  const float score = a.scores[row];
+  const int length = a.counts[row] + (fin ? 0 : 1);
+  w.base[k] = dead(score) ? -INFINITY : (double)score;
+  w.norm[k] = a.alpha == 0.0 ? 1.0 : pow((double)max(length, 1), a.alpha);
+  w.fins[k] = fin ? 2 : dead(score);
+  w.lengths[k] = length;
+}
+
 // The group's choice by one CTA, from its tasks' results (global or shared memory).
-template <typename T>
-__device__ void choose(const BeamArgs& a, int64_t g, const char* work) {
-  __shared__ double lsum[CV3_MAX_BEAMS], base[CV3_MAX_BEAMS], norm[CV3_MAX_BEAMS];
-  __shared__ float tops[CV3_MAX_BEAMS];
-  __shared__ int fins[CV3_MAX_BEAMS], lengths[CV3_MAX_BEAMS];
+__device__ void choose(const BeamArgs& a, int64_t g, const char* work, Group& w) {
   __shared__ Cand lists[BW][32];
   const int K = a.beams, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t tb = task_bytes(K);
   for (int k = warp; k < K; k += BW) {
-    const int64_t row = g * K + k;
-    const bool fin = a.done[row] != 0, skip = skipped(a, row);
+    if (w.fins[k]) continue;
+    const char* from = work + (int64_t)k * a.chunks * tb;
     float m = -INFINITY;
     double s = 0.0;
-    if (!skip) {
-      const char* w = work + (int64_t)k * a.chunks * tb;
-      for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, *reinterpret_cast<const float*>(w + c * tb + 8));
-      m = warp_max(m);
-      for (int c = lane; c < a.chunks; c += 32) {
-        const float t = *reinterpret_cast<const float*>(w + c * tb + 8);
-        if (t > -INFINITY) s += *reinterpret_cast<const double*>(w + c * tb) * (t == m ? 1.0 : exp((double)t - (double)m));
-      }
-      s = warp_sum_d(s);
+    for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, *reinterpret_cast<const float*>(from + c * tb + 8));
+    m = warp_max(m);
+    for (int c = lane; c < a.chunks; c += 32) {
+      const float t = *reinterpret_cast<const float*>(from + c * tb + 8);
+      if (t > -INFINITY) s += *reinterpret_cast<const double*>(from + c * tb) * (t == m ? 1.0 : exp((double)t - (double)m));
     }
+    s = warp_sum_d(s);
     if (lane == 0) {
-      const float sc = a.scores[row];
-      const int held = a.counts[row], n = max(held, 0) + (fin ? 0 : 1);
-      tops[k] = m;
-      lsum[k] = log(s);
-      base[k] = dead(sc) ? -INFINITY : (double)sc;
-      norm[k] = a.alpha == 0.0 ? 1.0 : pow((double)max(n, 1), a.alpha);
-      fins[k] = fin ? 2 : skip;
-      lengths[k] = held + (fin ? 0 : 1);
+      w.tops[k] = m;
+      w.lsum[k] = log(s);
     }
   }
   __syncthreads();
@@ -372,13 +385,13 @@ __device__ void choose(const BeamArgs& a, int64_t g, const char* work) {
     Cand c = {0, 0};
     if (i < all) {
       const int k = i / per, r = i - k * per;
-      if (fins[k]) {  // a finished one itself, then what stands in where nothing is left
+      if (w.fins[k]) {  // a finished one itself, then what stands in where nothing is left
         if (r < K && r < a.vocab)
-          c = Cand{ordered(r == 0 && fins[k] == 2 ? base[k] / norm[k] : -(double)INFINITY), ~(u64)(k * a.vocab + r)};
+          c = Cand{ordered(r == 0 && w.fins[k] == 2 ? w.base[k] / w.norm[k] : -(double)INFINITY), ~(u64)(k * a.vocab + r)};
       } else {
         const u64 u = *reinterpret_cast<const u64*>(work + (int64_t)(k * a.chunks + r / K) * tb + 16 + r % K * 8);
         if (u)
-          c = Cand{ordered(continued(base[k], unordered((uint32_t)(u >> 32)), tops[k], lsum[k]) / norm[k]),
+          c = Cand{ordered(continued(w.base[k], unordered((uint32_t)(u >> 32)), w.tops[k], w.lsum[k]) / w.norm[k]),
                    ~(u64)(k * a.vocab + (uint32_t)~(uint32_t)u)};
       }
     }
@@ -390,9 +403,9 @@ __device__ void choose(const BeamArgs& a, int64_t g, const char* work) {
   lists[warp][lane] = list;
   __syncthreads();
 #pragma unroll
-  for (int w = BW / 2; w > 0; w >>= 1) {
-    if (warp < w && w * 32 < all) {  // (warps beyond the candidates have empty lists)
-      list = merged(list, lists[warp + w][lane]);
+  for (int half = BW / 2; half > 0; half >>= 1) {
+    if (warp < half && half * 32 < all) {  // (warps beyond the candidates have empty lists)
+      list = merged(list, lists[warp + half][lane]);
       if (lane >= K) list = Cand{0, 0};
       lists[warp][lane] = list;
     }
@@ -402,14 +415,14 @@ __device__ void choose(const BeamArgs& a, int64_t g, const char* work) {
   const int64_t id = (int64_t)~list.tie;
   const int k = (int)(id / a.vocab);
   const int64_t v = id - (int64_t)k * a.vocab, to = g * K + lane;
-  const bool fin = fins[k] == 2;
+  const bool fin = w.fins[k] == 2;
   // the key times the length's power is the score again (to the last bits of 64); the outputs may be
   // the inputs' own buffers, of which nothing is read any more
-  const double cum = list.key > ordered(-(double)INFINITY) ? (fin ? base[k] : unordered(list.key) * norm[k]) : -(double)INFINITY;
+  const double cum = list.key > ordered(-(double)INFINITY) ? (fin ? w.base[k] : unordered(list.key) * w.norm[k]) : -(double)INFINITY;
   a.tokens[to] = fin ? 0 : v;
   a.parents[to] = k;
   a.scores_out[to] = (float)cum;
-  a.counts_out[to] = lengths[k];
+  a.counts_out[to] = w.lengths[k];
   a.done_out[to] = fin || (v >= a.stop_lo && v < a.stop_hi) ? 1 : 0;
 }
 
@@ -420,12 +433,10 @@ __global__ void __launch_bounds__(BT, 3) beam_scan_kernel(const BeamArgs a) {
   dep_wait();
   dep_release();
   const int64_t row = blockIdx.y;
-  if (skipped(a, row)) return;
   u64 list;
   float m;
   double s;
-  scan<T>(a, row, blockIdx.x, sh, list, m, s);
-  if (threadIdx.x < 32) {
+  if (scan<T>(a, row, blockIdx.x, sh, list, m, s) && threadIdx.x < 32) {
     char* w = a.work + (row * a.chunks + blockIdx.x) * task_bytes(a.beams);
     if (threadIdx.x < a.beams) reinterpret_cast<u64*>(w + 16)[threadIdx.x] = list;
     if (threadIdx.x == 0) {
@@ -435,12 +446,14 @@ __global__ void __launch_bounds__(BT, 3) beam_scan_kernel(const BeamArgs a) {
   }
 }
 
-template <typename T>
 __global__ void __launch_bounds__(BT) beam_pick_kernel(const BeamArgs a) {
+  __shared__ Group w;
   dep_wait();
   dep_release();
   const int64_t g = blockIdx.x;
-  choose<T>(a, g, a.work + g * a.beams * a.chunks * task_bytes(a.beams));
+  prepare(a, g, w);
+  __syncthreads();
+  choose(a, g, a.work + g * a.beams * a.chunks * task_bytes(a.beams), w);
 }
 
 __device__ __forceinline__ void put8(uint32_t at, u64 x) {
@@ -452,6 +465,7 @@ template <typename T>
 __global__ void __launch_bounds__(BT) beam_cluster_kernel(const BeamArgs a, int cluster) {
   extern __shared__ __align__(16) char work[];
   __shared__ Scratch sh;
+  __shared__ Group w;
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   dep_wait();
   dep_release();
@@ -460,14 +474,12 @@ __global__ void __launch_bounds__(BT) beam_cluster_kernel(const BeamArgs a, int 
   const int rank = blockIdx.x % cluster;
   uint32_t first;
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(first) : "r"((uint32_t)__cvta_generic_to_shared(work)));
+  if (rank == 0) prepare(a, g, w);
   for (int i = rank; i < a.beams * a.chunks; i += cluster) {
-    const int64_t row = g * a.beams + i / a.chunks;
-    if (skipped(a, row)) continue;
     u64 list;
     float m;
     double s;
-    scan<T>(a, row, i % a.chunks, sh, list, m, s);
-    if (threadIdx.x < 32) {
+    if (scan<T>(a, g * a.beams + i / a.chunks, i % a.chunks, sh, list, m, s) && threadIdx.x < 32) {
       const uint32_t at = first + (uint32_t)(i * task_bytes(a.beams));
       if (threadIdx.x < a.beams) put8(at + 16 + threadIdx.x * 8, list);
       if (threadIdx.x == 0) {
@@ -477,7 +489,7 @@ __global__ void __launch_bounds__(BT) beam_cluster_kernel(const BeamArgs a, int 
     }
   }
   cv3p::cluster_sync();
-  if (rank == 0) choose<T>(a, g, work);
+  if (rank == 0) choose(a, g, work, w);
 }
 
 // How a call is cut.  One launch with a cluster per group where every warp then walks few tiles -- 4, or
@@ -522,7 +534,7 @@ int launch(const BeamArgs& a, const Plan& plan, int64_t groups, cudaStream_t st)
   int rc = cv3::check_launch("beam_scan", cv3::launch_dep(beam_scan_kernel<T>, dim3((unsigned)plan.chunks, (unsigned)(groups * a.beams)),
                                                           dim3(BT), 0, st, a));
   if (rc) return rc;
-  return cv3::check_launch("beam_pick", cv3::launch_dep(beam_pick_kernel<T>, dim3((unsigned)groups), dim3(BT), 0, st, a));
+  return cv3::check_launch("beam_pick", cv3::launch_dep(beam_pick_kernel, dim3((unsigned)groups), dim3(BT), 0, st, a));
 }
 
 }  // namespace
