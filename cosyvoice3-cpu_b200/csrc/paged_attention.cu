@@ -28,8 +28,8 @@
 //
 // Measured: 64 requests of 1 to 16384 keys, 32 / 8 heads of 128, bf16 (2.15 GB): 344 us, 6.2 TB/s (390 us
 // when it runs on and on and the card's power limit lowers its clock); 32 of 64 to 1650 keys, 14 / 2
-// heads of 64, fp32 (28 MB): 14.4 us, of which the products, half of a step, and the chain length ->
-// table -> keys are most; one of 325 keys: 5.8 us.
+// heads of 64, fp32 (28 MB): 14.5 us, of which the products, half of a step, and the chain length ->
+// table -> keys are most; one of 325 keys: 6.0 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -168,6 +168,11 @@ __device__ __forceinline__ uint32_t element(const Raw<B>& x, int e) {
 __device__ __forceinline__ uint32_t tf32_rest(uint32_t x) {
   return __float_as_uint(__uint_as_float(x) - __uint_as_float(tf32_hi(x)));
 }
+// the same, rounded to the nearest tf32 by the pipe, which drops the low 13 bits (of an infinity: 0).  For
+// what goes into scores, whose errors the softmax multiplies by the score's own size, and for the
+// probabilities: the worst relative error of 1714 to 30000 keys falls from 1.5e-6 to 5.6e-7 of fp32's own 0.5
+// to 2.6e-6.  Values take the plain rest: rounded too 4.7e-7, but 2% slower.
+__device__ __forceinline__ uint32_t tf32_near(uint32_t x) { return tf32_rest(x) + 0x1000u; }
 __device__ __forceinline__ float or_zero(float x) { return x == x ? x : 0.f; }
 
 __device__ __forceinline__ int page_index(const AttnArgs& a, int key) {
@@ -222,9 +227,9 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float x = cv3p::load_any(a.q, a.q_type, at + d + e) * (a.scale * LOG2E);
-            const uint32_t r = __float_as_uint(or_zero(__uint_as_float(tf32_rest(__float_as_uint(x)))));
+            const uint32_t r = __float_as_uint(or_zero(__uint_as_float(tf32_near(__float_as_uint(x)))));
             v[2 * e] = tf32_hi(__float_as_uint(x));
-            v[2 * e + 1] = (r & 0x7FFFFFFFu) ? r : __float_as_uint(copysignf(TINY, x));
+            v[2 * e + 1] = (r & 0x7FFFE000u) ? r : __float_as_uint(copysignf(TINY, x));
           }
         }
         *reinterpret_cast<uint4*>(&sq[s][ln][0]) = make_uint4(v[0], v[1], v[2], v[3]);
@@ -375,7 +380,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
             const uint32_t b1 = element<KT>(kr[i][s / (KE / 2)], s % (KE / 2) * 2 + 1);
             if constexpr (WIDE) {
               mma_tf32(s0[i], qa, tf32_hi(b0), tf32_hi(b1));
-              mma_tf32(s1[i], qa, tf32_rest(b0), tf32_rest(b1));
+              mma_tf32(s1[i], qa, tf32_near(b0), tf32_near(b1));
             } else {
               mma_tf32(s & 1 ? s1[i] : s0[i], qa, b0, b1);
             }
@@ -437,7 +442,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             p[i][2 * r] = tf32_hi(__float_as_uint(pr[i][r]));
-            p[i][2 * r + 1] = __float_as_uint(fmaxf(pr[i][r] - __uint_as_float(p[i][2 * r]), TINY));
+            p[i][2 * r + 1] = __float_as_uint(fmaxf(pr[i][r] - __uint_as_float(p[i][2 * r]), TINY)) + 0x1000u;
           }
 #pragma unroll
         for (int j = 0; j < D / 8; ++j) {
