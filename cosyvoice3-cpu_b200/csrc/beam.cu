@@ -552,6 +552,9 @@ extern "C" int cv3_beam_select(const cv3_beam_params* p, void* stream) {
   CV3_REQUIRE(p->beams > 0 && p->beams <= CV3_MAX_BEAMS, CV3_ERR_UNSUPPORTED, "beam_select: %lld beams (1 to %d)",
               (long long)p->beams, CV3_MAX_BEAMS);
   CV3_REQUIRE(cv3p::type_ok(p->type), CV3_ERR_VALUE, "beam_select: unknown element type");
+  // (lengths to that power stay finite and above 0 in 64 bits)
+  CV3_REQUIRE(p->length_penalty >= -16.0 && p->length_penalty <= 16.0, CV3_ERR_VALUE,
+              "beam_select: length penalty %g (-16 to 16)", p->length_penalty);
   CV3_REQUIRE(p->groups <= 65535 && p->groups * p->beams <= 65535, CV3_ERR_UNSUPPORTED,
               "beam_select: more than 65535 hypotheses");
   CV3_REQUIRE((uintptr_t)p->logits % cv3p::type_size(p->type) == 0, CV3_ERR_VALUE, "beam_select: misaligned logits");

@@ -295,7 +295,7 @@ PyObject* beam(PyObject*, PyObject* const* args, Py_ssize_t) {
   cv3_beam_params p = {sizeof(p)};
   p.groups = x.size(0), p.beams = x.size(1), p.vocab = x.size(2);
   const int64_t n = p.groups * p.beams, shape[2] = {p.groups, p.beams};
-  c.need(n > 0 && p.vocab > 0 && x.stride(2) == 1 && (p.groups == 1 || x.stride(0) == p.beams * x.stride(1)) &&
+  c.need(n > 0 && p.vocab > 0 && x.stride(2) == 1 && (p.groups == 1 || p.beams == 1 || x.stride(0) == p.beams * x.stride(1)) &&
          alike(scores, shape, at::kFloat) && alike(counts, shape, at::kInt) && alike(done, shape, at::kInt));
   p.min_len = c.ints(5, p.groups, true);
   p.length_penalty = c.real(6);

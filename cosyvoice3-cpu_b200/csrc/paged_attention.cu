@@ -826,7 +826,7 @@ extern "C" int cv3_paged_attention(const cv3_paged_attention_params* p, void* st
   if (p->batch == 0) return CV3_OK;
   const int64_t max_len = p->max_blocks * p->page_size;
   const Plan plan = plan_of(p->batch, p->heads, p->kv_heads, d, es, max_len);
-  CV3_REQUIRE(plan.grid <= INT32_MAX, CV3_ERR_VALUE, "paged_attention: too many requests and heads");
+  CV3_REQUIRE(plan.grid <= INT32_MAX && plan.pairs <= INT32_MAX, CV3_ERR_VALUE, "paged_attention: too many requests and heads");
   CV3_REQUIRE(plan.floats == 0 || (p->workspace && p->workspace_floats >= plan.floats && ((uintptr_t)p->workspace & 7) == 0),
               CV3_ERR_VALUE, "paged_attention: the workspace must hold cv3_paged_attention_workspace() floats");
   // n / page_size by a product: with 2^(sh-1) < page_size <= 2^sh and mul = ceil(2^(31+sh) / page_size), the excess

@@ -231,6 +231,8 @@ class CosyVoice3LM:
             return []
         if not 1 <= K <= MAX_DECODE_BATCH or max_len < 1:
             raise ValueError(f"{beams} beams (1 to {MAX_DECODE_BATCH}) of up to {max_len} tokens (1 at least)")
+        if min(int(np.shape(p)[0]) for p in prompts) < 1:
+            raise ValueError("a prompt without tokens")
         mins = [int(min_len)] * B if np.ndim(min_len) == 0 else [int(m) for m in min_len]
         if len(mins) != B:
             raise ValueError(f"{len(mins)} minimum lengths for {B} prompts")

@@ -207,8 +207,8 @@ class BeamEngine:
         lens = [int(np.shape(p)[0]) for p in prompts]
         if len(prompts) != G or len(min_lens) != G:
             raise ValueError(f"{len(prompts)} prompts and {len(min_lens)} minimum lengths for {G} groups")
-        if max(lens) > self.max_prompt or not 1 <= max_len <= self.max_steps:
-            raise ValueError(f"prompts of up to {max(lens)} and {max_len} tokens in an engine for {self.max_prompt} and "
+        if min(lens) < 1 or max(lens) > self.max_prompt or not 1 <= max_len <= self.max_steps:
+            raise ValueError(f"prompts of {min(lens)} to {max(lens)} and {max_len} tokens in an engine for {self.max_prompt} and "
                              f"{self.max_steps}")
         # the prompts in one pass through a contiguous cache (freed afterwards), then into pages
         ps = self.cache.page_size

@@ -327,7 +327,7 @@ def beam_select(logits, scores, counts, done, stop: Optional[Tuple[int, int]] = 
 
     ``logits`` ``(groups, beams, vocab)``; ``scores`` (float32 sums of log-probabilities), ``counts``
     and ``done`` (int32) are ``(groups, beams)``.  A candidate's key is its new score divided by its
-    length to the power ``length_penalty``; the ``beams`` best of all ``beams * vocab`` are kept, equal
+    length to the power ``length_penalty`` (-16 to 16); the ``beams`` best of all ``beams * vocab`` are kept, equal
     keys in the order of the lower hypothesis and token.  A token in ``stop`` (first, end) finishes a
     hypothesis, and is no candidate while it has fewer than ``min_len[group]`` tokens; a finished one
     stays as it is (token 0).  A score of -inf marks a hypothesis that does not exist, as all but the
@@ -345,6 +345,8 @@ def beam_select(logits, scores, counts, done, stop: Optional[Tuple[int, int]] = 
         raise ValueError(f"{name}: logits must be (groups, beams, vocab), got {tuple(logits.shape)}")
     G, K, V = logits.shape
     sg, sk, sv = logits.stride()
+    if K == 1:
+        sk = sg
     if (V > 1 and sv != 1) or (G > 1 and sg != K * sk):
         raise ValueError(f"{name}: rows of logits must be contiguous and evenly spaced")
     n = G * K

@@ -494,7 +494,7 @@ int64_t cv3_paged_attention_workspace(int64_t batch, int64_t heads, int64_t kv_h
  * logits rows (g*beams + k) of `vocab` entries, ld apart.  Candidate (k, v) has the key
  * (scores[k] + log_softmax(logits[k])[v]) / (counts[k] + 1)^length_penalty; a done
  * hypothesis has one candidate, itself (token 0, key scores[k] / counts[k]^
- * length_penalty).  Tokens of [stop_lo, stop_hi) end a hypothesis; they are no
+ * length_penalty); length_penalty is from -16 to 16.  Tokens of [stop_lo, stop_hi) end a hypothesis; they are no
  * candidates while counts[k] < min_len[g] (min_len may be NULL).  NaN logits, and
  * hypotheses with a score of -inf or NaN, give no candidates.  The `beams` best keys
  * in descending order (equal keys: the lowest k*vocab + v; -inf keys where too few

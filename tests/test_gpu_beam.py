@@ -172,3 +172,14 @@ def test_beam_refusals(small_weights):
         eng.run([p, p], [0, 0], 5)
     with pytest.raises(ValueError):
         eng.run([p], [0], 257)
+
+
+def test_prompts_without_tokens_are_refused(small_weights):
+    W = small_weights["balanced"]
+    lm, olm = _models(W)
+    (p,), _ = _prompts(lm, olm, W, (4,), 1)
+    for prompts in ([p[:0]], [p, p[:0]]):
+        with pytest.raises(ValueError):
+            lm.generate_beam(prompts, 2, 5)
+    with pytest.raises(ValueError):
+        lm.beam_engine(1, 2, 256, 256, 16, None, 0.0).run([p[:0]], [0], 5)

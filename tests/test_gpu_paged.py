@@ -426,6 +426,18 @@ def _beam(logits, scores, counts, done, stop=None, min_len=None, alpha=0.0, act=
     return got
 
 
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_beam_one_hypothesis_of_several(act):
+    """A view of every group's third row: its rows are a group's logits apart."""
+    import torch
+    ops, rng = _ops(), np.random.default_rng(77)
+    x = _cuda(rng.normal(size=(3, 5, 1111)).astype(np.float32) * 3, _dt(act))
+    z, s = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.zeros(3, 1, device="cuda")
+    got, want = ops.beam_select(x[:, 2:3], s, z, z), ops.beam_select(x[:, 2:3].contiguous(), s, z, z)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(x[:, 2].gather(1, got.tokens)[:, 0], x[:, 2].amax(-1))
+
+
 def _state(rng, G, K, fin=0.2):
     counts = np.repeat(rng.integers(1, 30, (G, 1)), K, 1).astype(np.int32)
     done = (rng.random((G, K)) < fin).astype(np.int32)

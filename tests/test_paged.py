@@ -218,6 +218,33 @@ def test_c_entries_refuse_before_any_device_work():
         L.check(reorder(beams=33), "cv3_paged_reorder")
 
 
+def test_more_pairs_than_a_grid_holds():
+    L, p = pkg("_lib"), pkg("paged")
+    lib, at, H = L.load(), 1 << 20, 1 << 16
+    for batch in (1 << 15, 1 << 24):
+        block = p._ATTENTION.pack(p._ATTENTION.size, at, 0, 32, 32, at, at, 0, 512, 512, 32, 512, 512, 32, 9, 16, at, 1, 1, at,
+                                  batch, H, H, 32, 0, at, 32, 32, 0, 0, at, 1 << 60, 0.1)
+        assert lib.cv3_paged_attention(block, None) == L.CV3_ERR_VALUE
+        assert b"too many" in lib.cv3_last_error()
+
+
+@pytest.mark.parametrize("alpha", [float("nan"), float("inf"), -float("inf"), 16.5, -17.0])
+def test_length_penalties_whose_powers_leave_64_bits(alpha):
+    L, p = pkg("_lib"), pkg("paged")
+    lib = L.load()
+    block = p._BEAM.pack(p._BEAM.size, 0, 0, 100, 0, 4, 100, *[0] * 13, alpha)
+    assert lib.cv3_beam_select(block, None) == L.CV3_ERR_VALUE and b"length penalty" in lib.cv3_last_error()
+    for fine in (0.0, -16.0, 16.0):
+        assert lib.cv3_beam_select(p._BEAM.pack(p._BEAM.size, 0, 0, 100, 0, 4, 100, *[0] * 13, fine), None) == 0
+
+
+def test_one_hypothesis_of_several_is_evenly_spaced(ops):
+    import torch
+    one = dict(logits=torch.zeros(3, 5, 50)[:, 2:3], scores=torch.zeros(3, 1), counts=_i32(3, 1), done=_i32(3, 1))
+    with pytest.raises(AssertionError, match="accepted"):
+        ops.beam_select(**one)
+
+
 def test_oracle_extend_and_reorder_by_hand():
     """The restatement itself on cases small enough to write down."""
     t = np.array([[4, -1], [5, 6]], np.int32)
