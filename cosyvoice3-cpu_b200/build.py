@@ -68,7 +68,7 @@ def _bind(src: str, force: bool) -> None:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=1",
            "-I", os.path.join(torch_dir, "include"), "-I", os.path.join(cuda, "include"),
            "-I", sysconfig.get_paths()["include"], src, "-o", out, "-L", os.path.join(torch_dir, "lib"),
-           "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
+           "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {os.path.basename(src)}:\n{r.stdout}\n{r.stderr}")

@@ -8,12 +8,14 @@
 // the library.
 #include <Python.h>
 
-#include <ATen/ops/empty.h>
+#include <ATen/core/Tensor.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <utility>
 
 #include "../../../include/cv3cuda.h"
 
@@ -130,12 +132,27 @@ bool alike(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
   return t.sizes() == sizes && t.scalar_type() == type && t.is_contiguous();
 }
 
+// A contiguous uninitialised tensor, and n elements of one from `at` on (past the dispatcher, whose 0.4 us a
+// tensor are a third of such a call).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+Tensor part_of(const Tensor& all, int64_t at, int64_t n) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(at);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
+// an instance of a named tuple class, as its _make gives it
 PyObject* made(PyObject* cls, std::initializer_list<Tensor> parts) {
-  PyObject* v[8];
-  size_t n = 0;
-  for (const Tensor& t : parts) v[n++] = THPVariable_Wrap(t);
-  PyObject* r = PyObject_Vectorcall(cls, v, n, nullptr);
-  for (size_t i = 0; i < n; ++i) Py_DECREF(v[i]);
+  PyObject* v = PyTuple_New((Py_ssize_t)parts.size());
+  Py_ssize_t n = 0;
+  for (const Tensor& t : parts) PyTuple_SET_ITEM(v, n++, THPVariable_Wrap(t));
+  PyObject* args = PyTuple_Pack(1, v);
+  PyObject* r = PyTuple_Type.tp_new(reinterpret_cast<PyTypeObject*>(cls), args, nullptr);
+  Py_DECREF(args);
+  Py_DECREF(v);
   return r;
 }
 
@@ -159,14 +176,9 @@ PyObject* extend(PyObject*, PyObject* const* args, Py_ssize_t) {
   p.release = c.ints(7, p.batch, true);
   const int64_t T = p.max_tokens, n = p.batch;
   if (!c.ok || T < 0 || T > INT32_MAX) Py_RETURN_NONE;
-  const Tensor slots = at::empty({T}, lens.options().dtype(at::kLong));
-  const Tensor all = at::empty({2 * T + 3 * n + 3}, lens.options());
+  const Tensor slots = fresh({T}, at::kLong, lens), all = fresh({2 * T + 3 * n + 3}, at::kInt, lens);
   int64_t at = 0;
-  auto part = [&](int64_t m) {
-    const Tensor t = all.as_strided({m}, {1}, at);
-    at += m;
-    return t;
-  };
+  auto part = [&](int64_t m) { return part_of(all, std::exchange(at, at + m), m); };
   const Tensor seq = part(T), pos = part(T), offsets = part(n + 1), lens_out = part(n), count = part(1);
   p.slots = slots.data_ptr<int64_t>();
   p.seq = seq.data_ptr<int>();
@@ -213,7 +225,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t) {
   if (!c.ok) Py_RETURN_NONE;
   Tensor out;
   if (c.none(8)) {
-    out = at::empty({p.rows, p.heads, p.head_dim}, qkv.options());
+    out = fresh({p.rows, p.heads, p.head_dim}, qkv.scalar_type(), qkv);
   } else {
     out = c.tensor(8);
     if (!c.ok || !alike(out, {p.rows, p.heads, p.head_dim}, qkv.scalar_type())) Py_RETURN_NONE;
@@ -251,7 +263,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t) {
   if (!c.ok) Py_RETURN_NONE;
   Tensor out;
   if (c.none(7)) {
-    out = at::empty({p.batch, p.heads, p.head_dim}, q.options());
+    out = fresh({p.batch, p.heads, p.head_dim}, q.scalar_type(), q);
   } else {
     out = c.tensor(7);
     if (!c.ok || !alike(out, q.sizes(), q.scalar_type())) Py_RETURN_NONE;
@@ -260,7 +272,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t) {
   if (!want_lse && args[8] != Py_False) Py_RETURN_NONE;
   Tensor lse, ws;
   if (want_lse) {
-    lse = at::empty({p.batch, p.heads}, q.options().dtype(at::kFloat));
+    lse = fresh({p.batch, p.heads}, at::kFloat, q);
     p.lse = lse.data_ptr<float>();
   }
   p.q = q.data_ptr();
@@ -275,7 +287,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t) {
   p.workspace_floats = cv3.attention_workspace(p.batch, p.heads, p.kv_heads, p.head_dim, (int)p.kv_type,
                                                p.max_blocks * p.page_size);
   if (p.workspace_floats) {
-    ws = at::empty({p.workspace_floats}, q.options().dtype(at::kFloat));
+    ws = fresh({p.workspace_floats}, at::kFloat, q);
     p.workspace = ws.data_ptr<float>();
   }
   if (cv3.attention(&p, c.stream())) Py_RETURN_NONE;
@@ -310,15 +322,14 @@ PyObject* beam(PyObject*, PyObject* const* args, Py_ssize_t) {
   p.type = type_of(x);
   p.ld = n == 1 ? p.vocab : p.beams > 1 ? x.stride(1) : x.stride(0);
   p.scores = scores.data_ptr<float>(), p.counts = counts.data_ptr<int>(), p.done = done.data_ptr<int>();
-  const Tensor tokens = at::empty(shape, counts.options().dtype(at::kLong)), parents = at::empty(shape, counts.options()),
-               s = at::empty(shape, scores.options()), cnt = at::empty(shape, counts.options()),
-               fin = at::empty(shape, counts.options());
+  const Tensor tokens = fresh(shape, at::kLong, x), parents = fresh(shape, at::kInt, x), s = fresh(shape, at::kFloat, x),
+               cnt = fresh(shape, at::kInt, x), fin = fresh(shape, at::kInt, x);
   p.tokens = tokens.data_ptr<int64_t>(), p.parents = parents.data_ptr<int>(), p.scores_out = s.data_ptr<float>();
   p.counts_out = cnt.data_ptr<int>(), p.done_out = fin.data_ptr<int>();
   p.workspace_bytes = cv3.beam_workspace(p.groups, p.beams, p.vocab);
   Tensor ws;
   if (p.workspace_bytes) {
-    ws = at::empty({p.workspace_bytes / 8}, tokens.options());
+    ws = fresh({p.workspace_bytes / 8}, at::kLong, x);
     p.workspace = ws.data_ptr();
   }
   if (cv3.beam(&p, c.stream())) Py_RETURN_NONE;
