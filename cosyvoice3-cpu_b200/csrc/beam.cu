@@ -120,9 +120,15 @@ __device__ __forceinline__ float exp_far(float d) {
   return y;
 }
 
+__device__ __forceinline__ float warp_top(float x) {  // of values that are not NaN
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // The CTA's shared memory for a task.
 struct Scratch {
-  u64 held[BW][64];  // candidates on their way into a warp's list
+  u64 held[BW][64];  // near terms (logit, how many << 32), then candidates on their way into a warp's list
   u64 lists[BW][32];
   double ss[BW];
   float ms[BW];
@@ -169,7 +175,7 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
     float top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
-    return warp_max(top);
+    return top;
   };
 
   // the first tile and the row's state on their way together
@@ -182,11 +188,24 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
 
   // first reading: the sum of exp against a running maximum that begins with the first BW tiles', and
   // the tiles' maxima
-  float wtop = -INFINITY;
+  float mine = -INFINITY, wtop = -INFINITY;  // the tile's maximum in this lane and in the warp
   if (warp < tiles) {
     take(warp);
-    wtop = maximum();
+    mine = maximum();
+    wtop = warp_top(mine);
   }
+  u64* held = sh.held[warp];
+  int count = 0;
+  auto add_near = [&]() {  // the first 32 of the near terms
+    __syncwarp();
+    const u64 u = lane < count ? held[lane] : 0ull, rest = lane + 32 < count ? held[lane + 32] : 0ull;
+    __syncwarp();
+    held[lane] = rest;
+    __syncwarp();
+    count = max(count - 32, 0);
+    const float y = __uint_as_float((uint32_t)u);
+    if (u) s += (double)(uint32_t)(u >> 32) * (y == m ? 1.0 : exp((double)y - (double)m));  // (m may be infinite)
+  };
   __syncthreads();  // (the last task's shared memory is done with)
   if (lane == 0) sh.ms[warp] = wtop;
   __syncthreads();
@@ -205,31 +224,35 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
       allowed = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 16; ++e) allowed = stopped(e) ? allowed : fmaxf(allowed, x[e]);
-      allowed = warp_max(allowed);
+      allowed = warp_top(allowed);
     }
     if (lane == 0) sh.tops[tile] = ordered(allowed);
     if (m > -INFINITY) {
-      const bool close = wtop >= m - NEAR;
-      unsigned near = 0;
-      if (close) {
+      // the lane's largest, as long as it is near, leaves the tile for the queue of near terms: 32 of them
+      // take one evaluation in 64 bits
+      const float bound = m - NEAR;
+      for (unsigned who; (who = __ballot_sync(0xffffffffu, mine >= bound)) != 0;) {
+        const bool near = mine >= bound;
+        unsigned alike = 0;
+        if (near) {
+          float next = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) near |= (x[e] >= m - NEAR ? 1u : 0u) << e;
-        for (unsigned left = near; __any_sync(0xffffffffu, left != 0); left &= left - 1) {
-          float y = -INFINITY;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) y = (left & (0u - left)) == 1u << e ? x[e] : y;
-          if (left) s += y == m ? 1.0 : exp((double)y - (double)m);  // (m may be infinite)
+          for (int e = 0; e < 16; ++e) {
+            const bool it = x[e] == mine;
+            alike += it;
+            x[e] = it ? -INFINITY : x[e];
+            next = fmaxf(next, x[e]);
+          }
+          held[count + __popc(who & ((1u << lane) - 1u))] = (u64)alike << 32 | __float_as_uint(mine);
+          mine = next;
         }
+        count += __popc(who);
+        if (count >= 32) add_near();
       }
       auto rest = [&]() -> float {
         float t[16];
-        if (close) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) t[e] = near >> e & 1u ? 0.f : exp_far(x[e] - m);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) t[e] = exp_far(x[e] - m);
-        }
+        for (int e = 0; e < 16; ++e) t[e] = exp_far(x[e] - m);
 #pragma unroll
         for (int w = 8; w > 0; w >>= 1)
 #pragma unroll
@@ -246,9 +269,11 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
     tile += BW;
     if (tile < tiles) {
       take(tile);
-      wtop = maximum();
+      mine = maximum();
+      wtop = warp_top(mine);
     }
   }
+  if (count) add_near();
   __syncthreads();
 
   // the bar: the K-th largest of the tiles' maxima (none where there are fewer tiles)
@@ -266,8 +291,8 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
   // second reading: what reaches the bar, merged into the warp's list 32 at a time
   const uint32_t bar = sh.bar;
   const float least = bar ? unordered(bar) : -INFINITY;
-  u64* held = sh.held[warp];
-  int count = 0, turn = 0;
+  int turn = 0;
+  count = 0;
   bool listed = false;
   list = 0;
   auto flush = [&]() {
@@ -275,6 +300,7 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
     const u64 key = lane < count ? held[lane] : 0ull, rest = lane + 32 < count ? held[lane + 32] : 0ull;
     __syncwarp();
     held[lane] = rest;
+    __syncwarp();
     count = max(count - 32, 0);
     list = listed ? merged(list, sorted(key)) : sorted(key);
     listed = true;
@@ -287,10 +313,10 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
       fetch(t0 + __ffs(reach) - 1);
       take(t0 + __ffs(reach) - 1);
       no_nan();
-      unsigned mine = 0;
+      unsigned fits = 0;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mine |= (x[e] >= least && inside(e) ? 1u : 0u) << e;
-      for (unsigned left = __reduce_or_sync(0xffffffffu, mine); left; left &= left - 1) {
+      for (int e = 0; e < 16; ++e) fits |= (x[e] >= least && inside(e) ? 1u : 0u) << e;
+      for (unsigned left = __reduce_or_sync(0xffffffffu, fits); left; left &= left - 1) {
         const int e = __ffs(left) - 1;
         float y = 0.f;
 #pragma unroll
@@ -298,7 +324,7 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
         if (early && stopped(e)) y = -INFINITY;
         const u64 key = (u64)ordered(y) << 32 | (uint32_t)~(uint32_t)(v0 + e * 32);
         const u64 last = from_lane(list, K - 1);  // (by all lanes: not within a condition)
-        const bool pass = (mine >> e & 1u) && y >= least && key > last;
+        const bool pass = (fits >> e & 1u) && y >= least && key > last;
         const unsigned who = __ballot_sync(0xffffffffu, pass);
         if (pass) held[count + __popc(who & ((1u << lane) - 1u))] = key;
         count += __popc(who);
@@ -321,9 +347,9 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
     __syncthreads();
   }
   if (warp == 0) {
-    const float mine = lane < BW ? sh.ms[lane] : -INFINITY;
-    m = warp_max(mine);
-    s = warp_sum_d(mine == -INFINITY ? 0.0 : sh.ss[lane] * (mine == m ? 1.0 : exp((double)mine - (double)m)));
+    const float top = lane < BW ? sh.ms[lane] : -INFINITY;
+    m = warp_max(top);
+    s = warp_sum_d(top == -INFINITY ? 0.0 : sh.ss[lane] * (top == m ? 1.0 : exp((double)top - (double)m)));
   }
   return true;
 }
