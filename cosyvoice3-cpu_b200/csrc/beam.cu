@@ -404,27 +404,34 @@ __device__ void choose(const BeamArgs& a, int64_t g, const char* work, Group& w)
     }
   }
   __syncthreads();
+  // A task's candidates are in descending order, so a warp takes its tasks' first ones before the next ones and
+  // stops when none is among its best K: `ranks` of every task at a time, as many as 256 lanes hold.
   Cand list = {0, 0};
-  const int per = a.chunks * K, all = per * K;
+  const int tasks = a.chunks * K, ranks = max(1, min(K, BT / tasks)), all = tasks * ranks;
+  bool first = true;
   for (int i0 = warp * 32; i0 < all; i0 += BT) {
-    const int i = i0 + lane;
-    Cand c = {0, 0};
-    if (i < all) {
-      const int k = i / per, r = i - k * per;
-      if (w.fins[k]) {  // a finished one itself, then what stands in where nothing is left
-        if (r < K && r < a.vocab)
-          c = Cand{ordered(r == 0 && w.fins[k] == 2 ? w.base[k] / w.norm[k] : -(double)INFINITY), ~(u64)(k * a.vocab + r)};
-      } else {
-        const u64 u = *reinterpret_cast<const u64*>(work + (int64_t)(k * a.chunks + r / K) * tb + 16 + r % K * 8);
-        if (u)
-          c = Cand{ordered(continued(w.base[k], unordered((uint32_t)(u >> 32)), w.tops[k], w.lsum[k]) / w.norm[k]),
-                   ~(u64)(k * a.vocab + (uint32_t)~(uint32_t)u)};
-      }
+    const int task = (i0 + lane) / ranks, k = min(task / a.chunks, K - 1);
+    const int fin = w.fins[k];
+    const bool scanned = task < tasks && !fin, alone = task < tasks && fin && task == k * a.chunks;
+    const u64* from = reinterpret_cast<const u64*>(work + (int64_t)task * tb + 16);
+    int r = (i0 + lane) % ranks;
+    u64 u = scanned && r < K ? from[r] : 0ull;
+    for (int r0 = 0; r0 < K; r0 += ranks) {
+      const u64 next = scanned && r + ranks < K ? from[r + ranks] : 0ull;
+      Cand c = {0, 0};
+      if (u)
+        c = Cand{ordered(continued(w.base[k], unordered((uint32_t)(u >> 32)), w.tops[k], w.lsum[k]) / w.norm[k]),
+                 ~(u64)(k * a.vocab + (uint32_t)~(uint32_t)u)};
+      else if (alone && r < K && r < a.vocab)  // a finished one itself, then what stands in where nothing is left
+        c = Cand{ordered(r == 0 && fin == 2 ? w.base[k] / w.norm[k] : -(double)INFINITY), ~(u64)(k * a.vocab + r)};
+      u = next;
+      r += ranks;
+      const Cand last = from_lane(list, K - 1);
+      if (!__any_sync(0xffffffffu, better(c, last))) break;
+      list = first ? sorted(c) : merged(list, sorted(c));
+      first = false;
+      if (lane >= K) list = Cand{0, 0};
     }
-    const Cand last = from_lane(list, K - 1);
-    if (!__any_sync(0xffffffffu, better(c, last))) continue;
-    list = i0 < BT ? sorted(c) : merged(list, sorted(c));
-    if (lane >= K) list = Cand{0, 0};
   }
   lists[warp][lane] = list;
   __syncthreads();
