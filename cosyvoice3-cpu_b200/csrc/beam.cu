@@ -6,10 +6,10 @@
 // Bound by the logits' bytes.  Within a hypothesis the key grows with the logit, so a row gives its K
 // largest logits (lowest token on ties) and its log-sum-exp; the K * K candidates are then ordered by
 // keys in 64 bits.  A CTA reads its chunk of a row in tiles of 512 logits, once for the sum and the
-// tiles' maxima; the K-th largest of these maxima bounds the K-th logit from below, so only the tiles
-// that reach it -- K of them, but for ties -- are read again (from L2) for candidates.  (Lists kept
+// tiles' maxima; the K-th largest of these maxima (with fewer than K tiles: of the lanes') bounds the K-th logit from
+// below, so only the tiles that reach it -- at most K, but for ties -- are read again (from L2) for candidates.  (Lists kept
 // while reading cost more than all the rest: 32 x 8 rows over 151936 tokens, 156 MB, took 94 us; so they
-// take 48 us, 3.2 TB/s: the sum's arithmetic and the waits of the two readings bound it.)
+// take 41 us, 3.8 TB/s: the sum's arithmetic and the waits of the two readings bound it.)
 //
 // Precision: candidates of different hypotheses may lie closer than fp32 resolves, so the log-sum-exp
 // is held to about 2e-8.  Terms within e^-2 of the running maximum are evaluated in 64 bits; the
@@ -213,20 +213,28 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
   s = 0.0;
 #pragma unroll
   for (int w = 0; w < BW; ++w) m = fmaxf(m, sh.ms[w]);
+  // too few maxima to bound the K-th logit: the lanes' serve (32 of 151936 tokens in chunks of 24 tiles: 46 us
+  // instead of 63, where all were candidates)
+  const bool few = tiles < K;
+  u64 best = 0;
   for (int tile = warp; tile < tiles;) {
     if (tile + BW < tiles) fetch(tile + BW);  // on its way while this one is worked on
     if (wtop > m) {
       if (s != 0.0) s *= exp((double)m - (double)wtop);
       m = wtop;
     }
-    float allowed = wtop;
+    float mine_allowed = mine, allowed = wtop;
     if (early && v0 - lane < a.stop_hi && v0 - lane + TILE > a.stop_lo) {
-      allowed = -INFINITY;
+      mine_allowed = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) allowed = stopped(e) ? allowed : fmaxf(allowed, x[e]);
-      allowed = warp_top(allowed);
+      for (int e = 0; e < 16; ++e) mine_allowed = stopped(e) ? mine_allowed : fmaxf(mine_allowed, x[e]);
+      allowed = warp_top(mine_allowed);
     }
     if (lane == 0) sh.tops[tile] = ordered(allowed);
+    if (few) {
+      const u64 key = ordered(mine_allowed);
+      best = tile == warp ? sorted(key) : merged(best, sorted(key));
+    }
     if (m > -INFINITY) {
       // the lane's largest, as long as it is near, leaves the tile for the queue of near terms: 32 of them
       // take one evaluation in 64 bits
@@ -274,14 +282,18 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
     }
   }
   if (count) add_near();
+  if (few) sh.lists[warp][lane] = best;
   __syncthreads();
 
-  // the bar: the K-th largest of the tiles' maxima (none where there are fewer tiles)
+  // the bar: the K-th largest of the tiles' maxima, or of the lanes'
   if (warp == 0) {
-    u64 best = 0;
-    for (int i = 0; i < tiles; i += 32) {
-      const u64 key = i + lane < tiles ? (u64)sh.tops[i + lane] : 0ull;
-      if (__any_sync(0xffffffffu, key > from_lane(best, K - 1))) best = i ? merged(best, sorted(key)) : sorted(key);
+    if (few) {
+      for (int w = 1; w < min(tiles, BW); ++w) best = merged(best, sh.lists[w][lane]);
+    } else {
+      for (int i = 0; i < tiles; i += 32) {
+        const u64 key = i + lane < tiles ? (u64)sh.tops[i + lane] : 0ull;
+        if (__any_sync(0xffffffffu, key > from_lane(best, K - 1))) best = i ? merged(best, sorted(key)) : sorted(key);
+      }
     }
     const uint32_t bar = (uint32_t)from_lane(best, K - 1);
     if (lane == 0) sh.bar = bar;
@@ -526,13 +538,19 @@ __global__ void __launch_bounds__(BT) beam_cluster_kernel(const BeamArgs a, int 
 }
 
 // How a call is cut.  One launch with a cluster per group where every warp then walks few tiles -- 4, or
-// 16 if the groups' clusters fill the GPU --, else two, with chunks for four CTAs on every SM and a tile
-// per warp at least.  Measured, one / two launches (fp32, us): 4 hypotheses of 6761 tokens 9.9 / 10.2, 32 x
-// 8 of them 14.0 / 22.3; 4 of 50000 15.9 / 14.0, of 151936 28.8 / 16.6.  (Chunks for three or eight CTAs
-// instead of four: 60 and 52 instead of 47 us for 32 x 8 rows of 151936.)
+// 16 if the groups' clusters fill the GPU --, else two, measured (one / two, fp32, us): 4 hypotheses of 6761
+// tokens 8.8 / 9.5, 32 x 8 of them 12.7 / 21.7; 4 of 50000 13.5 / 11.9, of 151936 24.0 / 11.9.
+//
+// Two launches: as many chunks as one wave of three CTAs on every SM takes, or one more that overshoots it by
+// at most a third of a chunk's share, since finished rows leave their CTAs early (32 x 8 rows of 151936, chunks
+// 1 / 2 / 3: 52 / 41 / 50 us with a seventh of the rows finished, 52 / 58 / 52 with none; 16 x 8, chunks 3 / 4:
+// 31 / 36 us).  But a chunk has 8 + 2 K tiles: the bar takes K maxima, and every chunk gives the second
+// launch K candidates (151936 tokens, such chunks against the wave's: 8 hypotheses 14.9 / 18.6 us, 32 of them
+// 32 / 46; half as many tiles: 14.7, 36; 16 + 3 K: 16.2, 38).
 struct Plan {
   int64_t cluster, chunks, tiles, bytes;  // cluster 0: two launches; bytes of results
 };
+constexpr int64_t TILES_LEAST = 8, TILES_BEAM = 2;
 constexpr int64_t CLUSTER = 8, CLUSTER_TILES = 4, CLUSTER_TILES_FULL = 16;  // (at most 32 tasks: 9 KB of results)
 
 Plan plan_of(int64_t groups, int64_t beams, int64_t vocab) {
@@ -549,7 +567,10 @@ Plan plan_of(int64_t groups, int64_t beams, int64_t vocab) {
     p.cluster = std::min<int64_t>(CLUSTER, beams * p.chunks);
     while (p.cluster & (p.cluster - 1)) ++p.cluster;  // a power of two
   } else {
-    cut(std::max<int64_t>(1, 4 * cv3::sm_count() / (groups * beams)));
+    const int64_t rows = groups * beams, wave = 3 * cv3::sm_count();
+    int64_t chunks = std::max<int64_t>(1, wave / rows);
+    if (rows * (chunks + 1) <= wave + wave / (3 * (chunks + 1))) ++chunks;
+    cut(std::max<int64_t>(1, std::min(chunks, row / (TILES_LEAST + TILES_BEAM * beams))));
   }
   p.bytes = (p.cluster ? 1 : groups) * beams * p.chunks * task_bytes(beams);
   return p;

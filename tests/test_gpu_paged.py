@@ -458,6 +458,32 @@ def test_beam(G, K, V, act, alpha):
     _beam(logits, scores, counts, done, stop, rng.integers(0, 30, G).astype(np.int32), alpha, act)
 
 
+@pytest.mark.parametrize("G,K,V", [(1, 32, 700), (2, 32, 6761), (1, 32, 40009), (2, 20, 30001), (1, 12, 100000), (1, 3, 140000)])
+@pytest.mark.parametrize("kind", ["plain", "ties", "one", "rising", "flat", "banned"])
+def test_beam_few_tiles_and_many_candidates(G, K, V, kind):
+    """Chunks with fewer tiles than hypotheses and rows of many chunks: ties everywhere, all winners in one
+    row, in its last tile or chunk, every logit near the maximum, the best tokens not allowed yet."""
+    rng = np.random.default_rng(V + K)
+    x = (rng.normal(size=(G, K, V)) * 3).astype(np.float32)
+    scores, counts, done = _state(rng, G, K)
+    stop = min_len = None
+    if kind == "ties":
+        x = np.round(x / 2) * 2
+        scores, counts, done = np.zeros_like(scores), np.ones_like(counts), done * 0
+    elif kind == "one":
+        scores -= 50
+        scores[:, K // 2], done[:, K // 2] = 0, 0
+    elif kind == "rising":
+        x = np.sort(x, -1)
+    elif kind == "flat":
+        x = (x / 8 - 4).astype(np.float32)
+    elif kind == "banned":
+        stop, min_len = (V // 3, V - 5), np.full(G, 100, np.int32)
+        x[:, :, V // 3:V - 5] += 9
+        x[:, 0, :V // 3] = -np.inf
+    _beam(x, scores, counts, done, stop, min_len, 0.6)
+
+
 def test_beam_first_step_and_ties():
     """Only the first hypothesis exists at the start; equal keys go to the lower hypothesis, then token."""
     rng = np.random.default_rng(2)
