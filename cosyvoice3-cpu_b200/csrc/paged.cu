@@ -497,9 +497,9 @@ extern "C" int cv3_paged_append(const cv3_paged_append_params* p, void* stream) 
   CV3_REQUIRE(p->ldq >= (p->heads + 2 * p->kv_heads) * p->head_dim, CV3_ERR_VALUE, "paged_append: ldq too small");
   const int ae = 16 / cv3p::type_size((int)p->type), ce = 16 / cv3p::type_size((int)p->kv_type);
   CV3_REQUIRE(cv3p::aligned16(p->qkv) && cv3p::aligned16(p->q_out) && cv3p::aligned16(p->k_pages) &&
-                  cv3p::aligned16(p->v_pages) && p->ldq % ae == 0 &&
-                  (p->ksp | p->ksh | p->kst | p->vsp | p->vsh | p->vst) % ce == 0,
-              CV3_ERR_VALUE, "paged_append: rows must start on 16-byte boundaries");
+                  cv3p::aligned16(p->v_pages) && cv3p::aligned16(p->cos_table) && cv3p::aligned16(p->sin_table) &&
+                  p->ldq % ae == 0 && (p->ksp | p->ksh | p->kst | p->vsp | p->vsh | p->vst) % ce == 0,
+              CV3_ERR_VALUE, "paged_append: rows and tables must start on 16-byte boundaries");
   if (p->rows == 0) return CV3_OK;
   // one head a thread until the GPU is full, then two rounds of HU
   const int64_t all = p->heads + 2 * p->kv_heads, per = p->head_dim / 2 / ae, full = (int64_t)cv3::sm_count() * 2048;

@@ -224,8 +224,8 @@ def paged_append(qkv, slots, pos, k_pages, v_pages, heads: int, cos=None, sin=No
     ``qkv`` ``(rows, (heads + 2 * kv_heads) * head_dim)`` holds query, key and value heads; returns the
     rotated queries ``(rows, heads, head_dim)`` in its type and writes keys (rotated) and values in the
     pools' type at ``slots`` (int64; -1: not stored).  ``cos`` / ``sin`` are fp32 ``(positions,
-    head_dim)`` half-split tables read at ``pos`` (int32); without them nothing is rotated and ``pos``
-    may be None.  A slot outside the pool, or a position outside the tables, stores nothing and counts
+    head_dim)`` half-split tables on 16-byte boundaries, read at ``pos`` (int32); without them nothing is
+    rotated and ``pos`` may be None.  A slot outside the pool, or a position outside the tables, stores nothing and counts
     into ``bad`` (int32, one value).  The slots of one call must differ.
     """
     if _bound or _bind():

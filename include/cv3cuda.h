@@ -436,7 +436,7 @@ int cv3_paged_extend(const cv3_paged_extend_params* params, void* stream);
  * nothing; another slot outside the pool, or a position outside the tables
  * [positions][head_dim], stores nothing and adds 1 to *bad (may be NULL).  NULL
  * tables: no rotation (pos may be NULL).  Slots of one call must differ.  head_dim a
- * multiple of 16 up to 256; rows on 16-byte boundaries. */
+ * multiple of 16 up to 256; rows and tables on 16-byte boundaries. */
 typedef struct cv3_paged_append_params {
   int64_t size;
   const void* qkv;

@@ -289,3 +289,14 @@ def test_oracle_attention_against_torch():
             a = 0.3 * (kk @ torch.from_numpy(q[b, h]))
             assert np.allclose(out[b, h], (torch.softmax(a, 0) @ vv).numpy())
             assert np.isclose(lse[b, h], float(torch.logsumexp(a, 0)))
+
+
+@pytest.mark.parametrize("cos,sin,code", [(0, 0, 0), (0, 16, 0), (4, 0, 1), (0, 8, 1), (12, 12, 1)])
+def test_rotation_tables_off_16_byte_boundaries(cos, sin, code):
+    """The tables are read 16 bytes at a time: a contiguous view that begins elsewhere is refused."""
+    L, p = pkg("_lib"), pkg("paged")
+    lib, at = L.load(), 1 << 20
+    rc = lib.cv3_paged_append(p._APPEND.pack(p._APPEND.size, at, 0, 0, 512, at + cos, at + sin, 50, at, at, 4, 2, 64, at, at, at,
+                                             0, 2048, 1024, 64, 2048, 1024, 64, 9, 16, 0), None)
+    assert rc == (L.CV3_ERR_VALUE if code else 0)
+    assert not code or b"16-byte" in lib.cv3_last_error()
