@@ -500,6 +500,8 @@ extern "C" int cv3_paged_append(const cv3_paged_append_params* p, void* stream) 
                   cv3p::aligned16(p->v_pages) && cv3p::aligned16(p->cos_table) && cv3p::aligned16(p->sin_table) &&
                   p->ldq % ae == 0 && (p->ksp | p->ksh | p->kst | p->vsp | p->vsh | p->vst) % ce == 0,
               CV3_ERR_VALUE, "paged_append: rows and tables must start on 16-byte boundaries");
+  CV3_REQUIRE(p->num_pages <= INT32_MAX && p->page_size <= INT32_MAX, CV3_ERR_VALUE,
+              "paged_append: pages and their rows are 32-bit numbers");
   if (p->rows == 0) return CV3_OK;
   // one head a thread until the GPU is full, then two rounds of HU
   const int64_t all = p->heads + 2 * p->kv_heads, per = p->head_dim / 2 / ae, full = (int64_t)cv3::sm_count() * 2048;

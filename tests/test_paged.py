@@ -300,3 +300,15 @@ def test_rotation_tables_off_16_byte_boundaries(cos, sin, code):
                                              0, 2048, 1024, 64, 2048, 1024, 64, 9, 16, 0), None)
     assert rc == (L.CV3_ERR_VALUE if code else 0)
     assert not code or b"16-byte" in lib.cv3_last_error()
+
+
+@pytest.mark.parametrize("pages,ps,code", [(9, (1 << 31) - 1, 0), (9, 1 << 31, 1), (9, 1 << 32, 1), (1 << 31, 16, 1),
+                                           ((1 << 31) - 1, 16, 0)])
+def test_pages_and_rows_of_a_page_are_32_bit_numbers(pages, ps, code):
+    """A slot is divided by the page size in 32 bits where the slot fits in them."""
+    L, p = pkg("_lib"), pkg("paged")
+    lib, at = L.load(), 1 << 20
+    rc = lib.cv3_paged_append(p._APPEND.pack(p._APPEND.size, at, 0, 0, 512, 0, 0, 0, at, 0, 4, 2, 64, at, at, at, 0, 2048, 1024, 64,
+                                             2048, 1024, 64, pages, ps, 0), None)
+    assert rc == (L.CV3_ERR_VALUE if code else 0)
+    assert not code or b"32-bit" in lib.cv3_last_error()
