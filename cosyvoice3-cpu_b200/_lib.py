@@ -107,6 +107,7 @@ SIGNATURES = {
     "cv3_beam_select": [P, P],
     "cv3_beam_workspace": [I64, I64, I64],
     "cv3_paged_reorder": [P, P],
+    "cv3_paged_give_back": [P, P],
 }
 _RESTYPE = {"cv3_last_error": ctypes.c_char_p, "cv3_launch_count": ctypes.c_ulonglong,
             "cv3_decode_sync_words": ctypes.c_int64, "cv3_paged_attention_workspace": ctypes.c_int64,

@@ -1,6 +1,6 @@
 // The paged key/value cache's bookkeeping and writes: block tables and slot maps from request
 // lengths (paged_extend), RoPE + store by slot (paged_append), beams following their parents
-// (paged_reorder).
+// (paged_reorder), pages that several rows name (paged_give_back).
 //
 // A cache is a pool of pages [page][kv_head][page_size][head_dim] (any strides with contiguous
 // rows); a request owns the pages its block-table row names, token t at row t % page_size of page
@@ -454,7 +454,161 @@ __global__ void __launch_bounds__(256) reorder_kernel(const ReorderArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// pages that several table rows name
+// ---------------------------------------------------------------------------
+
+// shares[p]: how many table rows name page p beyond the first (0 for a free page too, so taking one from
+// the stack changes nothing).  Rows leave their pages -- released requests all of them, beams the full pages
+// that their parent does not have in the same column -- and a page whose number falls below 0 goes back.
+struct GiveArgs {
+  int* shares;
+  int64_t pages;
+  const int* tables;
+  int64_t ld, max_blocks, ps;
+  const int* lens;
+  int64_t rows;
+  const int* release;  // NULL: beams follow `parents`
+  int* lens_out;
+  const int* parents;
+  int64_t beams;
+  int* stack;
+  int64_t cap;
+  const int* count;
+  int* count_out;
+  int* given;  // [rows] scratch: pages that the row gives back
+};
+
+struct Leaving {
+  const int *row, *next;  // entries that are left, and taken over instead (NULL: none)
+  int n;
+};
+
+__device__ __forceinline__ Leaving leaving(const GiveArgs& a, int64_t b) {
+  Leaving w = {a.tables + b * a.ld, nullptr, 0};
+  if (a.release) {
+    if (a.release[b]) w.n = (int)min(blocks_of(max(a.lens[b], 0), a.ps), a.max_blocks);
+  } else {
+    const int64_t first = b / a.beams * a.beams;
+    const int p = a.parents[b];
+    if (p >= 0 && p < a.beams && first + p != b) {
+      w.next = a.tables + (first + p) * a.ld;
+      w.n = (int)min(max(a.lens[first], 0) / a.ps, a.max_blocks);
+    }
+  }
+  return w;
+}
+
+// the page that column j leaves, -1: none of the pool, or it stays
+__device__ __forceinline__ int left_page(const GiveArgs& a, const Leaving& w, int j) {
+  const int page = w.row[j];
+  if (w.next && w.next[j] == page) return -1;
+  return page >= 0 && page < a.pages ? page : -1;
+}
+
+// A warp per row, the rows dealt to a cluster of CTAs.  A page that several rows leave at once goes back one time, for
+// the first of them (rows, then columns, in order), so the stack does not depend on timing: a page below 0
+// takes the number of its first place -- far below what counting reaches -- until that place gives it back.
+constexpr int MARK = INT32_MIN;
+
+__global__ void __launch_bounds__(ET) give_back_kernel(const GiveArgs a) {
+  __shared__ Sum2 red[ET / 32];
+  __shared__ int64_t place[ET];
+  dep_wait();
+  dep_release();
+  const int tid = threadIdx.x, T = blockDim.x, lane = tid & 31, warps = gridDim.x * (T >> 5);
+  const int64_t warp = blockIdx.x * (T >> 5) + (tid >> 5);
+  int64_t have = min((int64_t)max(*a.count, 0), a.cap);
+  auto sync = [&]() {
+    if (gridDim.x > 1) cv3p::cluster_sync();
+    else __syncthreads();
+  };
+  for (int64_t b = warp; b < a.rows; b += warps) {
+    const Leaving w = leaving(a, b);
+    for (int j = lane; j < w.n; j += 32) {
+      const int page = left_page(a, w, j);
+      if (page >= 0) atomicSub(a.shares + page, 1);
+      const int next = w.next ? w.next[j] : -1;
+      if (next != w.row[j] && next >= 0 && next < a.pages) atomicAdd(a.shares + next, 1);
+    }
+  }
+  sync();
+  for (int64_t b = warp; b < a.rows; b += warps) {
+    const Leaving w = leaving(a, b);
+    for (int j = lane; j < w.n; j += 32) {
+      const int page = left_page(a, w, j);
+      if (page >= 0 && __ldcg(a.shares + page) < 0) atomicMin(a.shares + page, MARK + (int)(b * a.max_blocks + j));
+    }
+  }
+  sync();
+  for (int64_t b = warp; b < a.rows; b += warps) {
+    const Leaving w = leaving(a, b);
+    int n = 0;
+    for (int j = lane; j < w.n; j += 32) {
+      const int page = left_page(a, w, j);
+      n += page >= 0 && __ldcg(a.shares + page) == MARK + (int)(b * a.max_blocks + j);
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) a.given[b] = n;
+  }
+  sync();
+  for (int64_t b0 = 0; b0 < a.rows; b0 += T) {
+    const int64_t n = b0 + tid < a.rows ? __ldcg(a.given + b0 + tid) : 0;
+    Sum2 total;
+    place[tid] = have + block_scan(Sum2{n, 0}, red, total).x - n;
+    __syncthreads();
+    const int most = (int)min((int64_t)T, a.rows - b0);
+    for (int i = (int)warp; i < most; i += warps) {
+      const int64_t b = b0 + i;
+      const Leaving w = leaving(a, b);
+      int64_t at = place[i];
+      for (int j0 = 0; j0 < w.n; j0 += 32) {
+        const int j = j0 + lane, page = j < w.n ? left_page(a, w, j) : -1;
+        const bool mine = page >= 0 && __ldcg(a.shares + page) == MARK + (int)(b * a.max_blocks + j);
+        const unsigned who = __ballot_sync(0xffffffffu, mine);
+        if (mine) {
+          const int64_t to = at + __popc(who & ((1u << lane) - 1u));
+          if (to < a.cap) a.stack[to] = page;
+          a.shares[page] = 0;
+        }
+        at += __popc(who);
+      }
+      __syncwarp();  // (lens_out may be lens)
+      if (a.lens_out && lane == 0) a.lens_out[b] = a.release[b] ? 0 : max(a.lens[b], 0);
+    }
+    have += total.x;
+    __syncthreads();
+  }
+  if (blockIdx.x == 0 && tid == 0) *a.count_out = (int)min(have, a.cap);
+}
+
 }  // namespace
+
+extern "C" int cv3_paged_give_back(const cv3_paged_give_back_params* p, void* stream) {
+  CV3_REQUIRE(p && p->size == (int64_t)sizeof(*p), CV3_ERR_VALUE, "paged_give_back: bad parameter block");
+  CV3_REQUIRE(p->num_pages >= 0 && p->rows >= 0 && p->max_blocks >= 0 && p->table_ld >= p->max_blocks &&
+                  p->page_size > 0 && p->free_cap >= 0,
+              CV3_ERR_VALUE, "paged_give_back: bad shape");
+  CV3_REQUIRE((p->release == nullptr) != (p->parents == nullptr), CV3_ERR_VALUE,
+              "paged_give_back: either release or parents is given");
+  CV3_REQUIRE(p->release ? p->lens_out != nullptr : p->beams > 0 && p->rows % p->beams == 0, CV3_ERR_VALUE,
+              "paged_give_back: release goes with lens_out, parents with groups of beams");
+  CV3_REQUIRE(p->release || (p->beams <= CV3_MAX_BEAMS && p->rows / p->beams <= 65535), CV3_ERR_UNSUPPORTED,
+              "paged_give_back: more than 65535 groups or %d beams", CV3_MAX_BEAMS);
+  CV3_REQUIRE(p->num_pages <= INT32_MAX && p->free_cap <= INT32_MAX && p->page_size <= INT32_MAX && p->rows <= 1 << 30 &&
+                  p->max_blocks <= 1 << 30 && p->rows * p->max_blocks <= 1 << 30 &&
+                  p->max_blocks * p->page_size <= INT32_MAX,
+              CV3_ERR_VALUE, "paged_give_back: pages and positions are 32-bit numbers, places of the tables 30-bit ones");
+  const GiveArgs a = {p->shares, p->num_pages, p->block_tables, p->table_ld, p->max_blocks, p->page_size, p->lens, p->rows,
+                      p->release, p->release ? p->lens_out : nullptr, p->parents, p->beams, p->free_pages, p->free_cap,
+                      p->free_count, p->free_count_out, p->scratch};
+  const int64_t ctas = p->rows >= 16 ? 8 : 1;
+  const unsigned threads = (unsigned)std::min<int64_t>(ET, std::max<int64_t>(64, (p->rows + ctas - 1) / ctas * 32));
+  cudaStream_t st = cv3::as_stream(stream);
+  return cv3::check_launch("paged_give_back",
+                           ctas > 1 ? cv3p::launch_cluster(give_back_kernel, dim3(8), dim3(threads), 0, 8u, st, a)
+                                    : cv3::launch_dep(give_back_kernel, dim3(1), dim3(threads), 0, st, a));
+}
 
 extern "C" int cv3_paged_extend(const cv3_paged_extend_params* p, void* stream) {
   CV3_REQUIRE(p && p->size == (int64_t)sizeof(*p), CV3_ERR_VALUE, "paged_extend: bad parameter block");
@@ -541,7 +695,6 @@ extern "C" int cv3_paged_reorder(const cv3_paged_reorder_params* p, void* stream
   CV3_REQUIRE(cv3p::aligned16(p->k_pages) && cv3p::aligned16(p->v_pages) && p->head_dim * es % 16 == 0 &&
                   (p->ksl | p->ksp | p->ksh | p->kst | p->vsl | p->vsp | p->vsh | p->vst) * es % 16 == 0,
               CV3_ERR_VALUE, "paged_reorder: cache rows must be 16-byte pieces on 16-byte boundaries");
-  if (p->groups == 0 || p->beams == 1) return CV3_OK;
   const ReorderArgs a = {static_cast<char*>(p->k_pages), static_cast<char*>(p->v_pages), p->ksl * es, p->ksp * es,
                          p->ksh * es, p->kst * es, p->vsl * es, p->vsp * es, p->vsh * es, p->vst * es, p->layers,
                          p->num_pages, p->kv_heads, p->page_size, p->head_dim * es / 16, p->block_tables, p->table_ld,
@@ -551,6 +704,7 @@ extern "C" int cv3_paged_reorder(const cv3_paged_reorder_params* p, void* stream
   CV3_REQUIRE(p->kv_heads <= 1 << 16 && p->page_size <= 1 << 20 && a.row16 <= 1 << 12 && most <= 1 << 30 &&
                   p->max_blocks <= 1 << 30 && p->layers <= 32767,
               CV3_ERR_UNSUPPORTED, "paged_reorder: pages too large or too many layers");
+  if (p->groups == 0 || p->beams == 1) return CV3_OK;
   const int64_t gz = std::max<int64_t>(1, 2 * p->layers);
   const int64_t gx = std::max<int64_t>(1, std::min<int64_t>((most + 255) / 256, 16 * cv3::sm_count() / (p->groups * gz) + 1));
   using Fn = void (*)(const ReorderArgs);

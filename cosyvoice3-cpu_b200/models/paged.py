@@ -25,10 +25,14 @@ torch = D.torch
 
 class PagedKVCache:
     """Pages ``(layers, pages, kv_heads, page_size, head_dim)`` of keys and of values for ``requests``
-    requests of up to ``max_len`` tokens; ``dtype`` float32, float16 or bfloat16."""
+    requests of up to ``max_len`` tokens; ``dtype`` float32, float16 or bfloat16.
+
+    Beams share pages, which ``shares`` counts: a page returns to the stack when no request names it any
+    more.  ``releases=False`` saves the counting for a cache whose requests are never released: pages that
+    beams leave then stay out of the stack until :meth:`start_beams` begins anew."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, requests: int, max_len: int, pages: int,
-                 page_size: int = 16, dtype=None):
+                 page_size: int = 16, dtype=None, releases: bool = True):
         dtype = D.F32 if dtype is None else dtype
         self.layers, self.kv_heads, self.head_dim, self.page_size, self.pages = layers, kv_heads, head_dim, page_size, pages
         self.blocks = -(-max_len // page_size)
@@ -39,6 +43,7 @@ class PagedKVCache:
         self.free_count = torch.full((1,), pages, dtype=torch.int32, device="cuda")
         self.lens = torch.zeros(requests, dtype=torch.int32, device="cuda")
         self.bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+        self.shares = torch.zeros(pages, dtype=torch.int32, device="cuda") if releases else None
 
     def nbytes(self) -> int:
         return 2 * self.k.numel() * self.k.element_size()
@@ -52,8 +57,10 @@ class PagedKVCache:
         return self.extend_into(out, new_lens, release)
 
     def extend_into(self, out: ops.PagedStep, new_lens, release=None) -> ops.PagedStep:
+        if release is not None and self.shares is None:
+            raise ValueError("a cache made with releases=False releases no requests")
         return ops.paged_extend(self.lens, new_lens, self.tables, self.free, self.free_count, self.page_size,
-                                out.slots.shape[0], release=release, out=out)
+                                out.slots.shape[0], release=release, out=out, shares=self.shares)
 
     def append(self, layer: int, qkv, step: ops.PagedStep, heads: int, cos, sin, out=None):
         """Rotated queries of fused rows; their keys and values go to the step's slots."""
@@ -65,13 +72,14 @@ class PagedKVCache:
                                    bad=self.bad)
 
     def reorder(self, parents) -> None:
-        ops.paged_reorder(self.k, self.v, self.tables, parents, self.lens)
+        counts = () if self.shares is None else (self.shares, self.free, self.free_count)
+        ops.paged_reorder(self.k, self.v, self.tables, parents, self.lens, *counts)
 
     def start_beams(self, prompts, cache, beams: int) -> None:
         """Begins ``beams`` hypotheses of every prompt (lengths ``prompts``) from the contiguous prefill
         ``cache``: full pages are shared by a group's rows, each row has a last page of its own."""
         ps, at = self.page_size, 0
-        tables = np.full(tuple(self.tables.shape), -1, np.int32)
+        tables, shares = np.full(tuple(self.tables.shape), -1, np.int32), np.zeros(self.pages, np.int32)
         src, dst = [], []      # (group, block) -> page
         for g, n in enumerate(prompts):
             rows = slice(g * beams, (g + 1) * beams)
@@ -79,6 +87,7 @@ class PagedKVCache:
             if -(-n // ps) > self.blocks:
                 raise ValueError(f"a prompt of {n} tokens in a cache of {self.blocks} pages per request")
             tables[rows, :full] = np.arange(at, at + full)
+            shares[at:at + full] = beams - 1
             src += [(g, j) for j in range(full)]
             dst += list(range(at, at + full))
             at += full
@@ -90,6 +99,8 @@ class PagedKVCache:
         if at > self.pages:
             raise ValueError(f"{at} pages for the prompts, {self.pages} in the cache")
         self.tables.copy_(torch.from_numpy(tables))
+        if self.shares is not None:
+            self.shares.copy_(torch.from_numpy(shares))
         self.free.copy_(torch.arange(self.pages, dtype=torch.int32))
         self.free[:self.pages - at] = torch.arange(self.pages - 1, at - 1, -1, dtype=torch.int32)
         self.free_count.fill_(self.pages - at)
@@ -119,7 +130,8 @@ class BeamEngine:
         H, Hk, hd, hid = c.num_attention_heads, c.num_key_value_heads, c.head_dim, c.hidden_size
         self.max_prompt, self.max_steps = max_prompt, max_steps
         need = -(-max_prompt // page_size) + beams * (-(-max_steps // page_size) + 2)
-        self.cache = PagedKVCache(c.num_hidden_layers, Hk, hd, R, max_prompt + max_steps, groups * need, page_size, cache_dtype)
+        self.cache = PagedKVCache(c.num_hidden_layers, Hk, hd, R, max_prompt + max_steps, groups * need, page_size, cache_dtype,
+                                  releases=False)   # (every run begins anew)
         self.head = Lin(head_w, head_bias)
         self.vocab = self.head.n
         self.emb = speech_emb

@@ -10,9 +10,10 @@ values; a transposed view of ``(pages, page_size, kv_heads, head_dim)`` serves a
     out = ops.paged_attention(q, k_pages, v_pages, block_tables, step.lens)
     ...                                                # the other layers, the head
     best = ops.beam_select(logits, scores, counts, done, stop=(6561, 6761))
-    ops.paged_reorder(k_all, v_all, block_tables, best.parents, step.lens)
+    ops.paged_reorder(k_all, v_all, block_tables, best.parents, step.lens, shares, free_pages, step.free_count)
 
-Pools, tables and state are updated in place, so every argument is a device array; a host array
+Beams share pages; ``shares`` counts them, so that each goes back to the stack once, when no row names
+it any more.  Pools, tables and state are updated in place, so every argument is a device array; a host array
 raises ValueError.  Shape, type and alignment errors raise ValueError, configurations that are not
 built RuntimeError.  The calls are ordered on the current stream of the current device (on which
 all arrays have to be), take no persistent workspace and can be captured into a CUDA graph: what
@@ -39,8 +40,8 @@ MAX_BEAMS = 32   # CV3_MAX_BEAMS
 
 # The C entries' parameter blocks (include/cv3cuda.h): 64-bit fields, packed here in one call -- a
 # third of what 20 to 35 ctypes arguments cost.
-_EXTEND, _APPEND, _ATTENTION, _BEAM, _REORDER = (struct.Struct("=" + f) for f in
-                                                 ("20q", "26q", "32qd", "20qd", "24q"))
+_EXTEND, _APPEND, _ATTENTION, _BEAM, _REORDER, _GIVE_BACK = (struct.Struct("=" + f) for f in
+                                                             ("20q", "26q", "32qd", "20qd", "24q", "18q"))
 
 if torch is not None:
     _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -165,8 +166,21 @@ def _like(name: str, out, shape, dtype):
     return out
 
 
+def _give_back(name, d, shares, tables, lens, n, page_size, free_pages, free_count, count_out, release=0, lens_out=0, parents=0,
+               beams=0):
+    """Rows leave their pages (cv3_paged_give_back); pointers but for the arrays shares, lens and free_pages."""
+    tp, ld, cols = tables
+    scratch = _new(lens, (n,), D.I32)
+    rc = load().cv3_paged_give_back(
+        _GIVE_BACK.pack(_GIVE_BACK.size, _ints(name, "shares", shares, shares.numel()), shares.numel(), tp, ld, cols, page_size,
+                        lens.data_ptr(), n, release, lens_out, parents, beams, free_pages.data_ptr(), free_pages.numel(),
+                        free_count, count_out, scratch.data_ptr()), D.raw_stream(d))
+    if rc:
+        check(rc, name)
+
+
 def paged_extend(lens, new_lens, block_tables, free_pages, free_count, page_size: int, max_tokens: int, release=None,
-                 out: Optional[PagedStep] = None) -> PagedStep:
+                 out: Optional[PagedStep] = None, shares=None) -> PagedStep:
     """Cache pages and slots for the new tokens of every request.
 
     Request ``b`` holds ``lens[b]`` tokens (int32) and gets ``new_lens[b]`` more; where ``release[b]``
@@ -176,24 +190,31 @@ def paged_extend(lens, new_lens, block_tables, free_pages, free_count, page_size
     pages, rows (``max_tokens`` over all) or table columns do not suffice on, none gets new tokens.
     Returns a :class:`PagedStep`, whose rows behind the last token have slot -1; ``out`` gives it its tensors (``out.lens`` may be ``lens`` and
     ``out.free_count`` may be ``free_count``: the state then advances in place).
+
+    ``shares`` (int32, one number per page of the pool, zeros to begin with, updated in place) holds for
+    every page the rows that name it beyond the first, as :func:`paged_reorder` leaves them: a released
+    row then gives back the pages that no other row names.  Without it every page of a released row goes
+    back, so rows that share pages must not be released.
     """
-    if out is None and (_bound or _bind()):
+    if out is None and shares is None and (_bound or _bind()):
         r = _bound.extend(lens, new_lens, block_tables, free_pages, free_count, page_size, max_tokens, release)
         if r is not None:
             return r
     name = "paged_extend"
     arrays = (lens, new_lens, block_tables, free_pages, free_count)
-    d = _device(name, *(arrays if release is None else arrays + (release,)))
+    d = _device(name, *arrays, *(x for x in (release, shares) if x is not None))
     if len(lens.shape) != 1:
         raise ValueError(f"{name}: lens must be (requests,), got {tuple(lens.shape)}")
     n, T = lens.shape[0], int(max_tokens)
-    if page_size <= 0 or T < 0:
+    if page_size <= 0 or not 0 <= T < 2 ** 31 - 1024:
         raise ValueError(f"{name}: page_size {page_size}, max_tokens {max_tokens}")
     pl, pn = _ints(name, "lens", lens, n), _ints(name, "new_lens", new_lens, n)
     pr = 0 if release is None else _ints(name, "release", release, n)
     tp, ld, cols = _table(name, block_tables, n)
     cap = free_pages.numel()
     pf, pc = _ints(name, "free_pages", free_pages, cap), _ints(name, "free_count", free_count, 1)
+    if shares is not None:
+        _ints(name, "shares", shares, shares.numel())
     if out is None:
         sizes = (T, T, n + 1, n, 1, n + 1)
         if torch is not None:
@@ -209,6 +230,11 @@ def paged_extend(lens, new_lens, block_tables, free_pages, free_count, page_size
                            ("lens", out.lens, n), ("free_count", out.free_count, 1)):
             _ints(name, "out." + what, x, m)
         scratch = _new(lens, (n + 1,), D.I32)
+    if shares is not None and release is not None:
+        held, left = _new(lens, (n,), D.I32), _new(lens, (1,), D.I32)
+        _give_back(name, d, shares, (tp, ld, cols), lens, n, page_size, free_pages, pc, left.data_ptr(), release=pr,
+                   lens_out=held.data_ptr())
+        pl, pr, pc = held.data_ptr(), 0, left.data_ptr()
     rc = load().cv3_paged_extend(
         _EXTEND.pack(_EXTEND.size, pl, pn, pr, n, tp, ld, cols, page_size, pf, cap, pc, T, out.slots.data_ptr(),
                      out.seq.data_ptr(), out.pos.data_ptr(), out.offsets.data_ptr(), out.lens.data_ptr(),
@@ -377,7 +403,7 @@ def beam_select(logits, scores, counts, done, stop: Optional[Tuple[int, int]] = 
     return out
 
 
-def paged_reorder(k_pages, v_pages, block_tables, parents, lens) -> None:
+def paged_reorder(k_pages, v_pages, block_tables, parents, lens, shares=None, free_pages=None, free_count=None) -> None:
     """The cache follows the beams, in place.
 
     Pools ``(layers, pages, kv_heads, page_size, head_dim)`` (or one layer without the first
@@ -385,11 +411,19 @@ def paged_reorder(k_pages, v_pages, block_tables, parents, lens) -> None:
     ``lens`` int32 ``(groups * beams,)``, alike within a group.  Beam k becomes what beam
     ``parents[g][k]`` was: full pages are shared through the table, the tokens of the last, partly
     filled page are copied into the page that beam k's own row names there (and no other beam's).
+
+    ``shares`` (int32, one number per page: the rows that name it beyond the first), ``free_pages`` and
+    ``free_count`` (all three or none, updated in place) keep account of the shared pages: those that no
+    beam names any more go back to the stack, and :func:`paged_extend` with ``shares`` may release beams.
+    Without them a page that is left stays out of the stack, and beams must not be released.
     """
-    if (_bound or _bind()) and _bound.reorder(k_pages, v_pages, block_tables, parents, lens):
+    if shares is None and free_pages is None and free_count is None and (_bound or _bind()) and _bound.reorder(k_pages, v_pages, block_tables, parents, lens):
         return
     name = "paged_reorder"
-    d = _device(name, k_pages, v_pages, block_tables, parents, lens)
+    counted = tuple(x for x in (shares, free_pages, free_count) if x is not None)
+    if len(counted) not in (0, 3):
+        raise ValueError(f"{name}: shares, free_pages and free_count go together")
+    d = _device(name, k_pages, v_pages, block_tables, parents, lens, *counted)
     dims = len(k_pages.shape)
     if dims not in (4, 5):
         raise ValueError(f"{name}: pools of 4 or 5 dimensions expected, got {tuple(k_pages.shape)}")
@@ -403,8 +437,19 @@ def paged_reorder(k_pages, v_pages, block_tables, parents, lens) -> None:
     pp = _ints(name, "parents", parents, G * K)
     tp, ld, cols = _table(name, block_tables, G * K)
     plens = _ints(name, "lens", lens, G * K)
-    rc = load().cv3_paged_reorder(
-        _REORDER.pack(_REORDER.size, k_pages.data_ptr(), v_pages.data_ptr(), kt, layers, pages, kv, ps, dim, *ks[:4],
-                      *vs[:4], tp, ld, cols, pp, plens, G, K), D.raw_stream(d))
+    if counted:
+        _ints(name, "shares", shares, pages), _ints(name, "free_pages", free_pages, free_pages.numel())
+        pc = _ints(name, "free_count", free_count, 1)
+    lib = load()
+    block = _REORDER.pack(_REORDER.size, k_pages.data_ptr(), v_pages.data_ptr(), kt, layers, pages, kv, ps, dim, *ks[:4], *vs[:4], tp,
+                          ld, cols, pp, plens, G, K)
+    if counted:
+        # (no groups: what the copy refuses is refused before anything is counted)
+        rc = lib.cv3_paged_reorder(block[:-16] + struct.pack("=2q", 0, K), D.raw_stream(d))
+        if rc:
+            check(rc, name)
+        if G > 0 and K > 1:
+            _give_back(name, d, shares, (tp, ld, cols), lens, G * K, ps, free_pages, pc, pc, parents=pp, beams=K)
+    rc = lib.cv3_paged_reorder(block, D.raw_stream(d))
     if rc:
         check(rc, name)

@@ -407,7 +407,9 @@ int cv3_head_select(const float* logits, int64_t batch, int64_t vocab, int64_t s
  * per new token, requests one after another (rows behind the last: slot -1, seq -1,
  * pos 0); offsets [batch + 1], request b's rows being offsets[b] .. offsets[b+1];
  * lens_out [batch]; *free_count_out.  lens_out may be lens, free_count_out may be
- * free_count.  scratch: batch + 1 ints. */
+ * free_count.  scratch: batch + 1 ints.  A released row's pages go back whatever other
+ * rows name them: where rows share pages, as cv3_paged_reorder lets them, requests
+ * are released by cv3_paged_give_back instead. */
 typedef struct cv3_paged_extend_params {
   int64_t size;
   const int* lens;
@@ -529,7 +531,8 @@ int64_t cv3_beam_workspace(int64_t groups, int64_t beams, int64_t vocab);
  * tokens of the last, partly filled page are copied in every layer into the page that
  * beam k's own row names there, which no other beam may name.  A parent outside
  * [0, beams) counts as k; a beam whose own or whose parent's last page lies outside the
- * pool keeps that page as it is.  Pools: layers s_l apart. */
+ * pool keeps that page as it is.  Pools: layers s_l apart.  The pages that a beam had
+ * instead are not given back: cv3_paged_give_back, called before, does that. */
 typedef struct cv3_paged_reorder_params {
   int64_t size;
   void* k_pages;
@@ -542,6 +545,40 @@ typedef struct cv3_paged_reorder_params {
   int64_t groups, beams;
 } cv3_paged_reorder_params;
 int cv3_paged_reorder(const cv3_paged_reorder_params* params, void* stream);
+
+/* Pages that several table rows name.  shares[p], for every page of the pool, is the number
+ * of rows that name it beyond the first (0 for a free page; zeros to begin with, and
+ * cv3_paged_extend, which takes pages for one row each, leaves it as it is).  Rows leave
+ * pages, each lowering its number by one, and pages whose number falls below 0 go
+ * to the end of the stack free_pages[0 .. *free_count), in the order in which rows, then columns, name
+ * them first, with the number 0 again.
+ * release non-NULL [rows]: rows with release[b] != 0 leave the pages of their lens[b]
+ * tokens; lens_out[b] (may be lens) is 0 for them and max(lens[b], 0) for the others, and
+ * cv3_paged_extend follows with these lengths and without release.
+ * parents non-NULL [rows]: what cv3_paged_reorder with the same arguments is about to do (rows a
+ * group's `beams` after another): beams leave their full pages and take their parents',
+ * each of which raises its number by one.
+ * free_count_out may be free_count.  Page numbers outside the pool are passed over.
+ * rows * max_blocks is at most 2^30.  scratch: `rows` ints. */
+typedef struct cv3_paged_give_back_params {
+  int64_t size;
+  int* shares;
+  int64_t num_pages;
+  const int* block_tables;
+  int64_t table_ld, max_blocks, page_size;
+  const int* lens;
+  int64_t rows;
+  const int* release;
+  int* lens_out;
+  const int* parents;
+  int64_t beams;
+  int* free_pages;
+  int64_t free_cap;
+  const int* free_count;
+  int* free_count_out;
+  int* scratch;
+} cv3_paged_give_back_params;
+int cv3_paged_give_back(const cv3_paged_give_back_params* params, void* stream);
 
 /* ------------------------------------------------------------------ */
 /* DiT flow estimator and Euler/CFG solve (cv3cpu/models/dit.py, flow.py) */

@@ -43,6 +43,40 @@ def extend(lens, new_lens, tables, free_pages, free_count, page_size, max_tokens
     return tables, stack, slots, seq, pos, np.array(offsets, np.int32), np.array(out_lens, np.int32), count
 
 
+def give_back(tables, lens, page_size, free_pages, free_count, shares, release=None, parents=None):
+    """(free_pages, free_count, shares, lens) after rows left their pages: released ones all of them, beams the full
+    pages that their parent does not have in the same column (and takes instead)."""
+    stack, shares, lens = free_pages.copy(), shares.copy(), np.maximum(lens, 0)
+    count, P = int(np.clip(free_count, 0, len(stack))), len(shares)
+    cols, left = tables.shape[1], []
+    for b in range(len(tables)):
+        if release is not None:
+            if release[b]:
+                left += tables[b, :min(-(-int(lens[b]) // page_size), cols)].tolist()
+                lens[b] = 0
+            continue
+        K = parents.shape[1]
+        p = int(parents.reshape(-1)[b])
+        if 0 <= p < K and p != b % K:
+            first = b // K * K
+            for j in range(min(int(lens[first]) // page_size, cols)):
+                old, new = int(tables[b, j]), int(tables[first + p, j])
+                if old != new:
+                    left.append(old)
+                    if 0 <= new < P:
+                        shares[new] += 1
+    left = [p for p in left if 0 <= p < P]
+    for p in left:
+        shares[p] -= 1
+    for p in left:
+        if shares[p] < 0:
+            if count < len(stack):
+                stack[count] = p
+                count += 1
+            shares[p] = 0
+    return stack, count, shares, lens
+
+
 def rope_rows(x, cos, sin):
     """Half-split rotation of rows ``(rows, heads, dim)`` by tables rows ``(rows, dim)``, in float64."""
     x = x.astype(np.float64)

@@ -312,3 +312,66 @@ def test_pages_and_rows_of_a_page_are_32_bit_numbers(pages, ps, code):
                                              2048, 1024, 64, pages, ps, 0), None)
     assert rc == (L.CV3_ERR_VALUE if code else 0)
     assert not code or b"32-bit" in lib.cv3_last_error()
+
+
+# ---------------------------------------------------------------------------
+# pages that several rows name
+# ---------------------------------------------------------------------------
+
+def test_oracle_gives_shared_pages_back_once():
+    """Two beams of two full pages each both follow the first and are released together: the pages that the second left
+    go back when it follows, the shared ones one time when both are released, in the order of their places."""
+    t = np.array([[0, 1], [2, 3]], np.int32)
+    none, par = np.full(4, -1, np.int32), np.array([[0, 0]], np.int32)
+    stack, count, shares, lens = ref.give_back(t, np.array([8, 8]), 4, none, 0, np.zeros(4, np.int32), parents=par)
+    assert stack[:count].tolist() == [2, 3] and shares.tolist() == [1, 1, 0, 0] and lens.tolist() == [8, 8]
+    t[1] = t[0]
+    one, n, left, held = ref.give_back(t, lens, 4, stack, count, shares, release=[1, 0])
+    assert n == 2 and left.tolist() == [0] * 4 and held.tolist() == [0, 8]
+    stack, count, shares, lens = ref.give_back(t, lens, 4, stack, count, shares, release=[1, 1])
+    assert stack[:count].tolist() == [2, 3, 0, 1] and shares.tolist() == [0] * 4
+    tables, stack, slots, *_ = ref.extend(lens, [8, 8], t, stack, count, 4, 16)
+    assert sorted(tables.reshape(-1).tolist()) == [0, 1, 2, 3] and len(set(slots.tolist())) == 16
+
+
+def test_refusals_of_shared_pages(ops):
+    import torch
+    good = dict(lens=_i32(3), new_lens=_i32(3), block_tables=_i32(3, 5), free_pages=_i32(9), free_count=_i32(1),
+                page_size=16, max_tokens=4, release=_i32(3), shares=_i32(9))
+    with pytest.raises(AssertionError, match="accepted"):
+        ops.paged_extend(**good)
+    for bad in (torch.zeros(9), torch.zeros(9, dtype=torch.int64), _i32(18)[::2]):
+        with pytest.raises(ValueError, match="shares"):
+            ops.paged_extend(**{**good, "shares": bad})
+    pool = torch.zeros(2, 9, 2, 16, 64)
+    fine = dict(k_pages=pool, v_pages=pool, block_tables=_i32(6, 3), parents=_i32(2, 3), lens=_i32(6), shares=_i32(9),
+                free_pages=_i32(9), free_count=_i32(1))
+    with pytest.raises(AssertionError, match="accepted"):
+        ops.paged_reorder(**fine)
+    for change in (dict(shares=_i32(8)), dict(shares=torch.zeros(9)), dict(free_pages=torch.zeros(9)), dict(free_count=_i32(2))):
+        with pytest.raises(ValueError):
+            ops.paged_reorder(**{**fine, **change})
+    for gone in ("shares", "free_pages", "free_count"):
+        with pytest.raises(ValueError, match="go together"):
+            ops.paged_reorder(**{**fine, gone: None})
+
+
+def test_entry_for_shared_pages():
+    """The parameter block has the header's fields, and what is refused is refused before any device work."""
+    L, p = pkg("_lib"), pkg("paged")
+    lib, at = L.load(), 1 << 20
+    text = open(os.path.join(REPO, "include", "cv3cuda.h")).read()
+    body = re.search(r"typedef struct cv3_paged_give_back_params \{(.*?)\}", text, re.S).group(1)
+    fields = [x.strip() for line in body.split(";") for x in line.split(",") if x.strip()]
+    assert p._GIVE_BACK.size == 8 * len(fields) and p._GIVE_BACK.format.lstrip("=") == "%dq" % len(fields)
+
+    def give_back(size=p._GIVE_BACK.size, pages=9, ld=3, cols=3, ps=16, rows=4, release=at, lens_out=at, parents=0, beams=0, cap=9):
+        return lib.cv3_paged_give_back(p._GIVE_BACK.pack(size, at, pages, at, ld, cols, ps, at, rows, release, lens_out, parents,
+                                                         beams, at, cap, at, at, at), None)
+    V, U = L.CV3_ERR_VALUE, L.CV3_ERR_UNSUPPORTED
+    assert give_back(size=8) == V and give_back(ld=2) == V and give_back(ps=0) == V and give_back(cap=-1) == V
+    assert give_back(release=0) == V and give_back(parents=at) == V and give_back(lens_out=0) == V
+    assert give_back(release=0, parents=at, beams=3) == V and give_back(release=0, parents=at, beams=64, rows=64) == U
+    assert give_back(release=0, parents=at, beams=2, rows=1 << 18) == U
+    assert give_back(rows=1 << 20, cols=1 << 11, ld=1 << 11) == V and give_back(cols=1 << 28, ld=1 << 28) == V
+    assert give_back(pages=1 << 31) == V
