@@ -23,7 +23,7 @@
 //    part: 22 bits of both at no cost.  The matrix pipe truncates when it adds, so only one tile's
 //    p.v is summed there; tiles are added in fp32 registers, the softmax's rescaling on the way.
 //    Queries of the cache's own 16-bit type need less: 16-bit products, exact for q.k, and p in two
-//    16-bit parts, whose 2^-16 is far below the result's rounding (64 ragged requests: 377 instead of
+//    16-bit parts, whose 2^-16 (bf16) or 2^-22 (fp16) is far below the result's rounding (64 ragged requests: 377 instead of
 //    404 us).
 //
 // Measured: 64 requests of 1 to 16384 keys, 32 / 8 heads of 128, bf16 (2.15 GB): 344 us, 6.2 TB/s (390 us
@@ -93,8 +93,15 @@ __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// two probabilities as 16-bit parts: the upper ones, and what these leave (never 0, see TINY; 6e-8, the
-// smallest fp16, is below the arithmetic's own rounding)
+// Two probabilities as 16-bit parts: the upper ones, and what these leave (never 0, so that 0 * inf does not
+// arise).  bf16 has fp32's exponents: 16 bits of any probability, TINY where nothing is left.  fp16 begins at 6e-8, and
+// many keys behind a dominating one may have less each: the upper parts are those of p * P16, the lower ones are raised by
+// R16 once more, both powers of two that go out of the sums again.  22 bits of p down to 2^-28, 2^-50 below; 2^-49 for 0.
+template <typename KT>
+constexpr float P16 = std::is_same<KT, __half>::value ? 16384.f : 1.f;
+template <typename KT>
+constexpr float R16 = std::is_same<KT, __half>::value ? 2048.f : 1.f;
+
 template <typename KT>
 __device__ __forceinline__ void split_16(float x, float y, uint32_t& hi, uint32_t& lo) {
   if constexpr (std::is_same<KT, __nv_bfloat16>::value) {
@@ -104,10 +111,12 @@ __device__ __forceinline__ void split_16(float x, float y, uint32_t& hi, uint32_
     const __nv_bfloat162 l = __floats2bfloat162_rn(rx == 0.f ? TINY : rx, ry == 0.f ? TINY : ry);
     lo = *reinterpret_cast<const uint32_t*>(&l);
   } else {
+    x *= P16<KT>;
+    y *= P16<KT>;
     const __half2 h = __floats2half2_rn(x, y);
     hi = *reinterpret_cast<const uint32_t*>(&h);
     const float2 back = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - back.x, y - back.y);
+    const __half2 l = __floats2half2_rn((x - back.x) * R16<KT>, (y - back.y) * R16<KT>);
     lo = *reinterpret_cast<const uint32_t*>(&l);
     lo |= (lo & 0x7FFFu ? 0u : 1u) | (lo & 0x7FFF0000u ? 0u : 0x10000u);
   }
@@ -432,8 +441,8 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
             mma_16<KT>(acc, p[i / 2], __byte_perm(vr[i][0][x].r[w], vr[i][1][x].r[w], half),
                        __byte_perm(vr[i + 1][0][x].r[w], vr[i + 1][1][x].r[w], half));
           }
-          o[j][0] = fmaf(o[j][0], fade, acc[0] + acc[2]);
-          o[j][1] = fmaf(o[j][1], fade, acc[1] + acc[3]);
+          o[j][0] = fmaf(o[j][0], fade, fmaf(acc[2], 1.f / R16<KT>, acc[0]));
+          o[j][1] = fmaf(o[j][1], fade, fmaf(acc[3], 1.f / R16<KT>, acc[1]));
         }
       } else {
         uint32_t p[NT][4];
@@ -472,12 +481,13 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attention_kernel(const AttnA
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (t == 0) { sm[warp][n] = m; sl[warp][n] = l; }
+    constexpr float BACK = H16 ? 1.f / P16<KT> : 1.f;
 #pragma unroll
     for (int x = 0; x < VC; ++x)
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        so[warp][n][x * 8 * VE + 2 * t * VE + e] = o[x * VE + e][0];
-        so[warp][n][x * 8 * VE + (2 * t + 1) * VE + e] = o[x * VE + e][1];
+        so[warp][n][x * 8 * VE + 2 * t * VE + e] = o[x * VE + e][0] * BACK;
+        so[warp][n][x * 8 * VE + (2 * t + 1) * VE + e] = o[x * VE + e][1] * BACK;
       }
     __syncthreads();
   };
