@@ -72,3 +72,45 @@ def test_fp16_values_of_any_size_and_infinite_ones(length):
     assert float(got2[0, 0, 5]) == float("inf") and bool(got2[0, 0, 6].isnan())
     keep = [i for i in range(dim) if i not in (5, 6)]
     assert torch.equal(got2[..., keep].double(), got[..., keep])
+
+
+@pytest.mark.parametrize("act,cache", [("f32", "f32"), ("bf16", "f32"), ("f32", "f16"), ("f32", "bf16"), ("f16", "f16"),
+                                       ("bf16", "bf16")])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+def test_one_key_gives_its_value(act, cache, dim):
+    """One visible key has the weight 1, so the result is its value: exactly in the 16-bit types; fp32 values enter as two tf32
+    parts of 11 bits, the upper one cut off, so that 13 of 24 bits are left, and the lower one rounded to the nearest 11 of
+    these: at most half of 2^-21 of the value's power of two is lost, 2^-22 of the value (and the result's own rounding)."""
+    import torch
+    ops = pkg("ops")
+    rng = np.random.default_rng(dim)
+    B, H, kv, ps = 40, 6, 2, 16
+    x = (rng.normal(size=(B, kv, ps, dim)) * 2.0 ** rng.integers(-12, 12, (B, kv, ps, dim))).astype(np.float32)
+    v = torch.from_numpy(x).cuda().to(_dt(cache))
+    k = torch.from_numpy(rng.normal(size=(B, kv, ps, dim)).astype(np.float32)).cuda().to(_dt(cache))
+    q = torch.from_numpy(rng.normal(size=(B, H, dim)).astype(np.float32)).cuda().to(_dt(act))
+    tables = torch.arange(B, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    for n, window in ((1, 0), (9, 1), (16, 1)):
+        lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+        got = ops.paged_attention(q, k, v, tables, lens, window=window).double()
+        want = v[:, :, n - 1].double().repeat_interleave(H // kv, 1)
+        tol = (2.0 ** -22 if cache == "f32" else 0.0) + (0.0 if act in (cache, "f32") else HALF[act])
+        assert bool(((got - want).abs() <= tol * want.abs()).all()), (n, float(((got - want).abs() / want.abs()).max()))
+
+
+@pytest.mark.parametrize("length", [1, 7, 100])
+def test_fp32_values_are_not_cut_to_one_side(length):
+    """Errors of a few keys' results have either sign: over 40 x 6 x 64 results of positive values, each off by at most 2^-22 and
+    by 2^-23 on average if all pointed one way, the mean error stays below 2^-24 of the value, the step of an fp32 rounding."""
+    import torch
+    ops = pkg("ops")
+    rng = np.random.default_rng(length)
+    B, H, ps, dim = 40, 6, 128, 64
+    v = torch.from_numpy(rng.uniform(1, 2, (B, H, ps, dim)).astype(np.float32)).cuda()
+    k = torch.zeros_like(v)
+    q = torch.zeros(B, H, dim, device="cuda")
+    tables = torch.arange(B, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    lens = torch.full((B,), length, dtype=torch.int32, device="cuda")
+    got = ops.paged_attention(q, k, v, tables, lens).double()
+    want = v[:, :, :length].double().mean(2)
+    assert abs(float(((got - want) / want).mean())) <= 2.0 ** -24
