@@ -12,9 +12,8 @@
 // take 41 us, 3.8 TB/s: the sum's arithmetic and the waits of the two readings bound it.)
 //
 // Precision: candidates of different hypotheses may lie closer than fp32 resolves, so the log-sum-exp
-// is held to about 2e-8.  Terms within e^-2 of the running maximum are evaluated in 64 bits; the
-// others, each below 1/7 of the sum, in fp32 (relative errors of about 2^-23, of either sign, which
-// over many terms cancel), 16 at a time, and added up in 64 bits.
+// is held to 2e-8 whatever the logits are: a term e^(x - m) is 2^(k + j/32) (1 + q), the power of two a 64-bit number
+// put together from a table and added up in 64 bits, q -- at most 0.022 -- a cubic in fp32 (see Terms).
 #include <algorithm>
 
 #include "paged.cuh"
@@ -44,7 +43,6 @@ typedef unsigned long long u64;
 
 constexpr int BW = 8, BT = BW * 32;
 constexpr int TILE = 512;      // logits of a warp's step, 16 a lane
-constexpr float NEAR = 2.f;
 constexpr int TILES_MOST = 1024;  // of a task (a multiple of the warps)
 
 // A task's (row's chunk's) result: sum of exp against the largest logit, that logit, then `beams`
@@ -113,12 +111,54 @@ __device__ __forceinline__ X merged(X x, const X& other) {
   return x;
 }
 
-// e^d for d <= 0; log2(e) in two parts, since an error of it would not cancel over the terms
-__device__ __forceinline__ float exp_far(float d) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(d, 1.925963033e-8f, d * 1.442695022f)));
-  return y;
+// e^(x - m) = 2^n (1 + q), n the multiple of 1/32 that x log2(e) - R rounds to, R the one that m log2(e) rounds to.  Adding
+// 1.5 * 2^18 to a number rounds it to such a multiple and leaves it in the low bits of the sum; n + R is exact, and what is
+// left of x log2(e) (log2(e) in two parts) comes out of one fused product.  Taking off what is left of m log2(e), the term
+// of m itself is 1, exactly, and what is left of x is within 2^-5: 2^f - 1 = f (C1 + C2 f + C3 f^2), whose f^4 term
+// is spread over the others as the Chebyshev polynomial has it (2.3e-9 off at most).  x is taken no lower than m - 80, which
+// adds less than 1e-29 to any sum (NaN goes there too).
+constexpr float LOG2E_HI = 1.442695022f, LOG2E_LO = 1.925963033e-8f;  // the nearest fp32 number and the rest's
+constexpr float STEPS = 393216.f;
+constexpr float MOST = 65536.f;  // |m| up to which R + n stays a number of the sum's kind
+constexpr double LN2 = 0.693147180559945309;
+constexpr float C1 = (float)LN2, C3 = (float)(LN2 * LN2 * LN2 / 6),
+                C2 = (float)(LN2 * LN2 / 2 + LN2 * LN2 * LN2 * LN2 / 24 * 0.75 / 1024);
+
+// two fp32 numbers in one instruction
+struct Two {
+  u64 v;
+};
+__device__ __forceinline__ Two two(float x, float y) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
 }
+__device__ __forceinline__ Two fma(Two x, Two y, Two z) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(x.v), "l"(y.v), "l"(z.v));
+  return r;
+}
+__device__ __forceinline__ Two add(Two x, Two y) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(x.v), "l"(y.v));
+  return r;
+}
+__device__ __forceinline__ Two mul(Two x, Two y) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(x.v), "l"(y.v));
+  return r;
+}
+__device__ __forceinline__ void apart(Two x, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x.v)); }
+
+struct Reference {  // what the terms need of m
+  float least, start, rest;
+  __device__ __forceinline__ explicit Reference(float m) {
+    const float r = fmaf(m, LOG2E_HI, STEPS) - STEPS;
+    least = m - 80.f;
+    start = STEPS - r;
+    rest = fmaf(m, LOG2E_LO, fmaf(m, LOG2E_HI, -r));
+  }
+};
 
 __device__ __forceinline__ float warp_top(float x) {  // of values that are not NaN
   float y;
@@ -128,12 +168,21 @@ __device__ __forceinline__ float warp_top(float x) {  // of values that are not 
 
 // The CTA's shared memory for a task.
 struct Scratch {
-  u64 held[BW][64];  // near terms (logit, how many << 32), then candidates on their way into a warp's list
+  u64 held[BW][64];  // candidates on their way into a warp's list
   u64 lists[BW][32];
   double ss[BW];
   float ms[BW];
   uint32_t tops[TILES_MOST];  // ordered maxima of the tiles (stop ids left out where they are none)
   uint32_t bar;
+  uint32_t power_hi[32], power_lo[32];  // 2^(j/32) in 64 bits, the upper word less j << 15 (what j adds to it in a sum)
+
+  __device__ __forceinline__ void fill() {
+    if (threadIdx.x < 32) {
+      const u64 p = __double_as_longlong(exp2(threadIdx.x / 32.0));
+      power_hi[threadIdx.x] = (uint32_t)(p >> 32) - (threadIdx.x << 15);
+      power_lo[threadIdx.x] = (uint32_t)p;
+    }
+  }
 };
 
 // One task by the whole CTA; false for rows whose logits do not count (finished hypotheses and those that
@@ -196,16 +245,6 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
   }
   u64* held = sh.held[warp];
   int count = 0;
-  auto add_near = [&]() {  // the first 32 of the near terms
-    __syncwarp();
-    const u64 u = lane < count ? held[lane] : 0ull, rest = lane + 32 < count ? held[lane + 32] : 0ull;
-    __syncwarp();
-    held[lane] = rest;
-    __syncwarp();
-    count = max(count - 32, 0);
-    const float y = __uint_as_float((uint32_t)u);
-    if (u) s += (double)(uint32_t)(u >> 32) * (y == m ? 1.0 : exp((double)y - (double)m));  // (m may be infinite)
-  };
   __syncthreads();  // (the last task's shared memory is done with)
   if (lane == 0) sh.ms[warp] = wtop;
   __syncthreads();
@@ -213,6 +252,45 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
   s = 0.0;
 #pragma unroll
   for (int w = 0; w < BW; ++w) m = fmaxf(m, sh.ms[w]);
+  Reference ref(m);
+  // a tile's terms against m
+  auto add_terms = [&]() {
+    double powers[2] = {0.0, 0.0};
+    Two rests = two(0.f, 0.f);
+    const Two start = two(ref.start, ref.start), rest = two(-ref.rest, -ref.rest), log_hi = two(LOG2E_HI, LOG2E_HI),
+              log_lo = two(LOG2E_LO, LOG2E_LO);
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      const Two y = two(fmaxf(x[e], ref.least), fmaxf(x[e + 1], ref.least)), n = fma(y, log_hi, start);
+      Two f = fma(y, log_hi, fma(n, two(-1.f, -1.f), start));
+      f = add(fma(y, log_lo, f), rest);
+      const Two q = mul(f, fma(fma(two(C3, C3), f, two(C2, C2)), f, two(C1, C1)));
+      float at[2], power[2];
+      apart(n, at[0], at[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t bits = __float_as_uint(at[i]), hi = sh.power_hi[bits & 31u] + (bits << 15), lo = sh.power_lo[bits & 31u];
+        powers[i] += __hiloint2double((int)hi, (int)lo);
+        // the same power in fp32, cut off: 2^-23 of 0.022
+        power[i] = __uint_as_float(__funnelshift_l(lo, hi, 3) + ((127u - 1023u) << 23));
+      }
+      rests = fma(two(power[0], power[1]), q, rests);
+    }
+    float even, odd;
+    apart(rests, even, odd);
+    s += (powers[0] + powers[1]) + (double)(even + odd);
+  };
+  // the same where m is infinite or beyond what n holds: one by one in 64 bits (terms below e^-64 left out)
+  auto add_terms_far = [&]() {
+#pragma unroll 1
+    for (int e = 0; e < 16; ++e) {
+      float y = 0.f;
+#pragma unroll
+      for (int f = 0; f < 16; ++f) y = f == e ? x[f] : y;
+      if (y == m) s += 1.0;
+      else if (y > m - 64.f) s += exp((double)y - (double)m);
+    }
+  };
   // too few maxima to bound the K-th logit: the lanes' serve (32 of 151936 tokens in chunks of 24 tiles: 46 us
   // instead of 63, where all were candidates)
   const bool few = tiles < K;
@@ -222,6 +300,7 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
     if (wtop > m) {
       if (s != 0.0) s *= exp((double)m - (double)wtop);
       m = wtop;
+      ref = Reference(m);
     }
     float mine_allowed = mine, allowed = wtop;
     if (early && v0 - lane < a.stop_hi && v0 - lane + TILE > a.stop_lo) {
@@ -236,43 +315,8 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
       best = tile == warp ? sorted(key) : merged(best, sorted(key));
     }
     if (m > -INFINITY) {
-      // the lane's largest, as long as it is near, leaves the tile for the queue of near terms: 32 of them
-      // take one evaluation in 64 bits
-      const float bound = m - NEAR;
-      for (unsigned who; (who = __ballot_sync(0xffffffffu, mine >= bound)) != 0;) {
-        const bool near = mine >= bound;
-        unsigned alike = 0;
-        if (near) {
-          float next = -INFINITY;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const bool it = x[e] == mine;
-            alike += it;
-            x[e] = it ? -INFINITY : x[e];
-            next = fmaxf(next, x[e]);
-          }
-          held[count + __popc(who & ((1u << lane) - 1u))] = (u64)alike << 32 | __float_as_uint(mine);
-          mine = next;
-        }
-        count += __popc(who);
-        if (count >= 32) add_near();
-      }
-      auto rest = [&]() -> float {
-        float t[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) t[e] = exp_far(x[e] - m);
-#pragma unroll
-        for (int w = 8; w > 0; w >>= 1)
-#pragma unroll
-          for (int e = 0; e < w; ++e) t[e] += t[e + w];
-        return t[0];
-      };
-      float r = rest();
-      if (__any_sync(0xffffffffu, r != r)) {
-        no_nan();
-        r = rest();
-      }
-      s += (double)r;
+      if (fabsf(m) < MOST) add_terms();
+      else add_terms_far();
     }
     tile += BW;
     if (tile < tiles) {
@@ -281,7 +325,6 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
       wtop = warp_top(mine);
     }
   }
-  if (count) add_near();
   if (few) sh.lists[warp][lane] = best;
   __syncthreads();
 
@@ -475,6 +518,7 @@ __device__ void choose(const BeamArgs& a, int64_t g, const char* work, Group& w)
 template <typename T>
 __global__ void __launch_bounds__(BT, 3) beam_scan_kernel(const BeamArgs a) {
   __shared__ Scratch sh;
+  sh.fill();
   dep_wait();
   dep_release();
   const int64_t row = blockIdx.y;
@@ -512,6 +556,7 @@ __global__ void __launch_bounds__(BT) beam_cluster_kernel(const BeamArgs a, int 
   __shared__ Scratch sh;
   __shared__ Group w;
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  sh.fill();
   dep_wait();
   dep_release();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA of the cluster runs
