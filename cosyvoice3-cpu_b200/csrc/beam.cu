@@ -8,8 +8,9 @@
 // keys in 64 bits.  A CTA reads its chunk of a row in tiles of 512 logits, once for the sum and the
 // tiles' maxima; the K-th largest of these maxima (with fewer than K tiles: of the lanes') bounds the K-th logit from
 // below, so only the tiles that reach it -- at most K, but for ties -- are read again (from L2) for candidates.  (Lists kept
-// while reading cost more than all the rest: 32 x 8 rows over 151936 tokens, 156 MB, took 94 us; so they
-// take 41 us, 3.8 TB/s: the sum's arithmetic and the waits of the two readings bound it.)
+// while reading cost more than all the rest.)  32 x 8 rows over 151936 tokens take 58 us (156 MB, 2.7 TB/s), with a
+// seventh of them finished, which are not read, 46 us (133 MB, 2.9 TB/s): the sum's 21 instructions a logit (their issue slots are
+// half full, waits on one another fill the rest) and the waits of the two readings bound it.
 //
 // Precision: candidates of different hypotheses may lie closer than fp32 resolves, so the log-sum-exp
 // is held to 2e-8 whatever the logits are: a term e^(x - m) is 2^(k + j/32) (1 + q), the power of two a 64-bit number
@@ -291,8 +292,8 @@ __device__ bool scan(const BeamArgs& a, int64_t row, int64_t chunk, Scratch& sh,
       else if (y > m - 64.f) s += exp((double)y - (double)m);
     }
   };
-  // too few maxima to bound the K-th logit: the lanes' serve (32 of 151936 tokens in chunks of 24 tiles: 46 us
-  // instead of 63, where all were candidates)
+  // too few maxima to bound the K-th logit: the lanes' serve (32 x 32 rows of 6761 tokens: 62 us instead of 120, where
+  // all were candidates)
   const bool few = tiles < K;
   u64 best = 0;
   for (int tile = warp; tile < tiles;) {
@@ -582,21 +583,25 @@ __global__ void __launch_bounds__(BT) beam_cluster_kernel(const BeamArgs a, int 
   if (rank == 0) choose(a, g, work, w);
 }
 
-// How a call is cut.  One launch with a cluster per group where every warp then walks few tiles -- 4, or
-// 16 if the groups' clusters fill the GPU --, else two, measured (one / two, fp32, us): 4 hypotheses of 6761
-// tokens 8.8 / 9.5, 32 x 8 of them 12.7 / 21.7; 4 of 50000 13.5 / 11.9, of 151936 24.0 / 11.9.
+// How a call is cut.  One launch with a cluster per group where each of its CTAs has one task, every warp then walks
+// at most 4 tiles for every hypothesis that a CTA stands for, and the clusters take at most three CTAs for two SMs; else two,
+// measured (one / two, fp32, us): 1 x 4 hypotheses of 6761 tokens 9.0 / 9.9, 16 x 8 of them 11.4 / 11.3, 100 x 1 9.1 / 10.2;
+// 1 x 16 21.5 / 14.8 (two tasks a CTA), 32 x 8 13.2 / 12.8 and 100 x 4 21.9 / 13.1 (more CTAs), 4 x 8 of 20000 13.7 / 13.8, 1 x 4
+// of 151936 27.2 / 11.7.
 //
 // Two launches: as many chunks as one wave of three CTAs on every SM takes, or one more that overshoots it by
-// at most a third of a chunk's share, since finished rows leave their CTAs early (32 x 8 rows of 151936, chunks
-// 1 / 2 / 3: 52 / 41 / 50 us with a seventh of the rows finished, 52 / 58 / 52 with none; 16 x 8, chunks 3 / 4:
-// 31 / 36 us).  But a chunk has 8 + 2 K tiles: the bar takes K maxima, and every chunk gives the second
-// launch K candidates (151936 tokens, such chunks against the wave's: 8 hypotheses 14.9 / 18.6 us, 32 of them
-// 32 / 46; half as many tiles: 14.7, 36; 16 + 3 K: 16.2, 38).
+// at most a third of a chunk's share: with every row live that costs nothing on average, and as soon as some are finished, whose CTAs
+// leave early, it is faster.  Rows of 151936, the wave's chunks / one more, none finished and a seventh finished: 112 rows
+// 33.8 / 33.5 and 33.3 / 28.7 us, 120 33.9 / 35.7 and 33.6 / 29.2, 152 43.4 / 42.0 and 42.3 / 34.1, 224 57.3 / 55.4 and 56.6 / 44.7,
+// 256 57.2 / 56.3 and 56.7 / 44.8; past that third 128 rows 33.9 / 38.3 and 33.8 / 29.3, 144 34.6 / 39.6 and 34.0 / 38.1.
+// But a chunk has 8 + 2 K tiles: the bar takes K maxima, and every chunk gives the second
+// launch K candidates (151936 tokens, half as many tiles / such chunks / 16 + 3 K: 4 hypotheses 10.8 / 11.4 / 13.1 us, 8 of them 15.5
+// / 14.4 / 15.8, 16 26.5 / 23.4 / 22.0, 32 34.9 / 31.9 / 38.1).
 struct Plan {
   int64_t cluster, chunks, tiles, bytes;  // cluster 0: two launches; bytes of results
 };
 constexpr int64_t TILES_LEAST = 8, TILES_BEAM = 2;
-constexpr int64_t CLUSTER = 8, CLUSTER_TILES = 4, CLUSTER_TILES_FULL = 16;  // (at most 32 tasks: 9 KB of results)
+constexpr int64_t CLUSTER = 8, CLUSTER_TILES = 4;
 
 Plan plan_of(int64_t groups, int64_t beams, int64_t vocab) {
   Plan p = {};
@@ -606,12 +611,13 @@ Plan plan_of(int64_t groups, int64_t beams, int64_t vocab) {
     p.tiles = (std::max<int64_t>(1, (row + chunks - 1) / chunks) + BW - 1) / BW * BW;
     p.chunks = (row + p.tiles - 1) / p.tiles;
   };
-  const int64_t most = groups * CLUSTER >= cv3::sm_count() ? CLUSTER_TILES_FULL : CLUSTER_TILES;
-  if (beams * ((row + BW - 1) / BW) <= CLUSTER * most) {
-    cut(std::max<int64_t>(1, CLUSTER / beams));
-    p.cluster = std::min<int64_t>(CLUSTER, beams * p.chunks);
+  if (beams <= CLUSTER && beams * ((row + BW - 1) / BW) <= CLUSTER * CLUSTER_TILES) {
+    cut(CLUSTER / beams);
+    p.cluster = beams * p.chunks;
     while (p.cluster & (p.cluster - 1)) ++p.cluster;  // a power of two
-  } else {
+    if (2 * groups * p.cluster > 3 * cv3::sm_count()) p.cluster = 0;
+  }
+  if (!p.cluster) {
     const int64_t rows = groups * beams, wave = 3 * cv3::sm_count();
     int64_t chunks = std::max<int64_t>(1, wave / rows);
     if (rows * (chunks + 1) <= wave + wave / (3 * (chunks + 1))) ++chunks;
