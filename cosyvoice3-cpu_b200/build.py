@@ -1,7 +1,8 @@
 """Compile ``csrc/*.cu`` into the in-tree ``libcv3cuda.so`` for sm_100a.
 
 ``csrc/bind/*.cpp`` become Python extension modules next to it, for hosts with PyTorch (the short
-way of its callers to some entries; the library itself needs no GPU framework).
+way of its callers to some entries; the library itself needs no GPU framework, and one that does not
+compile is a warning).
 
 Each translation unit is compiled by nvcc (in parallel, skipped when its object
 is newer than its sources and headers) and linked with ``nvcc -shared``.  The
@@ -18,6 +19,7 @@ import glob
 import os
 import subprocess
 import sys
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -50,28 +52,38 @@ def _compile(src: str, force: bool, hdr_time: float, extra) -> str:
 
 
 def bind_path(src: str) -> str:
-    return os.path.join(HERE, "_" + os.path.basename(src)[:-4] + ".so")
+    """The extension module of ``csrc/bind/*.cpp`` for the installed PyTorch and the running Python, whose versions are
+    in its name: one built against others is not taken for it."""
+    from importlib import metadata
+    try:
+        version = metadata.version("torch")
+    except metadata.PackageNotFoundError:
+        version = "none"
+    return os.path.join(HERE, "_%s.%s-torch-%s.so" % (os.path.basename(src)[:-4], sys.implementation.cache_tag, version))
 
 
-def _bind(src: str, force: bool) -> None:
-    """One extension module against the installed PyTorch (skipped where there is none)."""
+def _bind(src: str, force: bool) -> str:
+    """One extension module against the installed PyTorch (skipped where there is none).  Returns what the compiler
+    says where it fails: without the module its callers take their long way."""
     import importlib.util
     import sysconfig
     spec = importlib.util.find_spec("torch")
     if spec is None or not spec.submodule_search_locations:
-        return
+        return ""
     out, torch_dir = bind_path(src), spec.submodule_search_locations[0]
     header = os.path.join(INCLUDE, "cv3cuda.h")
     if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), os.path.getmtime(header)):
-        return
+        return ""
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=1",
            "-I", os.path.join(torch_dir, "include"), "-I", os.path.join(cuda, "include"),
            "-I", sysconfig.get_paths()["include"], src, "-o", out, "-L", os.path.join(torch_dir, "lib"),
            "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for {os.path.basename(src)}:\n{r.stdout}\n{r.stderr}")
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        return f"{os.path.basename(src)} was not built: {e}"
+    return "" if r.returncode == 0 else f"{os.path.basename(src)} was not built:\n{r.stdout}\n{r.stderr}"
 
 
 def build(force: bool = False, jobs: int = 0, extra=()) -> str:
@@ -84,13 +96,14 @@ def build(force: bool = False, jobs: int = 0, extra=()) -> str:
     with ThreadPoolExecutor(jobs) as ex:
         binds = [ex.submit(_bind, s, force) for s in sorted(glob.glob(os.path.join(CSRC, "bind", "*.cpp")))]
         objs = list(ex.map(lambda s: _compile(s, force, hdr, list(extra)), srcs))
-        for b in binds:
-            b.result()
+        said = [b.result() for b in binds]
     if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < max(os.path.getmtime(o) for o in objs):
         cmd = [NVCC, *ARCH, "-shared", "-o", LIB, *objs, "-lcudart"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    for text in filter(None, said):
+        warnings.warn(text)
     return LIB
 
 

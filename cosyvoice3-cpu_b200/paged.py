@@ -27,12 +27,14 @@ import importlib.util
 import math
 import os
 import struct
+import warnings
 from typing import NamedTuple, Optional, Tuple
 
 import numpy as np
 
 from . import _dev as D
-from ._lib import HERE, check, load
+from ._lib import check, load
+from .build import bind_path
 
 torch = D.torch
 
@@ -73,15 +75,19 @@ _bound = None   # the short way (csrc/bind/paged_bind.cpp), False where there is
 
 def _bind():
     """The extension module that takes plain calls of PyTorch tensors; False without PyTorch or without
-    the built module (every call then goes the long way, which gives the same results)."""
+    a module built against it (every call then goes the long way, which gives the same results)."""
     global _bound
     if _bound is None:
-        path = os.path.join(HERE, "_paged_bind.so")
         _bound = False
-        if torch is not None and os.path.exists(path):
-            spec = importlib.util.spec_from_file_location("_paged_bind", path)
-            mod = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(mod)
+        path = bind_path("paged_bind.cpp") if torch is not None else ""
+        if os.path.exists(path):
+            try:
+                spec = importlib.util.spec_from_file_location("_paged_bind", path)
+                mod = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(mod)
+            except (ImportError, OSError, SystemError) as e:
+                warnings.warn(f"{path} does not load, the paged operators take the long way: {e}")
+                return _bound
             lib = load()
             mod.setup(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in
                         ("cv3_paged_extend", "cv3_paged_append", "cv3_paged_attention", "cv3_paged_attention_workspace",

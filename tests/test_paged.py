@@ -375,3 +375,61 @@ def test_entry_for_shared_pages():
     assert give_back(release=0, parents=at, beams=2, rows=1 << 18) == U
     assert give_back(rows=1 << 20, cols=1 << 11, ld=1 << 11) == V and give_back(cols=1 << 28, ld=1 << 28) == V
     assert give_back(pages=1 << 31) == V
+
+
+# ---------------------------------------------------------------------------
+# the extension module is a short cut, nothing depends on it
+# ---------------------------------------------------------------------------
+
+def _fake_tree(monkeypatch, tmp_path, cxx):
+    """A source tree of one kernel file and one binding, compilers that only touch their output (or fail)."""
+    b = pkg("build")
+    (tmp_path / "csrc" / "bind").mkdir(parents=True)
+    (tmp_path / "csrc" / "a.cu").write_text("")
+    (tmp_path / "csrc" / "bind" / "x_bind.cpp").write_text("")
+    tool = tmp_path / "tool"
+    tool.write_text('#!/bin/sh\nwhile [ $# -gt 0 ]; do if [ "$1" = -o ]; then touch "$2"; fi; shift; done\n')
+    broken = tmp_path / "broken"
+    broken.write_text("#!/bin/sh\necho 'no headers here' >&2\nexit 1\n")
+    for f in (tool, broken):
+        f.chmod(0o755)
+    for name, value in (("HERE", str(tmp_path)), ("CSRC", str(tmp_path / "csrc")), ("BUILD", str(tmp_path / "_build")),
+                        ("LIB", str(tmp_path / "lib.so")), ("NVCC", str(tool))):
+        monkeypatch.setattr(b, name, value)
+    monkeypatch.setenv("CXX", str(tool if cxx else broken))
+    return b
+
+
+def test_a_binding_that_does_not_compile_leaves_the_library(monkeypatch, tmp_path):
+    b = _fake_tree(monkeypatch, tmp_path, False)
+    with pytest.warns(UserWarning, match="no headers here"):
+        lib = b.build()
+    assert os.path.exists(lib) and not [f for f in os.listdir(tmp_path) if "x_bind" in f]
+
+
+def test_a_binding_belongs_to_one_pytorch(monkeypatch, tmp_path):
+    """Its file is named after the PyTorch and the Python that it was built against; another one's is not taken for it."""
+    import importlib.metadata
+    b = _fake_tree(monkeypatch, tmp_path, True)
+    src = str(tmp_path / "csrc" / "bind" / "x_bind.cpp")
+    b.build()
+    here = b.bind_path(src)
+    assert os.path.exists(here) and os.path.basename(here).startswith("_x_bind.") and here.endswith(".so")
+    monkeypatch.setattr(importlib.metadata, "version", lambda name: "99.1+other")
+    other = b.bind_path(src)
+    assert other != here and not os.path.exists(other)
+    b.build()
+    assert os.path.exists(other) and os.path.exists(here)
+
+
+def test_a_binding_that_does_not_load_is_left_out(monkeypatch, tmp_path):
+    p = pkg("paged")
+    file = tmp_path / "_paged_bind.so"
+    file.write_bytes(b"not a library")
+    monkeypatch.setattr(p, "bind_path", lambda src: str(file), raising=False)
+    monkeypatch.setattr(p, "_bound", None)
+    with pytest.warns(UserWarning, match="_paged_bind"):
+        assert p._bind() is False
+    assert p._bind() is False                     # (and says so once)
+    with pytest.raises(ValueError, match="CUDA tensors are expected"):
+        p.paged_extend(_i32(2), _i32(2), _i32(2, 3), _i32(9), _i32(1), 16, 4)
