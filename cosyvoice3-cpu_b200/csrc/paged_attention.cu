@@ -26,10 +26,10 @@
 //    16-bit parts, whose 2^-16 (bf16) or 2^-22 (fp16) is far below the result's rounding (64 ragged requests: 377 instead of
 //    404 us).
 //
-// Measured: 64 requests of 1 to 16384 keys, 32 / 8 heads of 128, bf16 (2.15 GB): 344 us, 6.2 TB/s (390 us
-// when it runs on and on and the card's power limit lowers its clock); 32 of 64 to 1650 keys, 14 / 2
-// heads of 64, fp32 (28 MB): 14.5 us, of which the products, half of a step, and the chain length ->
-// table -> keys are most; one of 325 keys: 6.0 us.
+// Measured: 64 requests of 1 to 16384 keys, 32 / 8 heads of 128, bf16 (2.15 GB): 346 us, 6.2 TB/s (375 us
+// when it runs on and on and the card's power limit lowers its clock; fp16 355 us); 32 of 64 to 1650 keys, 14 / 2
+// heads of 64, fp32 (28 MB): 14.8 us, up to four steps of the longest request, each its loads' latency and its
+// products, behind the chain length -> table -> keys; one of 325 keys: 6.0 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -782,8 +782,8 @@ struct Plan {
 // CTA of a cluster has to do for the longest request, `even` what one of the wave has if all are that
 // long.  The join costs about two steps, and only even pieces gain from shorter requests, so clusters
 // take up to even + 2 steps and 8 at most.  Measured, cluster / even pieces (fp32, head dim 64, us): one
-// request of 800 keys 5.9 / 8.2, of 1600 7.8 / 8.2, of 3200 11.2 / 8.3; 8 requests of up to 1650 8.4 /
-// 9.6, 32 of them 14.4 / 15.3, 32 of up to 6000 36 / 30.
+// request of 325 keys 6.0 / 7.8, of 800 6.1 / 8.3, of 1600 8.0 / 8.3, of 3200 11.6 / 8.4; 8 requests of up to 1650
+// 8.6 / 9.6, 32 of them 14.8 / 15.5, 32 of up to 6000 38 / 31.
 constexpr int64_t CLUSTER_STEPS = 8, JOIN_STEPS = 2;
 
 Plan plan_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t d, int64_t size, int64_t max_len) {

@@ -33,7 +33,8 @@ class SamplingConfig:
 
     ``beams`` > 0 (device extension): beam search with that many hypotheses instead of sampling;
     ``length_penalty`` divides a hypothesis's score by its length to that power.  The token/text
-    ratios bound the length as in sampling, no stop id being taken below the minimum."""
+    ratios bound the length as in sampling, no stop id being taken below the minimum; the first token
+    is there when the search has ended."""
 
     def __init__(self, top_p: float = 0.8, top_k: int = 25, win_size: int = 10, tau_r: float = 0.1,
                  seed: Optional[int] = None, max_token_text_ratio: float = 20.0,
@@ -224,7 +225,8 @@ class CosyVoice3LM:
 
         Hypotheses end at a stop id (none below ``min_len`` tokens, one number or one per prompt) or at
         ``max_len`` tokens.  Their keys and values live in pages that hypotheses share (``cache_dtype``
-        float32, float16 or bfloat16); ``MAX_DECODE_BATCH // beams`` prompts are searched together.
+        float32, float16 or bfloat16); ``MAX_DECODE_BATCH // beams`` prompts are searched together.  Each
+        combination of sizes (lengths in steps of 256), page size, type and penalty keeps its engine.
         """
         B, K = len(prompts), int(beams)
         if B == 0:

@@ -363,8 +363,9 @@ def beam_select(logits, scores, counts, done, stop: Optional[Tuple[int, int]] = 
     keys in the order of the lower hypothesis and token.  A token in ``stop`` (first, end) finishes a
     hypothesis, and is no candidate while it has fewer than ``min_len[group]`` tokens; a finished one
     stays as it is (token 0).  A score of -inf marks a hypothesis that does not exist, as all but the
-    first at the start.  NaN logits are no candidates.  Keys are computed in 64 bits.  ``out`` gives the
-    :class:`BeamStep` its tensors, which may be the input state.
+    first at the start.  NaN logits are no candidates.  Keys are computed in 64 bits, from
+    log-sum-exps held to 2e-8; a hypothesis offers its ``beams`` largest logits (equal ones: the lowest tokens).
+    ``out`` gives the :class:`BeamStep` its tensors, which may be the input state.
     """
     if out is None and (_bound or _bind()):
         r = _bound.beam(logits, scores, counts, done, stop, min_len, length_penalty)
