@@ -236,7 +236,7 @@ def paged_extend(lens, new_lens, block_tables, free_pages, free_count, page_size
                            ("lens", out.lens, n), ("free_count", out.free_count, 1)):
             _ints(name, "out." + what, x, m)
         scratch = _new(lens, (n + 1,), D.I32)
-    if shares is not None and release is not None:
+    if shares is not None and release is not None and n:
         held, left = _new(lens, (n,), D.I32), _new(lens, (1,), D.I32)
         _give_back(name, d, shares, (tp, ld, cols), lens, n, page_size, free_pages, pc, left.data_ptr(), release=pr,
                    lens_out=held.data_ptr())
@@ -424,10 +424,10 @@ def paged_reorder(k_pages, v_pages, block_tables, parents, lens, shares=None, fr
     beam names any more go back to the stack, and :func:`paged_extend` with ``shares`` may release beams.
     Without them a page that is left stays out of the stack, and beams must not be released.
     """
-    if shares is None and free_pages is None and free_count is None and (_bound or _bind()) and _bound.reorder(k_pages, v_pages, block_tables, parents, lens):
+    counted = tuple(x for x in (shares, free_pages, free_count) if x is not None)
+    if not counted and (_bound or _bind()) and _bound.reorder(k_pages, v_pages, block_tables, parents, lens):
         return
     name = "paged_reorder"
-    counted = tuple(x for x in (shares, free_pages, free_count) if x is not None)
     if len(counted) not in (0, 3):
         raise ValueError(f"{name}: shares, free_pages and free_count go together")
     d = _device(name, k_pages, v_pages, block_tables, parents, lens, *counted)

@@ -239,3 +239,19 @@ print("numpy host ok")
 """
     r = subprocess.run([sys.executable, "-c", child, REPO], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "numpy host ok" in r.stdout, r.stderr[-2000:]
+
+
+def test_no_requests_and_no_groups():
+    """Empty batches are fine with counts as without."""
+    import torch
+    ops = pkg("ops")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    e, t, s, c = torch.zeros(0, **i32), torch.zeros(0, 3, **i32), torch.arange(4, **i32), torch.full((1,), 3, **i32)
+    sh = torch.zeros(4, **i32)
+    r = ops.paged_extend(e, e, t, s, c, 16, 2, release=e, shares=sh)
+    assert int(r.free_count) == 3 and r.slots.tolist() == [-1, -1] and r.offsets.tolist() == [0]
+    k = torch.zeros(4, 1, 16, 8, device="cuda")
+    ops.paged_reorder(k, k, t, torch.zeros(0, 4, **i32), e, sh, s, c)
+    one = torch.zeros(1, 3, **i32)
+    ops.paged_reorder(k, k, one, torch.zeros(1, 1, **i32), torch.full((1,), 33, **i32), sh, s, c)
+    assert int(c) == 3 and not bool(sh.any()) and s.tolist() == [0, 1, 2, 3]
