@@ -1,7 +1,8 @@
 // Beam search's choice: the best K of a group's K x V continuations.
 //
 // key(k, v) = (score_k + log_softmax(x_k)_v) / (count_k + 1)^alpha; a finished hypothesis offers
-// itself, unchanged, as its one candidate.  Equal keys go to the lowest k * V + v.
+// itself, unchanged, as its one candidate.  Equal keys go to the lower hypothesis, its larger logit (the 64
+// bits of a key may have no room for it under a huge score), the lower token.
 //
 // Bound by the logits' bytes.  Within a hypothesis the key grows with the logit, so a row gives its K
 // largest logits (lowest token on ties) and its log-sum-exp; the K * K candidates are then ordered by
@@ -71,20 +72,27 @@ __device__ __forceinline__ double unordered(u64 u) {
 __device__ __forceinline__ bool dead(float score) { return !(score > -INFINITY); }
 
 
-// A candidate of the choice: ordered key, then lowest k * V + v.
+// A candidate of the choice: ordered key, then lowest hypothesis, largest logit, lowest token.
 struct Cand {
   u64 key;
-  u64 tie;  // ~(k * V + v)
+  u64 place;
 };
+constexpr int TOKEN_BITS = 27;  // 5 bits of the hypothesis, 32 of the ordered logit, these
+constexpr uint32_t TOKENS = 1u << TOKEN_BITS;
+
+__device__ __forceinline__ u64 place_of(int k, uint32_t logit, uint32_t token) {
+  return (u64)(CV3_MAX_BEAMS - 1 - k) << (TOKEN_BITS + 32) | (u64)logit << TOKEN_BITS | (TOKENS - 1 - token);
+}
+static_assert(CV3_MAX_BEAMS <= 32, "a hypothesis's number takes 5 bits");
 
 __device__ __forceinline__ bool better(u64 x, u64 y) { return x > y; }
 __device__ __forceinline__ bool better(const Cand& x, const Cand& y) {
-  return x.key > y.key || (x.key == y.key && x.tie > y.tie);
+  return x.key > y.key || (x.key == y.key && x.place > y.place);
 }
 __device__ __forceinline__ u64 from_lane(u64 x, int lane) { return __shfl_sync(0xffffffffu, x, lane); }
-__device__ __forceinline__ Cand from_lane(const Cand& x, int lane) { return {from_lane(x.key, lane), from_lane(x.tie, lane)}; }
+__device__ __forceinline__ Cand from_lane(const Cand& x, int lane) { return {from_lane(x.key, lane), from_lane(x.place, lane)}; }
 __device__ __forceinline__ u64 across(u64 x, int j) { return __shfl_xor_sync(0xffffffffu, x, j); }
-__device__ __forceinline__ Cand across(const Cand& x, int j) { return {across(x.key, j), across(x.tie, j)}; }
+__device__ __forceinline__ Cand across(const Cand& x, int j) { return {across(x.key, j), across(x.place, j)}; }
 
 // The warp's lists: lane i holds the i-th best, zeros behind the last.  A bitonic network sorts 32
 // entries in 15 exchanges; two sorted lists give the 32 best of both in 5.
@@ -475,11 +483,14 @@ __device__ void choose(const BeamArgs& a, int64_t g, const char* work, Group& w)
     for (int r0 = 0; r0 < K; r0 += ranks) {
       const u64 next = scanned && r + ranks < K ? from[r + ranks] : 0ull;
       Cand c = {0, 0};
-      if (u)
-        c = Cand{ordered(continued(w.base[k], unordered((uint32_t)(u >> 32)), w.tops[k], w.lsum[k]) / w.norm[k]),
-                 ~(u64)(k * a.vocab + (uint32_t)~(uint32_t)u)};
-      else if (alone && r < K && r < a.vocab)  // a finished one itself, then what stands in where nothing is left
-        c = Cand{ordered(r == 0 && fin == 2 ? w.base[k] / w.norm[k] : -(double)INFINITY), ~(u64)(k * a.vocab + r)};
+      if (u) {
+        const uint32_t logit = (uint32_t)(u >> 32), token = ~(uint32_t)u;
+        c.key = ordered(continued(w.base[k], unordered(logit), w.tops[k], w.lsum[k]) / w.norm[k]);
+        c.place = place_of(k, c.key > ordered(-(double)INFINITY) ? logit : ordered(-INFINITY), token);
+      } else if (alone && r < K && r < a.vocab) {  // a finished one itself, then what stands in where nothing is left
+        c.key = ordered(r == 0 && fin == 2 ? w.base[k] / w.norm[k] : -(double)INFINITY);
+        c.place = place_of(k, ordered(-INFINITY), r);
+      }
       u = next;
       r += ranks;
       const Cand last = from_lane(list, K - 1);
@@ -501,9 +512,8 @@ __device__ void choose(const BeamArgs& a, int64_t g, const char* work, Group& w)
     __syncthreads();
   }
   if (warp || lane >= K) return;
-  const int64_t id = (int64_t)~list.tie;
-  const int k = (int)(id / a.vocab);
-  const int64_t v = id - (int64_t)k * a.vocab, to = g * K + lane;
+  const int k = CV3_MAX_BEAMS - 1 - (int)(list.place >> (TOKEN_BITS + 32));
+  const int64_t v = TOKENS - 1 - (uint32_t)(list.place & (TOKENS - 1)), to = g * K + lane;
   const bool fin = w.fins[k] == 2;
   // the key times the length's power is the score again (to the last bits of 64); the outputs may be
   // the inputs' own buffers, of which nothing is read any more
@@ -652,10 +662,11 @@ extern "C" int64_t cv3_beam_workspace(int64_t groups, int64_t beams, int64_t voc
 
 extern "C" int cv3_beam_select(const cv3_beam_params* p, void* stream) {
   CV3_REQUIRE(p && p->size == (int64_t)sizeof(*p), CV3_ERR_VALUE, "beam_select: bad parameter block");
-  CV3_REQUIRE(p->groups >= 0 && p->vocab > 0 && p->vocab <= 1 << 30 && p->ld >= p->vocab && p->stop_lo <= p->stop_hi,
+  CV3_REQUIRE(p->groups >= 0 && p->vocab > 0 && p->ld >= p->vocab && p->stop_lo <= p->stop_hi,
               CV3_ERR_VALUE, "beam_select: bad shape");
   CV3_REQUIRE(p->beams > 0 && p->beams <= CV3_MAX_BEAMS, CV3_ERR_UNSUPPORTED, "beam_select: %lld beams (1 to %d)",
               (long long)p->beams, CV3_MAX_BEAMS);
+  CV3_REQUIRE(p->vocab <= TOKENS, CV3_ERR_UNSUPPORTED, "beam_select: %lld tokens (up to 2^27)", (long long)p->vocab);
   CV3_REQUIRE(cv3p::type_ok(p->type), CV3_ERR_VALUE, "beam_select: unknown element type");
   // (lengths to that power stay finite and above 0 in 64 bits)
   CV3_REQUIRE(p->length_penalty >= -16.0 && p->length_penalty <= 16.0, CV3_ERR_VALUE,

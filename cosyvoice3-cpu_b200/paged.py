@@ -360,11 +360,11 @@ def beam_select(logits, scores, counts, done, stop: Optional[Tuple[int, int]] = 
     ``logits`` ``(groups, beams, vocab)``; ``scores`` (float32 sums of log-probabilities), ``counts``
     and ``done`` (int32) are ``(groups, beams)``.  A candidate's key is its new score divided by its
     length to the power ``length_penalty`` (-16 to 16); the ``beams`` best of all ``beams * vocab`` are kept, equal
-    keys in the order of the lower hypothesis and token.  A token in ``stop`` (first, end) finishes a
+    keys go to the lower hypothesis, its larger logit, the lower token.  A token in ``stop`` (first, end) finishes a
     hypothesis, and is no candidate while it has fewer than ``min_len[group]`` tokens; a finished one
     stays as it is (token 0).  A score of -inf marks a hypothesis that does not exist, as all but the
     first at the start.  NaN logits are no candidates.  Keys are computed in 64 bits, from
-    log-sum-exps held to 2e-8; a hypothesis offers its ``beams`` largest logits (equal ones: the lowest tokens).
+    log-sum-exps held to 2e-8.
     ``out`` gives the :class:`BeamStep` its tensors, which may be the input state.
     """
     if out is None and (_bound or _bind()):

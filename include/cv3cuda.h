@@ -499,10 +499,11 @@ int64_t cv3_paged_attention_workspace(int64_t batch, int64_t heads, int64_t kv_h
  * length_penalty); length_penalty is from -16 to 16.  Tokens of [stop_lo, stop_hi) end a hypothesis; they are no
  * candidates while counts[k] < min_len[g] (min_len may be NULL).  NaN logits, and
  * hypotheses with a score of -inf or NaN, give no candidates.  The `beams` best keys
- * in descending order (equal keys: the lowest k*vocab + v; -inf keys where too few
+ * in descending order (equal keys: the lower hypothesis, its larger logit, the lower token;
+ * -inf keys where too few
  * remain) give tokens, parents (k), the new scores (fp32), counts and done flags, which
- * may be the input buffers.  Keys are computed in 64 bits, from log-sum-exps held to 2e-8; a
- * hypothesis offers its `beams` largest logits (equal ones: the lowest tokens).
+ * may be the input buffers.  Keys are computed in 64 bits, from log-sum-exps held to 2e-8.
+ * vocab is at most 2^27.
  * workspace: cv3_beam_workspace() bytes, 8-byte aligned, nothing kept in it. */
 #define CV3_MAX_BEAMS 32
 typedef struct cv3_beam_params {

@@ -136,7 +136,11 @@ def beam(logits, scores, counts, done, stop=(0, 0), min_len=None, alpha=0.0):
                 lp[stop[0]:stop[1]] = -np.inf
             cum[k] = s + lp
             key[k] = cum[k] / (int(counts[g, k]) + 1) ** alpha
-        best = np.argsort(-key.ravel(), kind="stable")[:K]
+        # equal keys (a huge score leaves no room for the logits): the lower hypothesis, its larger logit, the lower token
+        x = np.where((key > -np.inf) & (np.asarray(done[g])[:, None] == 0), np.nan_to_num(logits[g].astype(np.float64), nan=-np.inf,
+                                                                                          posinf=np.inf, neginf=-np.inf), -np.inf)
+        rows, toks = np.divmod(np.arange(K * V), V)
+        best = np.lexsort((toks, -x.ravel(), rows, -key.ravel()))[:K]
         par, tok = best // V, best % V
         was = np.asarray(done[g])[par] != 0
         outs[0].append(np.where(was, 0, tok))

@@ -107,3 +107,27 @@ def test_certain_tokens_keep_their_score():
     y = np.broadcast_to(np.array([0.3, -17.25, 1e5, 88.0, -1e9, 3e38], np.float32)[None, :, None], (1, K, V))
     got = ops.beam_select(cu(y), cu(s), cu(zero), cu(zero))
     assert got.parents.tolist() == [[0] * K] and got.tokens.tolist() == [list(range(K))]
+
+
+@pytest.mark.parametrize("score", [-1e30, float(np.finfo(np.float32).min), -1e12])
+@pytest.mark.parametrize("K,V", [(2, 300), (4, 6761), (8, 6761), (8, 151936), (20, 40009), (32, 151936)])
+def test_scores_that_swallow_the_logits(score, K, V):
+    """Hypotheses marked by a huge negative score: all their keys are one number in 64 bits (or nearly), and the tokens are
+    still those of the largest logits, the lower hypothesis's first, however the call is cut."""
+    import torch
+    rng = np.random.default_rng(V + K)
+    x = rng.normal(size=(2, K, V)).astype(np.float32)
+    x[1] = np.round(x[1] * 2) / 2                     # (equal logits: the lowest tokens)
+    s = np.full((2, K), -np.inf, np.float32)
+    s[:, K // 2:] = score
+    x[0, 0, 5:], s[0, 0] = -np.inf, -1.0              # one hypothesis with five tokens
+    zero = np.zeros((2, K), np.int32)
+    want = ref.beam(x, s, zero, zero)
+    cu = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    got = pkg("ops").beam_select(cu(x), cu(s), cu(zero), cu(zero))
+    assert np.array_equal(got.parents.cpu().numpy(), want[1]) and np.array_equal(got.tokens.cpu().numpy(), want[0])
+    if score > -1e20:       # (64 bits next to 1e12 still tell logits 1.2e-4 apart, so other hypotheses may come first)
+        return
+    assert want[1][1].tolist() == [K // 2] * K
+    order = np.lexsort((np.arange(V), -x[1, K // 2].astype(np.float64)))
+    assert want[0][1].tolist() == order[:K].tolist()

@@ -433,3 +433,10 @@ def test_a_binding_that_does_not_load_is_left_out(monkeypatch, tmp_path):
     assert p._bind() is False                     # (and says so once)
     with pytest.raises(ValueError, match="CUDA tensors are expected"):
         p.paged_extend(_i32(2), _i32(2), _i32(2, 3), _i32(9), _i32(1), 16, 4)
+
+
+def test_vocabularies_past_27_bits():
+    L, p = pkg("_lib"), pkg("paged")
+    lib = L.load()
+    for vocab, code in ((1 << 27, 0), ((1 << 27) + 1, L.CV3_ERR_UNSUPPORTED)):
+        assert lib.cv3_beam_select(p._BEAM.pack(p._BEAM.size, 0, 0, vocab, 0, 4, vocab, *[0] * 13, 0.0), None) == code
