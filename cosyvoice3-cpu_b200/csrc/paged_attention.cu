@@ -26,7 +26,7 @@
 //    16-bit parts, whose 2^-16 (bf16) or 2^-22 (fp16) is far below the result's rounding (64 ragged requests: 377 instead of
 //    404 us).
 //
-// Measured: 64 requests of 1 to 16384 keys, 32 / 8 heads of 128, bf16 (2.15 GB): 346 us, 6.2 TB/s (375 us
+// Measured: 64 requests of 1 to 16384 keys, 32 / 8 heads of 128, bf16 (2.15 GB): 346 us, 6.2 TB/s (390 us
 // when it runs on and on and the card's power limit lowers its clock; fp16 355 us); 32 of 64 to 1650 keys, 14 / 2
 // heads of 64, fp32 (28 MB): 14.8 us, up to four steps of the longest request, each its loads' latency and its
 // products, behind the chain length -> table -> keys; one of 325 keys: 6.0 us.
